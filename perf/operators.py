@@ -313,14 +313,19 @@ def work(case):
 # ---------------------------------------------------------------------------------------------
 # the operators in 64 bits, from their definitions
 # ---------------------------------------------------------------------------------------------
+def _exact_pow2(e):
+    """2^e in float64 by its bits: the device's exp2 need not be exact."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
 def _exact_e4m3(x):
     """(values that x's rows are held as, their exponents) in float64."""
     x = x.double()
     a = x.abs().amax(-1)
     e = torch.ceil(torch.log2(a / 448) - 1e-6).clamp(-117, 119)       # 16-bit values: the next above 448 * 2^e is 7e-4 off
     e = e.masked_fill(a == 0, -117)
-    y = x / torch.exp2(e)[..., None]
-    step = torch.exp2(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -9))).clamp(min=-6) - 3)
+    y = x / _exact_pow2(e)[..., None]
+    step = _exact_pow2(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -9))).clamp(min=-6) - 3)
     return (torch.round(y / step) * step).clamp(-448, 448), e
 
 
@@ -333,7 +338,7 @@ def _exact_rows(s, case, z, h, count, name):
     x = flat[page, off, h] if case["layout"] == "NHD" else flat[page, h, off]
     if not case["quantised"]:
         return x.double()
-    scale = torch.exp2(s[name + "_scale"].view(torch.uint8)[page, h, off].double() - 127)
+    scale = _exact_pow2(s[name + "_scale"].view(torch.uint8)[page, h, off].long() - 127)
     return x.view(E4M3).double() * scale[:, None]
 
 
@@ -351,7 +356,7 @@ def exact(case, seed):
                 x = s[name][z][:, take].transpose(0, 1)                       # [count, H_kv, D]
                 if case["quantised"]:
                     x, e = _exact_e4m3(x)
-                    outs[2 + n].transpose(1, 2)[page, off] = torch.exp2(e)
+                    outs[2 + n].transpose(1, 2)[page, off] = _exact_pow2(e)
                 (outs[n] if case["layout"] == "NHD" else outs[n].transpose(1, 2))[page, off] = x.double()
         return tuple(outs)
     Z, H_kv, D = case["Z"], case["H_kv"], case["D"]
