@@ -24,13 +24,20 @@ EXPORTS = ("fst_version", "fst_status_string", "fst_packed_meta_bytes", "fst_pre
            "fst_attention_fwd_ref", "fst_attention_fwd_ref_static",
            "fst_attention_split_workspace_bytes", "fst_attention_fwd_splitkv", "fst_attention_fwd_gqa", "fst_dfs_order",
            "fst_attention_fwd_paged", "fst_selftest_wait_timeout", "fst_tree_topk_nodes",
-           "fst_build_tree_topk", "fst_attention_fwd_scatter", "fst_attention_tree_kernel")
+           "fst_build_tree_topk", "fst_attention_fwd_scatter", "fst_attention_tree_kernel",
+           "fst_cache_append", "fst_cache_read", "fst_attention_chunk_workspace_bytes", "fst_attention_chunk")
 STATIC_SCRATCH_BYTES = 512 * 1024
 
 _lib = None
 
 _i, _i64, _sz, _p, _f = C.c_int, C.c_int64, C.c_size_t, C.c_void_p, C.c_float
 _TENSOR_STRIDES = [_i64] * 12
+
+
+class PagedCache(C.Structure):
+    """``fst_paged_cache``"""
+    _fields_ = [("k_pool", _p), ("v_pool", _p), ("k_scale", _p), ("v_scale", _p), ("block_table", _p), ("table_stride", _i),
+                ("page_size", _i), ("n_pages", _i), ("stride_page", _i64), ("stride_row", _i64), ("stride_head", _i64)]
 
 
 def _declare(lib):
@@ -78,6 +85,15 @@ def _declare(lib):
     lib.fst_attention_fwd_ref.argtypes = ([_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i]
                                           + _TENSOR_STRIDES
                                           + [_i, _i, _f, _i, _i, _p, _sz, _p, _p])
+    cache = C.POINTER(PagedCache)
+    lib.fst_cache_append.restype = _i
+    lib.fst_cache_append.argtypes = [cache, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i] + [_i64] * 6 + [_i, _p, _p]
+    lib.fst_cache_read.restype = _i
+    lib.fst_cache_read.argtypes = [cache, _p, _p, _p, _i, _i, _i, _i] + [_i64] * 6 + [_i, _p, _p]
+    lib.fst_attention_chunk_workspace_bytes.restype = _sz
+    lib.fst_attention_chunk_workspace_bytes.argtypes = [cache, _i, _i, _i, _i, _i]
+    lib.fst_attention_chunk.restype = _i
+    lib.fst_attention_chunk.argtypes = [_p, _p, _p, cache, _p, _p, _i, _i, _i, _i, _i] + [_i64] * 6 + [_f, _i, _i, _p, _sz, _p, _p]
     lib.fst_attention_fwd_ref_static.restype = _i
     lib.fst_attention_fwd_ref_static.argtypes = ([_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i]
                                                  + _TENSOR_STRIDES + [_i, _i, _f, _i, _i, _p, _p])

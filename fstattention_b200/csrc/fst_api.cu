@@ -2,7 +2,9 @@
 #include <atomic>
 #include <cmath>
 #include <cstdio>
+#include <initializer_list>
 
+#include "fst_chunk.cuh"
 #include "fst_common.cuh"
 #include "fst_plan.h"
 
@@ -55,6 +57,31 @@ static int cuda_status(cudaError_t e) {
     if (e == cudaErrorInvalidConfiguration) return FST_ERR_TOO_LARGE;   // what a launcher returns when the sizes do not fit an SM
     return FST_ERR_CUDA;
 }
+
+// a cache's fields, once they are found to be what the kernels can take
+static int open_cache(CacheArgs &c, const fst_paged_cache *cache, int head_dim, int dtype) {
+    if (!cache || !cache->k_pool || !cache->v_pool || !cache->block_table || cache->table_stride <= 0 || cache->n_pages <= 0 ||
+        !cache->k_scale != !cache->v_scale)
+        return FST_ERR_INVALID_ARG;
+    if ((head_dim != 64 && head_dim != 128) || (dtype != FST_F16 && dtype != FST_BF16)) return FST_ERR_UNSUPPORTED;
+    const int ps = cache->page_size;
+    if (ps != 16 && ps != 32 && ps != 64 && ps != 128) return FST_ERR_UNSUPPORTED;
+    if ((long long)cache->table_stride * ps > 0x7fffffffLL - 256) return FST_ERR_TOO_LARGE;
+    const int64_t unit = cache->k_scale ? 16 : 8;         // elements of 16 bytes
+    if (!aligned16(cache->k_pool) || !aligned16(cache->v_pool) || !aligned16(cache->k_scale) || !aligned16(cache->v_scale) ||
+        cache->stride_page % unit || cache->stride_row % unit || cache->stride_head % unit)
+        return FST_ERR_ALIGNMENT;
+    c = CacheArgs{cache->k_pool, cache->v_pool, cache->k_scale, cache->v_scale, cache->block_table, cache->table_stride,
+                  ps == 16 ? 4 : ps == 32 ? 5 : ps == 64 ? 6 : 7, cache->n_pages, cache->stride_page, cache->stride_row, cache->stride_head};
+    return FST_OK;
+}
+static bool aligned_strides(std::initializer_list<int64_t> strides) {
+    for (int64_t s : strides)
+        if (s & 7) return false;
+    return true;
+}
+// rows of a row tile of the kernel that a chunk call goes to
+static int chunk_rows(int n_q, int group) { return (long long)n_q * group <= 16 ? 16 : 32; }
 }  // namespace fst
 
 using namespace fst;
@@ -453,6 +480,81 @@ int fst_attention_fwd_paged(const void *q, const void *k_tree, const void *v_tre
                        pool_stride_page, pool_stride_row, pool_stride_head};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return cuda_status(launch_prefix_umma_paged(a, pg, dtype, kv_splits, st));
+}
+
+int fst_cache_append(const fst_paged_cache *cache, const void *k, const void *v, const int32_t *start, const int32_t *lens,
+                     const int32_t *rows, int Z, int H_kv, int N, int M, int head_dim, int64_t k_stride_z, int64_t k_stride_h,
+                     int64_t k_stride_n, int64_t v_stride_z, int64_t v_stride_h, int64_t v_stride_n, int dtype, int32_t *status,
+                     void *stream) {
+    AppendArgs a = {};
+    if (!k || !v || !start || Z <= 0 || H_kv <= 0 || N <= 0 || M <= 0 || (!rows && M != N)) return FST_ERR_INVALID_ARG;
+    const int rc = open_cache(a.c, cache, head_dim, dtype);
+    if (rc != FST_OK) return rc;
+    if (!aligned16(k) || !aligned16(v) || !aligned_strides({k_stride_z, k_stride_h, k_stride_n, v_stride_z, v_stride_h, v_stride_n}))
+        return FST_ERR_ALIGNMENT;
+    a.k = k; a.v = v;
+    a.ks_z = k_stride_z; a.ks_h = k_stride_h; a.ks_n = k_stride_n;
+    a.vs_z = v_stride_z; a.vs_h = v_stride_h; a.vs_n = v_stride_n;
+    a.start = start; a.lens = lens; a.rows = rows;
+    a.Z = Z; a.H_kv = H_kv; a.N = N; a.M = M;
+    a.status = status;
+    return cuda_status(launch_cache_append(a, dtype, head_dim, static_cast<cudaStream_t>(stream)));
+}
+
+int fst_cache_read(const fst_paged_cache *cache, void *k, void *v, const int32_t *lens, int Z, int H_kv, int max_rows, int head_dim,
+                   int64_t k_stride_z, int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_z, int64_t v_stride_h,
+                   int64_t v_stride_n, int dtype, int32_t *status, void *stream) {
+    ReadArgs a = {};
+    if (!k || !v || !lens || Z <= 0 || H_kv <= 0 || max_rows <= 0) return FST_ERR_INVALID_ARG;
+    const int rc = open_cache(a.c, cache, head_dim, dtype);
+    if (rc != FST_OK) return rc;
+    if (!aligned16(k) || !aligned16(v) || !aligned_strides({k_stride_z, k_stride_h, k_stride_n, v_stride_z, v_stride_h, v_stride_n}))
+        return FST_ERR_ALIGNMENT;
+    a.k = k; a.v = v;
+    a.ks_z = k_stride_z; a.ks_h = k_stride_h; a.ks_n = k_stride_n;
+    a.vs_z = v_stride_z; a.vs_h = v_stride_h; a.vs_n = v_stride_n;
+    a.lens = lens;
+    a.Z = Z; a.H_kv = H_kv; a.M = max_rows;
+    a.status = status;
+    return cuda_status(launch_cache_read(a, dtype, head_dim, static_cast<cudaStream_t>(stream)));
+}
+
+size_t fst_attention_chunk_workspace_bytes(const fst_paged_cache *cache, int Z, int H, int H_kv, int n_q, int head_dim) {
+    ChunkArgs a = {};
+    if (Z <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || n_q <= 0 || open_cache(a.c, cache, head_dim, FST_F16) != FST_OK) return 0;
+    if (!chunk_splits(a, 128)) return 0;
+    return size_t(2) * chunk_ctas() * chunk_rows(n_q, H / H_kv) * (head_dim + 2) * sizeof(float);
+}
+
+int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cache *cache, const int32_t *kv_lens,
+                        const int32_t *q_lens, int Z, int H, int H_kv, int n_q, int head_dim, int64_t q_stride_z,
+                        int64_t q_stride_h, int64_t q_stride_n, int64_t o_stride_z, int64_t o_stride_h, int64_t o_stride_n,
+                        float sm_scale, int causal, int dtype, void *workspace, size_t workspace_bytes, int32_t *status, void *stream) {
+    ChunkArgs a = {};
+    if (!q || !o || !kv_lens || Z <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || n_q <= 0) return FST_ERR_INVALID_ARG;
+    if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return FST_ERR_INVALID_ARG;
+    const int rc = open_cache(a.c, cache, head_dim, dtype);
+    if (rc != FST_OK) return rc;
+    if ((long long)n_q * (H / H_kv) > 0x7fffffffLL - 1024) return FST_ERR_TOO_LARGE;
+    if (!aligned16(q) || !aligned16(o) || !aligned16(workspace) ||
+        !aligned_strides({q_stride_z, q_stride_h, q_stride_n, o_stride_z, o_stride_h, o_stride_n}))
+        return FST_ERR_ALIGNMENT;
+    const size_t need = fst_attention_chunk_workspace_bytes(cache, Z, H, H_kv, n_q, head_dim);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return FST_ERR_WORKSPACE;
+    a.q = q; a.o = o; a.lse = lse;
+    a.kv_lens = kv_lens; a.q_lens = q_lens;
+    a.Z = Z; a.H = H; a.H_kv = H_kv; a.group = H / H_kv; a.n_q = n_q;
+    a.qs_z = q_stride_z; a.qs_h = q_stride_h; a.qs_n = q_stride_n;
+    a.os_z = o_stride_z; a.os_h = o_stride_h; a.os_n = o_stride_n;
+    a.scale_log2 = sm_scale * 1.4426950408889634f;
+    a.causal = causal != 0;
+    a.part = static_cast<float *>(workspace);
+    a.status = status;
+    const int n_ctas = chunk_ctas();
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == FST_F16)
+        return cuda_status(head_dim == 64 ? launch_chunk_f16_d64(a, n_ctas, st) : launch_chunk_f16_d128(a, n_ctas, st));
+    return cuda_status(head_dim == 64 ? launch_chunk_bf16_d64(a, n_ctas, st) : launch_chunk_bf16_d128(a, n_ctas, st));
 }
 
 size_t fst_attention_ref_workspace_bytes(int n_meta_trees, int n_q, int block_m, int max_ancestors) {

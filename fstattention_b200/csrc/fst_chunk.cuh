@@ -1,0 +1,272 @@
+// Attention of a chunk of new tokens over a paged K/V cache: what its kernels share.
+//
+// The cache holds kv_lens[z] rows of sequence z, the chunk's own q_lens[z] among them as the last ones; query i stands
+// at position kv_len - q_len + i and attends to the rows up to it (causal) or to all of them:
+//     o = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m),   s_j = sm_scale log2(e) q . k_j,   m = max_j s_j
+// A query that sees no row has o = 0 and a log-sum-exp of -inf.
+//
+// The rows (query i, head g of the group) of a sequence and K/V head, r = i * group + g, are cut into row tiles, the keys
+// that a row tile sees into key tiles.  Lengths live on the device, so the work is divided there: all (z, K/V
+// head, row tile) items stand in one line, each as long as its key tiles, and every CTA of a grid that fills the GPU once
+// takes an equal piece of the line.  Any mix of lengths is balanced that way without the host knowing
+// them, a captured graph stays valid while sequences grow, and a CTA has at most two pieces that are not whole items:
+// the first and the last.  Those leave their rows in a workspace of fixed size; chunk_combine_kernel merges them
+// in the order of the CTAs, so the result does not depend on timing.
+#pragma once
+
+#include <type_traits>
+
+#include "fst_attention_mma.cuh"
+#include "fst_cache.cuh"
+
+namespace fst {
+
+struct ChunkArgs {
+    CacheArgs c;
+    const void *q;
+    void *o;
+    float *lse;
+    const int32_t *kv_lens, *q_lens;       // [Z], q_lens null: n_q everywhere
+    int Z, H, H_kv, group, n_q;
+    int64_t qs_z, qs_h, qs_n, os_z, os_h, os_n;
+    float scale_log2;                      // sm_scale * log2(e), positive
+    int causal;
+    float *part;                           // pieces: [2 CTAs][rows][D] sums, then [2 CTAs][rows] (exponent, sum)
+    int32_t *status;
+};
+
+// The line of work for row tiles of ROWS and key tiles of KEYS.
+template <int ROWS, int KEYS>
+struct ChunkLine {
+    const ChunkArgs &a;
+    __device__ __forceinline__ explicit ChunkLine(const ChunkArgs &args) : a(args) {}
+
+    __device__ __forceinline__ int kv_len(int z) const {
+        const int n = __ldg(a.kv_lens + z), most = a.c.width << a.c.page_shift;
+        return min(max(n, 0), most);
+    }
+    __device__ __forceinline__ int q_len(int z) const { return a.q_lens == nullptr ? a.n_q : min(max(__ldg(a.q_lens + z), 0), a.n_q); }
+    __device__ __forceinline__ int row_tiles(int ql) const { return (ql * a.group + ROWS - 1) / ROWS; }
+    // keys that the last row of a row tile sees
+    __device__ __forceinline__ int keys(int kv, int ql, int qt) const {
+        if (!a.causal) return kv;
+        const int last = min(((qt + 1) * ROWS - 1) / a.group, ql - 1);
+        return max(0, min(kv, kv - ql + last + 1));
+    }
+    // at least one key tile, so that rows which see nothing are written too
+    __device__ __forceinline__ static int tiles_of(int keys) { return max(1, (keys + KEYS - 1) / KEYS); }
+    // key tiles of one K/V head of a sequence
+    __device__ __forceinline__ long long head_tiles(int kv, int ql) const {
+        const int n = row_tiles(ql);
+        if (!a.causal) return (long long)n * tiles_of(kv);
+        long long s = 0;
+#pragma unroll 1
+        for (int qt = 0; qt < n; ++qt) s += tiles_of(keys(kv, ql, qt));
+        return s;
+    }
+};
+
+// A place in the line; the same in all lanes of a warp.
+template <int ROWS, int KEYS>
+struct ChunkCursor {
+    int z, h, qt, tile, tiles, keys, kv, ql, n_qt;
+
+    __device__ __forceinline__ void at_row_tile(const ChunkLine<ROWS, KEYS> &line) {
+        keys = line.keys(kv, ql, qt);
+        tiles = line.tiles_of(keys);
+    }
+    __device__ __forceinline__ void open(const ChunkLine<ROWS, KEYS> &line) {
+        kv = line.kv_len(z);
+        ql = line.q_len(z);
+        n_qt = line.row_tiles(ql);
+    }
+    // by a whole warp: length of the line
+    __device__ __forceinline__ static long long total(const ChunkLine<ROWS, KEYS> &line) {
+        const int lane = threadIdx.x & 31;
+        long long sum = 0;
+#pragma unroll 1
+        for (int z = lane; z < line.a.Z; z += 32) sum += line.head_tiles(line.kv_len(z), line.q_len(z));
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        return sum * line.a.H_kv;
+    }
+    // by a whole warp: to tile `pos` of the line, which has to be in it
+    __device__ __forceinline__ void seek(const ChunkLine<ROWS, KEYS> &line, long long pos) {
+        const int lane = threadIdx.x & 31;
+        long long head = 1;
+        z = 0;
+#pragma unroll 1
+        for (int z0 = 0; z0 < line.a.Z; z0 += 32) {
+            const long long mine = z0 + lane < line.a.Z ? line.head_tiles(line.kv_len(z0 + lane), line.q_len(z0 + lane)) : 0;
+            long long upto = mine * line.a.H_kv;
+#pragma unroll
+            for (int s = 1; s < 32; s *= 2) {
+                const long long below = __shfl_up_sync(0xffffffffu, upto, s);
+                if (lane >= s) upto += below;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, pos < upto);
+            if (past != 0u) {
+                const int f = __ffs(past) - 1;
+                z = z0 + f;
+                head = __shfl_sync(0xffffffffu, mine, f);
+                pos -= __shfl_sync(0xffffffffu, upto, f) - head * line.a.H_kv;
+                break;
+            }
+            pos -= __shfl_sync(0xffffffffu, upto, 31);
+        }
+        open(line);
+        h = int(pos / head);
+        pos -= h * head;
+        qt = 0;
+        at_row_tile(line);
+#pragma unroll 1
+        while (pos >= tiles) {
+            pos -= tiles;
+            ++qt;
+            at_row_tile(line);
+        }
+        tile = int(pos);
+    }
+    // to the next tile; the last tile of the line has none
+    __device__ __forceinline__ void next(const ChunkLine<ROWS, KEYS> &line) {
+        if (++tile < tiles) return;
+        tile = 0;
+        if (++qt == n_qt) {
+            qt = 0;
+            if (++h == line.a.H_kv) {
+                h = 0;
+                do {
+                    if (++z == line.a.Z) {
+                        z = line.a.Z - 1;
+                        return;
+                    }
+                    open(line);
+                } while (n_qt == 0);
+            }
+        }
+        at_row_tile(line);
+    }
+};
+
+// CTA i of n takes [first(i), first(i + 1)) of the line
+__device__ __forceinline__ long long chunk_first(long long total, int i, int n) { return total / n * i + min((long long)i, total % n); }
+
+// ---- values that are not finite where not every row of a tile attends to them.  The second product multiplies a masked
+// key's V by a probability of zero, and zero times NaN or infinity is NaN.  In key groups that some row does not see, such elements
+// are taken out of V, and what they do to the rows that see them is added at the end: a kernel that met none never looks again.
+
+// Of two 16-bit values only those that are finite and among the first n; whether one among the first n was not finite.
+template <typename T>
+__device__ __forceinline__ bool keep_finite(uint32_t &w, int n) {
+    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    if (n < 2) w = n < 1 ? 0u : w & 0xffffu;
+    bool met = false;
+    if ((w & E) == E) {
+        w &= 0xffff0000u;
+        met = true;
+    }
+    if ((w >> 16 & E) == E) {
+        w &= 0xffffu;
+        met = true;
+    }
+    return met;
+}
+// out[k] += the elements c0 + k of V in rows [from, to) of a sequence that are not finite
+template <typename T, int N>
+__device__ __forceinline__ void add_not_finite(const ChunkArgs &a, int z, int h, int from, int to, int c0, float (&out)[N]) {
+#pragma unroll 1
+    for (int key = from; key < to; ++key) {
+        const int idx = key >> a.c.page_shift, off = key & ((1 << a.c.page_shift) - 1);
+        const int page = a.c.table == nullptr ? z * a.c.width + idx : __ldg(a.c.table + size_t(z) * a.c.width + idx);
+        if (unsigned(page) >= unsigned(a.c.n_pages)) continue;
+        const T *v = static_cast<const T *>(a.c.v_pool) + page * a.c.stride_page + off * a.c.stride_row + h * a.c.stride_head + c0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const float x = float(v[k]);
+            out[k] += isfinite(x) ? 0.f : x;
+        }
+    }
+}
+
+// A launch that may become resident while the kernel ahead of it drains; the kernel waits before its first access.
+template <typename... P, typename... A>
+cudaError_t launch_serialised(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const A &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// The pieces of the item that CTA x's last piece begins, merged: a warp per row, eight rows of the item per block.
+template <typename T, int D, int ROWS, int KEYS>
+__global__ void __launch_bounds__(256)
+chunk_combine_kernel(const ChunkArgs a, int n_ctas) {
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    using Line = ChunkLine<ROWS, KEYS>;
+    using Cursor = ChunkCursor<ROWS, KEYS>;
+    constexpr int C = D / 32;                             // columns of a lane
+    const Line line(a);
+    const long long total = Cursor::total(line), lo = chunk_first(total, blockIdx.x, n_ctas), hi = chunk_first(total, blockIdx.x + 1, n_ctas);
+    if (hi == lo || hi == total) return;
+    Cursor it;
+    it.seek(line, hi - 1);
+    const long long start = hi - 1 - it.tile, end = start + it.tiles;
+    if (end == hi || start < lo) return;                  // it ends with the CTA, or began before it
+    const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int r = it.qt * ROWS + row, tok = r / a.group, head = it.h * a.group + (r - tok * a.group);
+    if (tok >= it.ql) return;
+    const float2 *stats = reinterpret_cast<const float2 *>(a.part + size_t(2) * n_ctas * ROWS * D);
+    float acc[C] = {}, top = -INFINITY, sum = 0.f;
+    // (both loads of a piece are asked for before the arithmetic of the one ahead)
+#pragma unroll 4
+    for (int c = blockIdx.x; c < n_ctas && (c == int(blockIdx.x) || chunk_first(total, c, n_ctas) < end); ++c) {
+        const size_t at = (size_t(2) * c + (c == int(blockIdx.x) ? 1 : 0)) * ROWS + row;
+        const float2 st = stats[at];
+        float v[C];
+        const float *from = a.part + at * D + lane * C;
+        if constexpr (C == 4) {
+            const float4 x = *reinterpret_cast<const float4 *>(from);
+            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        } else {
+            const float2 x = *reinterpret_cast<const float2 *>(from);
+            v[0] = x.x; v[1] = x.y;
+        }
+        const float now = fmaxf(top, st.x), to = now == -INFINITY ? 0.f : now;
+        const float w_old = fast_exp2(top - to), w = fast_exp2(st.x - to);
+        const bool none = st.x == -INFINITY && st.y == 0.f;              // the piece saw nothing
+        sum = none ? sum : sum * (top == -INFINITY ? 1.f : w_old) + st.y * (st.x == -INFINITY ? 1.f : w);
+#pragma unroll
+        for (int k = 0; k < C; ++k) acc[k] = none ? acc[k] : acc[k] * (top == -INFINITY ? 1.f : w_old) + v[k] * (st.x == -INFINITY ? 1.f : w);
+        top = now;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T *dst = static_cast<T *>(a.o) + it.z * a.os_z + head * a.os_h + tok * a.os_n + lane * C;
+    if constexpr (C == 4) *reinterpret_cast<uint2 *>(dst) = make_uint2(MmaTraits<T>::pack(acc[0] * inv, acc[1] * inv), MmaTraits<T>::pack(acc[2] * inv, acc[3] * inv));
+    else *reinterpret_cast<uint32_t *>(dst) = MmaTraits<T>::pack(acc[0] * inv, acc[1] * inv);
+    if (a.lse != nullptr && lane == 0) a.lse[(size_t(it.z) * a.H + head) * a.n_q + tok] = sum == 0.f ? -INFINITY : top + log2f(sum);
+}
+
+template <typename T, int D, int ROWS, int KEYS>
+cudaError_t launch_chunk_combine(const ChunkArgs &a, int n_ctas, cudaStream_t stream) {
+    return launch_serialised(chunk_combine_kernel<T, D, ROWS, KEYS>, dim3(n_ctas, ROWS / 8), dim3(256), 0, stream, a, n_ctas);
+}
+
+// CTAs of a call's line: one per SM (a workspace holds two pieces for each).
+inline int chunk_ctas() { return sm_count(); }
+// Whether any piece can be less than an item: not if all that the table can hold is one key tile.
+inline bool chunk_splits(const ChunkArgs &a, int keys) { return ((long long)a.c.width << a.c.page_shift) > keys; }
+
+cudaError_t launch_chunk_f16_d64(const ChunkArgs &, int, cudaStream_t);
+cudaError_t launch_chunk_f16_d128(const ChunkArgs &, int, cudaStream_t);
+cudaError_t launch_chunk_bf16_d64(const ChunkArgs &, int, cudaStream_t);
+cudaError_t launch_chunk_bf16_d128(const ChunkArgs &, int, cudaStream_t);
+
+}  // namespace fst

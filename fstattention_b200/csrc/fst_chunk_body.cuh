@@ -1,0 +1,19 @@
+// Dispatch of a chunk attention call for one type and head dimension (the .cu files instantiate it).
+#pragma once
+
+#include "fst_chunk_mma.cuh"
+
+namespace fst {
+
+template <typename T, int D>
+cudaError_t launch_chunk_t(const ChunkArgs &a, int n_ctas, cudaStream_t stream) {
+    constexpr bool bf16 = !std::is_same<T, __half>::value;
+    alignas(64) CUtensorMap tk, tv;
+    if (!make_pool_maps(&tk, &tv, a.c, bf16, D, a.H_kv, 16)) return cudaErrorNotSupported;
+    const bool one = a.n_q * a.group <= 16;
+    if (a.c.k_scale != nullptr)
+        return one ? launch_chunk_mma<T, D, true, 1>(a, tk, tv, n_ctas, stream) : launch_chunk_mma<T, D, true, 2>(a, tk, tv, n_ctas, stream);
+    return one ? launch_chunk_mma<T, D, false, 1>(a, tk, tv, n_ctas, stream) : launch_chunk_mma<T, D, false, 2>(a, tk, tv, n_ctas, stream);
+}
+
+}  // namespace fst

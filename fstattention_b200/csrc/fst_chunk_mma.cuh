@@ -1,0 +1,483 @@
+// Chunk attention of few rows on mma.sync: decode steps and drafted tokens.
+//
+// A tile is 16 or 32 rows and 128 keys; a call like that reads each key and value once for a handful of products, so HBM bounds it
+// and the tensor cores' rate does not matter.  What matters is bytes in flight and that nobody waits for anybody: each of the
+// eight warps has 16 keys of a tile, a ring of its own that TMA fills (boxes of 16 rows; a page holds 16 or more), and an accumulator of its
+// own for all rows, so the loop has no barrier among warps.  They meet once per item, to add up.
+//
+// 8-bit rows become matrix fragments in registers.  The order of the summed index is free as long as both operands agree, so
+// lane (g, t) of a K fragment takes the contiguous bytes D/4 t .. of key g, and Q is loaded in the same order;
+// of V it takes bytes D/8 g .. of its four keys, which only permutes the columns of the result.  A byte
+// becomes a 16-bit float by moving its seven low bits under the format's exponent: bf16 holds value * 2^-120, fp16
+// value * 2^-8 (subnormals included), and the missing power of two goes where a multiplication is made anyway: for K into Q (2^60,
+// bf16) and into the score's factor with the key's own scale, for V into the probability with the row's scale (2^60) and
+// the final division.  Probabilities and V are bf16 for an 8-bit cache under fp16 queries too: 2^e of a row and its probability need the
+// range, and V has four significant bits.
+#pragma once
+
+#include "fst_chunk.cuh"
+#include "fst_chunk_map.cuh"
+#include "fst_umma.cuh"
+
+namespace fst {
+
+template <int D, bool QUANT, int MT>
+struct ChunkMmaGeo {
+    static constexpr int WARPS = 8, KW = 16, KEYS = WARPS * KW, ROWS = 16 * MT;
+    static constexpr int TILE = KW * D * (QUANT ? 1 : 2);           // bytes of 16 rows of K or V
+    static constexpr int STAGES = (D == 128 ? 2 : 4) * (QUANT ? 2 : 1);
+    static constexpr int OFF_MERGE = WARPS * STAGES * 2 * TILE;     // [warp][16 rows][D + 4] fp32
+    static constexpr int OFF_STATS = OFF_MERGE + WARPS * 16 * (D + 4) * 4;      // [warp][ROWS] (exponent, sum)
+    static constexpr int OFF_SCALES = OFF_STATS + WARPS * ROWS * 8; // [warp][stage] 16 bytes of K, 16 of V
+    static constexpr int OFF_BAR = OFF_SCALES + WARPS * STAGES * 32;
+    static constexpr int BYTES = OFF_BAR + WARPS * STAGES * 8 + 16 + 1024;      // + alignment
+};
+
+constexpr float kTiny = 1.152921504606846976e18f;        // 2^60, half of what a bf16 made of an e4m3's bits lacks
+
+// four e4m3 bytes -> two pairs of 16-bit floats (bytes 0 and 2, bytes 1 and 3), smaller by 2^120 (bf16) or 2^8 (fp16)
+template <bool BF16>
+__device__ __forceinline__ void widen(uint32_t w, uint32_t &even, uint32_t &odd) {
+    constexpr int S = BF16 ? 4 : 1;
+    constexpr uint32_t M = BF16 ? 0x07f007f0u : 0x3f803f80u;
+    odd = (w & 0x80008000u) | ((w >> S) & M);
+    const uint32_t u = w << 8;
+    even = (u & 0x80008000u) | ((u >> S) & M);
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
+}
+// `bytes` (a multiple of 16) contiguous bytes of global memory into shared memory
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, int bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+template <typename T, int D, bool QUANT, int MT>
+__global__ void __launch_bounds__(256, 1)
+chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+    using G = ChunkMmaGeo<D, QUANT, MT>;
+    using MT_ = MmaTraits<T>;
+    using MP = MmaTraits<typename std::conditional<QUANT, __nv_bfloat16, T>::type>;      // of the second product
+    using Line = ChunkLine<G::ROWS, G::KEYS>;
+    using Cursor = ChunkCursor<G::ROWS, G::KEYS>;
+    constexpr bool BF16 = !std::is_same<T, __half>::value;
+    constexpr int KS = D / 16, ND = D / 8;               // steps of the first product, column tiles of the second
+    constexpr int HALF_BYTES = 16 * 128;                 // 16 rows of 64 columns of 16 bits
+
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t s_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    unsigned char *smem = smem_raw + (s_base - smem_u32(smem_raw));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t ring = s_base + warp * G::STAGES * 2 * G::TILE, bars = s_base + G::OFF_BAR + warp * G::STAGES * 8;
+    unsigned char *scales = smem + G::OFF_SCALES + warp * G::STAGES * 32;
+    if (lane == 0) {
+        for (int i = 0; i < G::STAGES; ++i) mbar_init(bars + i * 8, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    __syncwarp();
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+
+    const Line line(a);
+    const long long total = Cursor::total(line), first = chunk_first(total, blockIdx.x, gridDim.x);
+    const int n_tiles = int(chunk_first(total, blockIdx.x + 1, gridDim.x) - first);
+    if (n_tiles == 0) return;
+
+    // ---- loads, one 16-key group of this warp at a time; the page of the next one is looked up a group ahead
+    Cursor ld;
+    ld.seek(line, first);
+    Cursor me = ld;
+    int left = n_tiles, page = 0, slot_in = 0, in_flight = 0;
+    auto group_of = [&](const Cursor &c) { return c.tile * G::KEYS + warp * G::KW; };
+    auto look_up = [&]() {                                // the next group that has keys, if any
+#pragma unroll 1
+        while (left > 0 && group_of(ld) >= ld.keys) {
+            ld.next(line);
+            --left;
+        }
+        if (left > 0) {
+            const int idx = group_of(ld) >> a.c.page_shift;
+            page = a.c.table == nullptr ? ld.z * a.c.width + idx : __ldg(a.c.table + size_t(ld.z) * a.c.width + idx);
+        }
+    };
+    auto load = [&]() {                                   // requests it, then looks for the one behind
+        if (left <= 0) return;
+        if (lane == 0) {
+            const int off = group_of(ld) & ((1 << a.c.page_shift) - 1);
+            const uint32_t bar = bars + slot_in * 8, dst = ring + slot_in * 2 * G::TILE;
+            const bool bad = unsigned(page) >= unsigned(a.c.n_pages);    // the boxes then read as zeros
+            if (bad) report(a.status, FST_DEV_INDEX_RANGE, ld.z, group_of(ld));
+            if constexpr (QUANT) {
+                const size_t at = ((size_t(bad ? 0 : page) * a.H_kv + ld.h) << a.c.page_shift) + off;
+                const uint4 zero = make_uint4(0, 0, 0, 0);
+                uint4 *sc = reinterpret_cast<uint4 *>(scales + slot_in * 32);
+                if (bad) {
+                    sc[0] = sc[1] = zero;
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                }
+                mbar_arrive_expect_tx(bar, 2 * G::TILE + (bad ? 0 : 32));
+                if (!bad) {
+                    bulk_load(smem_u32(sc), a.c.k_scale + at, 16, bar);
+                    bulk_load(smem_u32(sc + 1), a.c.v_scale + at, 16, bar);
+                }
+                tma_load_4d(dst, &tm_k, 0, off, ld.h, page, bar);
+                tma_load_4d(dst + G::TILE, &tm_v, 0, off, ld.h, page, bar);
+            } else {
+                mbar_arrive_expect_tx(bar, 2 * G::TILE);
+#pragma unroll
+                for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(dst + hf * HALF_BYTES, &tm_k, hf * 64, off, ld.h, page, bar);
+#pragma unroll
+                for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(dst + G::TILE + hf * HALF_BYTES, &tm_v, hf * 64, off, ld.h, page, bar);
+            }
+        }
+        if (++slot_in == G::STAGES) slot_in = 0;
+        ++in_flight;
+        ld.next(line);
+        --left;
+        look_up();
+    };
+    look_up();
+#pragma unroll 1
+    for (int i = 0; i < G::STAGES; ++i) load();
+
+    // ---- products
+    const float c2 = a.scale_log2 * (QUANT ? (BF16 ? kTiny : 256.f) : 1.f);
+    uint32_t qf[MT][KS][4];
+    float acc[MT][ND][4], m[MT][2], l[MT][2];
+    int limit[MT][2], lim_first = 0, slot = 0;
+    uint32_t parity = 0;
+    bool poisoned = false, alive = true;                  // a V that is not finite was met where not every row attends to it
+
+#pragma unroll 1
+    for (int i = 0; i < n_tiles; ++i) {
+        if (i == 0 || me.tile == 0) {                     // a new item: its rows of Q
+            if (tid == 0 && me.h == 0 && me.qt == 0 && (me.kv != __ldg(a.kv_lens + me.z) || (a.q_lens != nullptr && me.ql != __ldg(a.q_lens + me.z))))
+                report(a.status, FST_DEV_INDEX_RANGE, me.z, __ldg(a.kv_lens + me.z));
+            poisoned = false;
+            lim_first = a.causal ? min(me.kv, me.kv - me.ql + me.qt * G::ROWS / a.group + 1) : me.kv;
+#pragma unroll
+            for (int x = 0; x < MT; ++x) {
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    const int r = me.qt * G::ROWS + x * 16 + hh * 8 + g, tok = r / a.group;
+                    const bool real = tok < me.ql;
+                    limit[x][hh] = !real ? 0 : a.causal ? min(me.kv, me.kv - me.ql + tok + 1) : me.kv;
+                    m[x][hh] = -INFINITY;
+                    l[x][hh] = 0.f;
+                    const T *src = static_cast<const T *>(a.q) + me.z * a.qs_z + (me.h * a.group + (r - tok * a.group)) * a.qs_h + tok * a.qs_n;
+                    if constexpr (QUANT) {                // D / 4 contiguous values of the row, in the order of the K bytes
+#pragma unroll
+                        for (int s = 0; s < KS / 2; ++s) {
+                            uint4 w = real ? __ldg(reinterpret_cast<const uint4 *>(src + t * (D / 4) + s * 8)) : make_uint4(0, 0, 0, 0);
+                            if constexpr (BF16) {
+                                const __nv_bfloat162 f = __float2bfloat162_rn(kTiny);
+                                uint32_t *p = &w.x;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    const __nv_bfloat162 y = __hmul2(*reinterpret_cast<__nv_bfloat162 *>(p + k), f);
+                                    p[k] = *reinterpret_cast<const uint32_t *>(&y);
+                                }
+                            }
+                            // widen() gives bytes (0, 2) and (1, 3): Q's pairs to match
+                            qf[x][2 * s][hh] = __byte_perm(w.x, w.y, 0x5410);
+                            qf[x][2 * s][2 + hh] = __byte_perm(w.x, w.y, 0x7632);
+                            qf[x][2 * s + 1][hh] = __byte_perm(w.z, w.w, 0x5410);
+                            qf[x][2 * s + 1][2 + hh] = __byte_perm(w.z, w.w, 0x7632);
+                        }
+                    } else {
+#pragma unroll
+                        for (int s = 0; s < KS; ++s) {
+                            qf[x][s][hh] = real ? __ldg(reinterpret_cast<const uint32_t *>(src + s * 16 + 2 * t)) : 0u;
+                            qf[x][s][2 + hh] = real ? __ldg(reinterpret_cast<const uint32_t *>(src + s * 16 + 8 + 2 * t)) : 0u;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < ND; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[x][n][k] = 0.f;
+            }
+        }
+
+        const int key0 = group_of(me);
+        if (key0 < me.keys && alive) {
+            const uint32_t k_at = ring + slot * 2 * G::TILE, v_at = k_at + G::TILE;
+            const bool edge = key0 + G::KW > lim_first;   // not every row attends to all of the group
+            alive = __all_sync(0xffffffffu, mbar_wait(bars + slot * 8, parity, a.status, blockIdx.x));
+            float s[MT][2][4];
+#pragma unroll
+            for (int x = 0; x < MT; ++x)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[x][n][k] = 0.f;
+            float ks[2][2], vs[2][2];                     // scales of my four keys: 8 n + 2 t + k
+            if constexpr (QUANT) {
+                const uint16_t *sc = reinterpret_cast<const uint16_t *>(scales + slot * 32);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const uint32_t bk = sc[4 * n + t], bv = sc[8 + 4 * n + t];
+                    ks[n][0] = e8m0_value(bk & 255u) * c2;
+                    ks[n][1] = e8m0_value(bk >> 8) * c2;
+                    vs[n][0] = e8m0_value(bv & 255u) * kTiny;
+                    vs[n][1] = e8m0_value(bv >> 8) * kTiny;
+                }
+                // K: key 8 n + g, bytes D/4 t ..
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int row = 8 * n + g;
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c) {    // 16 bytes: four steps
+                        const int chunk = D == 128 ? ((2 * t + c) ^ (row & 7)) : (t ^ ((row >> 1) & 3));
+                        const uint4 b = lds128(k_at + row * D + chunk * 16);
+                        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t b0, b1;
+                            widen<BF16>(w[k], b0, b1);
+#pragma unroll
+                            for (int x = 0; x < MT; ++x) MT_::mma(s[x][n], qf[x][c * 4 + k], b0, b1);
+                        }
+                    }
+                }
+            } else {
+                const int row = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+                for (int st = 0; st < KS; ++st) {
+                    const int chunk = 2 * st + ((lane >> 3) & 1);
+                    uint32_t b[4];
+                    ldmatrix_x4(b, k_at + (chunk >> 3) * HALF_BYTES + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+#pragma unroll
+                    for (int x = 0; x < MT; ++x) {
+                        MT_::mma(s[x][0], qf[x][st], b[0], b[1]);
+                        MT_::mma(s[x][1], qf[x][st], b[2], b[3]);
+                    }
+                }
+            }
+            // ---- softmax of the group: scores in base-2 units against the row's running maximum
+            uint32_t pf[MT][4];
+#pragma unroll
+            for (int x = 0; x < MT; ++x) {
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float v = s[x][n][k] * (QUANT ? ks[n][k & 1] : c2);
+                        if (edge && key0 + 8 * n + 2 * t + (k & 1) >= limit[x][k >> 1]) v = -INFINITY;
+                        s[x][n][k] = v;
+                        mx[k >> 1] = fmaxf(mx[k >> 1], v);
+                    }
+                bool up = false;
+                float alpha[2], ref[2];
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 1));
+                    mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 2));
+                    const float now = fmaxf(m[x][hh], mx[hh]);
+                    up = up || now > m[x][hh];
+                    alpha[hh] = now == -INFINITY ? 1.f : fast_exp2(m[x][hh] - now);
+                    m[x][hh] = now;
+                    ref[hh] = now == -INFINITY ? 0.f : now;
+                }
+                if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+                    for (int n = 0; n < ND; ++n) {
+                        acc[x][n][0] *= alpha[0];
+                        acc[x][n][1] *= alpha[0];
+                        acc[x][n][2] *= alpha[1];
+                        acc[x][n][3] *= alpha[1];
+                    }
+                    l[x][0] *= alpha[0];
+                    l[x][1] *= alpha[1];
+                }
+                float p[2][4];
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        p[n][k] = fast_exp2(s[x][n][k] - ref[k >> 1]);
+                        l[x][k >> 1] += p[n][k];
+                        // the row's scale; what a masked key holds, NaN too, stays out
+                        if constexpr (QUANT) p[n][k] = s[x][n][k] == -INFINITY ? 0.f : p[n][k] * vs[n][k & 1];
+                    }
+                pf[x][0] = MP::pack(p[0][0], p[0][1]);
+                pf[x][1] = MP::pack(p[0][2], p[0][3]);
+                pf[x][2] = MP::pack(p[1][0], p[1][1]);
+                pf[x][3] = MP::pack(p[1][2], p[1][3]);
+            }
+            // ---- second product
+            if constexpr (QUANT) {
+                // V: keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9, bytes D/8 g ..: column tile j holds columns D/8 n + j
+                uint32_t w[4][D / 32];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int row = 2 * t + (k & 1) + (k >> 1) * 8;
+                    if constexpr (D == 128) {
+                        const uint4 b = lds128(v_at + row * 128 + ((g ^ (row & 7)) << 4));
+                        w[k][0] = b.x; w[k][1] = b.y; w[k][2] = b.z; w[k][3] = b.w;
+                    } else {
+                        const uint2 b = lds64(v_at + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8);
+                        w[k][0] = b.x; w[k][1] = b.y;
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                    for (int hl = 0; hl < 2; ++hl) {      // two column tiles from bytes 2 hl, 2 hl + 1 of either key
+                        uint32_t b0[2], b1[2];
+                        widen<true>(__byte_perm(w[0][c], w[1][c], hl ? 0x7632 : 0x5410), b0[0], b0[1]);
+                        widen<true>(__byte_perm(w[2][c], w[3][c], hl ? 0x7632 : 0x5410), b1[0], b1[1]);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+#pragma unroll
+                            for (int x = 0; x < MT; ++x) MP::mma(acc[x][c * 4 + hl * 2 + k], pf[x], b0[k], b1[k]);
+                    }
+            } else {
+                const int row = (lane & 7) + ((lane >> 3) & 1) * 8, here = min(me.kv - key0, G::KW);
+#pragma unroll
+                for (int j = 0; j < ND / 2; ++j) {
+                    const int chunk = 2 * j + (lane >> 4);
+                    uint32_t b[4];
+                    ldmatrix_x4_trans(b, v_at + (chunk >> 3) * HALF_BYTES + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+                    if (edge) {                           // zero times what is not finite would be NaN
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) poisoned = keep_finite<T>(b[k], here - (k & 1) * 8 - 2 * t) || poisoned;
+                    }
+#pragma unroll
+                    for (int x = 0; x < MT; ++x) {
+                        MP::mma(acc[x][2 * j], pf[x], b[0], b[1]);
+                        MP::mma(acc[x][2 * j + 1], pf[x], b[2], b[3]);
+                    }
+                }
+            }
+            __syncwarp();                                 // everybody is done with the slot
+            --in_flight;
+            if (alive) load();
+            if (++slot == G::STAGES) {
+                slot = 0;
+                parity ^= 1u;
+            }
+        }
+
+        if (me.tile + 1 == me.tiles || i + 1 == n_tiles) {
+            // ---- the warps' results of this piece: 16 rows at a time through shared memory
+            const bool from_start = i >= me.tile, whole = from_start && me.tile + 1 == me.tiles;
+            const bool bad = __syncthreads_or(poisoned) != 0;
+            float2 *stats = reinterpret_cast<float2 *>(smem + G::OFF_STATS);
+            float *rows = reinterpret_cast<float *>(smem + G::OFF_MERGE);
+#pragma unroll
+            for (int x = 0; x < MT; ++x) {
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    float sum = l[x][hh];
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    if (t == 0) stats[warp * G::ROWS + x * 16 + hh * 8 + g] = make_float2(m[x][hh], sum);
+                    float *to = rows + (warp * 16 + hh * 8 + g) * (D + 4);
+                    if constexpr (QUANT) {
+#pragma unroll
+                        for (int j = 0; j < ND; j += 4)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+                                *reinterpret_cast<float4 *>(to + (2 * t + k) * (D / 8) + j) =
+                                    make_float4(acc[x][j][2 * hh + k], acc[x][j + 1][2 * hh + k], acc[x][j + 2][2 * hh + k], acc[x][j + 3][2 * hh + k]);
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < ND; ++n)
+                            *reinterpret_cast<float2 *>(to + n * 8 + 2 * t) = make_float2(acc[x][n][2 * hh], acc[x][n][2 * hh + 1]);
+                    }
+                }
+                __syncthreads();
+                // sixteen threads a row, D / 16 columns each
+                const int row = tid >> 4, c0 = (tid & 15) * (D / 16);
+                float top = -INFINITY, sum = 0.f, out[D / 16];
+#pragma unroll
+                for (int w = 0; w < G::WARPS; ++w) top = fmaxf(top, stats[w * G::ROWS + x * 16 + row].x);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) out[k] = 0.f;
+#pragma unroll
+                for (int w = 0; w < G::WARPS; ++w) {
+                    const float2 st = stats[w * G::ROWS + x * 16 + row];
+                    if (st.x == -INFINITY && st.y == 0.f) continue;              // saw nothing
+                    const float f = top == -INFINITY ? 1.f : fast_exp2(st.x - top);
+                    sum += st.y * f;
+#pragma unroll
+                    for (int k = 0; k < D / 16; k += 4) {
+                        const float4 v = *reinterpret_cast<const float4 *>(rows + (w * 16 + row) * (D + 4) + c0 + k);
+                        out[k] += v.x * f;
+                        out[k + 1] += v.y * f;
+                        out[k + 2] += v.z * f;
+                        out[k + 3] += v.w * f;
+                    }
+                }
+                const int r = me.qt * G::ROWS + x * 16 + row, tok = r / a.group, head = me.h * a.group + (r - tok * a.group);
+                if (QUANT) {
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) out[k] *= kTiny;
+                }
+                if (bad && tok < me.ql) {
+                    // keys of this piece whose groups were looked through, as far as my row sees them
+                    const int keys = a.causal ? min(me.kv, me.kv - me.ql + tok + 1) : me.kv;
+                    add_not_finite<T, D / 16>(a, me.z, me.h, max(max(lim_first, 0) & ~(G::KW - 1), max(0, me.tile - i) * G::KEYS),
+                                              min(keys, (me.tile + 1) * G::KEYS), c0, out);
+                }
+                if (whole) {
+                    if (tok < me.ql) {
+                        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                        T *dst = static_cast<T *>(a.o) + me.z * a.os_z + head * a.os_h + tok * a.os_n + c0;
+                        uint32_t w[D / 32];
+#pragma unroll
+                        for (int k = 0; k < D / 32; ++k) w[k] = MT_::pack(out[2 * k] * inv, out[2 * k + 1] * inv);
+                        if constexpr (D == 128) *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+                        else *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+                        if (a.lse != nullptr && c0 == 0) a.lse[(size_t(me.z) * a.H + head) * a.n_q + tok] = sum == 0.f ? -INFINITY : top + log2f(sum);
+                    }
+                } else {
+                    const size_t at = (size_t(2) * blockIdx.x + (from_start ? 1 : 0)) * G::ROWS + x * 16 + row;
+#pragma unroll
+                    for (int k = 0; k < D / 16; k += 4)
+                        *reinterpret_cast<float4 *>(a.part + at * D + c0 + k) = make_float4(out[k], out[k + 1], out[k + 2], out[k + 3]);
+                    if (c0 == 0) reinterpret_cast<float2 *>(a.part + size_t(2) * gridDim.x * G::ROWS * D)[at] = make_float2(top, sum);
+                }
+                __syncthreads();
+            }
+        }
+        me.next(line);
+    }
+    if (!alive) {                                         // a wait ran out: nothing may land after this CTA has left
+#pragma unroll 1
+        for (; in_flight > 0; --in_flight) {
+            mbar_wait(bars + slot * 8, parity, a.status, blockIdx.x);
+            if (++slot == G::STAGES) {
+                slot = 0;
+                parity ^= 1u;
+            }
+        }
+    }
+}
+
+template <typename T, int D, bool QUANT, int MT>
+static cudaError_t launch_chunk_mma(const ChunkArgs &a, const CUtensorMap &tk, const CUtensorMap &tv, int n_ctas, cudaStream_t stream) {
+    using G = ChunkMmaGeo<D, QUANT, MT>;
+    static_assert(G::BYTES <= 227 * 1024, "one CTA's shared memory");
+    static DeviceOnce configured;
+    const cudaError_t ce = configured.run([&] {
+        return cudaFuncSetAttribute(chunk_mma_kernel<T, D, QUANT, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::BYTES);
+    });
+    if (ce != cudaSuccess) return ce;
+    const cudaError_t e = launch_serialised(chunk_mma_kernel<T, D, QUANT, MT>, dim3(n_ctas), dim3(256), G::BYTES, stream, a, tk, tv);
+    if (e != cudaSuccess || !chunk_splits(a, G::KEYS)) return e;
+    return launch_chunk_combine<T, D, G::ROWS, G::KEYS>(a, n_ctas, stream);
+}
+
+}  // namespace fst

@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <atomic>
+#include <climits>
 #include <cmath>
 #include <mutex>
 #include <optional>
@@ -403,6 +404,223 @@ PyObject *attention_paged(PyObject *const *a, Py_ssize_t n) {
     return results(c);
 }
 
+// ---- paged K/V cache ------------------------------------------------------------------------------
+// strides (elements) of the first three dimensions; that of a dimension of one says nothing and may be anything
+int64_t stride_of(const at::Tensor &t, int i) { return t.size(i) == 1 ? t.size(3) : t.stride(i); }
+#define FST_ROW_STRIDES(t) stride_of(t, 0), stride_of(t, 1), stride_of(t, 2)
+// The cache's tensors, checked: pools [n_pages, page_size, H_kv, D] (or HND), both 16-bit of one type or both float8_e4m3fn
+// with scales [n_pages, H_kv, page_size] of float8_e8m0fnu.
+struct Cache {
+    fst_paged_cache c = {};
+    int64_t H_kv = 0, D = 0;
+    at::ScalarType type = at::kHalf;
+    bool quantised = false;
+};
+Cache open_cache(PyObject *k_pool, PyObject *v_pool, PyObject *table_o, PyObject *k_scale, PyObject *v_scale, bool nhd, int64_t Z,
+                 const char *who) {
+    const at::Tensor &kp = tensor(k_pool), &vp = tensor(v_pool), &table = tensor(table_o);
+    for (const at::Tensor *t : {&kp, &vp, &table})
+        if (!t->is_cuda()) {
+            PyErr_Format(PyExc_RuntimeError, "%s runs on CUDA tensors only; there is no CPU path", who);
+            throw PyError{};
+        }
+    const int row_dim = nhd ? 1 : 2, head_dim = nhd ? 2 : 1;
+    Cache r;
+    r.type = kp.scalar_type();
+    if ((r.type != at::kHalf && r.type != at::kBFloat16 && r.type != at::kFloat8_e4m3fn) || vp.scalar_type() != r.type)
+        raise(PyExc_TypeError, "the pools must share one dtype out of float16, bfloat16, float8_e4m3fn");
+    bool alike = kp.dim() == 4 && vp.sizes() == kp.sizes() && kp.stride(3) == 1 && vp.stride(3) == 1;
+    for (int i = 0; i < 3 && alike; ++i) alike = stride_of(kp, i) == stride_of(vp, i);
+    if (!alike)
+        raise(PyExc_ValueError, "pools must be two equally laid out [n_pages, page_size, H_kv, D] (or HND) tensors");
+    r.quantised = r.type == at::kFloat8_e4m3fn;
+    r.H_kv = kp.size(head_dim);
+    r.D = kp.size(3);
+    if (r.D != 64 && r.D != 128) raise(PyExc_ValueError, "head dimension must be 64 or 128");
+    const int64_t ps = kp.size(row_dim);
+    if (ps != 16 && ps != 32 && ps != 64 && ps != 128) raise(PyExc_ValueError, "page size must be 16, 32, 64 or 128");
+    if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != Z || !table.is_contiguous())
+        raise(PyExc_ValueError, "block_table must be contiguous int32 [Z, pages]");
+    if (kp.size(0) > INT_MAX || table.size(1) > INT_MAX || r.H_kv > INT_MAX) raise(PyExc_ValueError, "cache too large");
+    on_device(vp, kp.device());
+    on_device(table, kp.device());
+    if (r.quantised != (k_scale != Py_None) || r.quantised != (v_scale != Py_None))
+        raise(PyExc_ValueError, "a float8_e4m3fn cache needs k_scale and v_scale, one of 16 bits takes none");
+    if (r.quantised) {
+        for (PyObject *o : {k_scale, v_scale}) {
+            const at::Tensor &s = tensor(o);
+            if (s.scalar_type() != at::kFloat8_e8m0fnu || s.dim() != 3 || s.size(0) != kp.size(0) || s.size(1) != r.H_kv || s.size(2) != ps ||
+                !s.is_contiguous())
+                raise(PyExc_ValueError, "k_scale and v_scale must be contiguous float8_e8m0fnu [n_pages, H_kv, page_size]");
+            on_device(s, kp.device());
+        }
+        r.c.k_scale = static_cast<uint8_t *>(tensor(k_scale).data_ptr());
+        r.c.v_scale = static_cast<uint8_t *>(tensor(v_scale).data_ptr());
+    }
+    r.c.k_pool = kp.data_ptr();
+    r.c.v_pool = vp.data_ptr();
+    r.c.block_table = static_cast<const int32_t *>(table.data_ptr());
+    r.c.table_stride = int(table.size(1));
+    r.c.page_size = int(ps);
+    r.c.n_pages = int(kp.size(0));
+    r.c.stride_page = stride_of(kp, 0);
+    r.c.stride_row = stride_of(kp, row_dim);
+    r.c.stride_head = stride_of(kp, head_dim);
+    return r;
+}
+// int32 [Z], contiguous, on the device of the cache
+at::Tensor lengths(PyObject *o, int64_t Z, const at::Device &dev, const char *name) {
+    const at::Tensor &t = tensor(o);
+    if (t.scalar_type() != at::kInt || t.dim() != 1 || t.size(0) != Z) {
+        PyErr_Format(PyExc_ValueError, "%s must be int32 [Z]", name);
+        throw PyError{};
+    }
+    on_device(t, dev);
+    return t.contiguous();
+}
+const int32_t *words(const at::Tensor &t) { return t.defined() ? static_cast<const int32_t *>(t.data_ptr()) : nullptr; }
+
+// cache_append(k, v, k_pool, v_pool, nhd, block_table, start, lens, rows, k_scale, v_scale)
+PyObject *cache_append(PyObject *const *a, Py_ssize_t n) {
+    want_args(n, 11);
+    const at::Tensor &k = tensor(a[0]), &v = tensor(a[1]);
+    if (k.dim() != 4 || v.sizes() != k.sizes()) raise(PyExc_ValueError, "k and v must be [Z, H_kv, N, D]");
+    const int64_t Z = k.size(0), N = k.size(2);
+    const Cache c = open_cache(a[2], a[3], a[5], a[9], a[10], a[4] == Py_True, Z, "fst_cache_append");
+    const at::Device dev = tensor(a[2]).device();
+    on_device(k, dev);
+    on_device(v, dev);
+    const at::ScalarType type = k.scalar_type();
+    if (dtype_code(type) < 0 || type == at::kFloat || v.scalar_type() != type || (!c.quantised && type != c.type))
+        raise(PyExc_TypeError, "k and v must share one dtype out of float16, bfloat16, that of a 16-bit cache");
+    if (k.size(1) != c.H_kv || k.size(3) != c.D) raise(PyExc_ValueError, "k and v must have the cache's heads and head dimension");
+    head_contiguous(k);
+    head_contiguous(v);
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor start = lengths(a[6], Z, dev, "start");
+    at::Tensor lens, rows;
+    if (a[7] != Py_None) lens = lengths(a[7], Z, dev, "lens");
+    int64_t M = N;
+    if (a[8] != Py_None) {
+        rows = tensor(a[8]);
+        if (rows.scalar_type() != at::kInt || rows.dim() != 2 || rows.size(0) != Z) raise(PyExc_ValueError, "rows must be int32 [Z, M]");
+        on_device(rows, dev);
+        rows = rows.contiguous();
+        M = rows.size(1);
+    }
+    if (Z == 0 || M == 0 || c.H_kv == 0) Py_RETURN_NONE;
+    if (N == 0) raise(PyExc_ValueError, "k and v have no rows");
+    if (Z > INT_MAX || N > INT_MAX || M > INT_MAX) raise(PyExc_ValueError, "k and v are too large");
+    int32_t *status = static_cast<int32_t *>(status_of(dev, true)->data_ptr());
+    void *stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        rc = fst_cache_append(&c.c, k.data_ptr(), v.data_ptr(), words(start), words(lens), words(rows), int(Z), int(c.H_kv), int(N),
+                              int(M), int(c.D), FST_ROW_STRIDES(k), FST_ROW_STRIDES(v), dtype_code(type), status, stream);
+    }
+    check_status(rc, "fst_cache_append");
+    Py_RETURN_NONE;
+}
+
+// cache_read(k_pool, v_pool, nhd, block_table, lens, max_rows, k_scale, v_scale, dtype is bf16 (None: the pools'), k_out, v_out) -> (k, v)
+PyObject *cache_read(PyObject *const *a, Py_ssize_t n) {
+    want_args(n, 11);
+    const int64_t Z = tensor(a[3]).dim() == 2 ? tensor(a[3]).size(0) : -1, M = integer(a[5]);
+    const Cache c = open_cache(a[0], a[1], a[3], a[6], a[7], a[2] == Py_True, Z, "fst_cache_read");
+    const at::Device dev = tensor(a[0]).device();
+    const at::ScalarType type = a[8] == Py_None ? (c.quantised ? at::kBFloat16 : c.type) : a[8] == Py_True ? at::kBFloat16 : at::kHalf;
+    if (!c.quantised && type != c.type) raise(PyExc_TypeError, "a 16-bit cache is read as what it is");
+    if (M < 0 || M > INT_MAX) raise(PyExc_ValueError, "max_rows must not be negative");
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor lens = lengths(a[4], Z, dev, "lens");
+    at::Tensor out[2];
+    for (int i = 0; i < 2; ++i) {
+        if (a[9 + i] == Py_None) {
+            out[i] = empty({Z, c.H_kv, M, c.D}, type, dev);
+            continue;
+        }
+        out[i] = tensor(a[9 + i]);
+        if (out[i].dim() != 4 || out[i].size(0) != Z || out[i].size(1) != c.H_kv || out[i].size(2) != M || out[i].size(3) != c.D ||
+            out[i].scalar_type() != type)
+            raise(PyExc_ValueError, "out must be two [Z, H_kv, max_rows, D] tensors of the dtype that is read");
+        on_device(out[i], dev);
+        head_contiguous(out[i]);
+    }
+    if (Z > 0 && M > 0 && c.H_kv > 0) {
+        int32_t *status = static_cast<int32_t *>(status_of(dev, true)->data_ptr());
+        void *stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+        int rc;
+        {
+            pybind11::gil_scoped_release no_gil;
+            rc = fst_cache_read(&c.c, out[0].data_ptr(), out[1].data_ptr(), words(lens), int(Z), int(c.H_kv), int(M), int(c.D),
+                                FST_ROW_STRIDES(out[0]), FST_ROW_STRIDES(out[1]), dtype_code(type), status, stream);
+        }
+        check_status(rc, "fst_cache_read");
+    }
+    PyObject *k = THPVariable_Wrap(out[0]), *v = THPVariable_Wrap(out[1]);
+    PyObject *pair = PyTuple_Pack(2, k, v);
+    Py_DECREF(k);
+    Py_DECREF(v);
+    return pair;
+}
+
+// attention_chunk(q, out, k_pool, v_pool, nhd, block_table, kv_lens, q_lens, k_scale, v_scale, sm_scale, causal, return_lse)
+PyObject *attention_chunk(PyObject *const *a, Py_ssize_t n) {
+    want_args(n, 13);
+    Call c;
+    c.q = tensor(a[0]);
+    if (c.q.dim() != 4) raise(PyExc_ValueError, "q must be [Z, H, N, D]");
+    c.Z = c.q.size(0); c.H = c.q.size(1); c.n_q = c.q.size(2); c.D = c.q.size(3);
+    const Cache cache = open_cache(a[2], a[3], a[5], a[8], a[9], a[4] == Py_True, c.Z, "fst_attention_chunk");
+    const at::Device dev = tensor(a[2]).device();
+    on_device(c.q, dev);
+    const at::ScalarType type = c.q.scalar_type();
+    c.dtype = dtype_code(type);
+    if (c.dtype < 0 || type == at::kFloat || (!cache.quantised && type != cache.type))
+        raise(PyExc_TypeError, "q must be float16 or bfloat16, the dtype of a 16-bit cache");
+    c.H_kv = cache.H_kv;
+    if (c.D != cache.D || c.H_kv < 1 || c.H < 1 || c.H % c.H_kv) raise(PyExc_ValueError, "q must have the cache's head dimension and a multiple of its heads");
+    if (c.Z > INT_MAX || c.H > INT_MAX || c.n_q > INT_MAX) raise(PyExc_ValueError, "q is too large");
+    const double s = real(a[10]);
+    if (!std::isfinite(s) || !(float(s) > 0.f)) raise(PyExc_ValueError, "sm_scale must be positive and finite");
+    c.scale = float(s);
+    head_contiguous(c.q);
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor kv_lens = lengths(a[6], c.Z, dev, "kv_lens");
+    at::Tensor q_lens;
+    if (a[7] != Py_None) q_lens = lengths(a[7], c.Z, dev, "q_lens");
+    const bool want_lse = a[12] == Py_True;
+    if (a[1] == Py_None) {
+        c.o = empty(c.q.sizes(), type, dev);
+        if (q_lens.defined()) c.o.zero_();                // rows behind a sequence's queries are not written
+    } else {
+        c.o = tensor(a[1]);
+        if (c.o.sizes() != c.q.sizes() || c.o.scalar_type() != type) raise(PyExc_ValueError, "out must match q");
+        on_device(c.o, dev);
+        head_contiguous(c.o);
+    }
+    if (want_lse) {
+        c.lse = empty({c.Z * c.H, c.n_q}, at::kFloat, dev);
+        if (q_lens.defined()) c.lse.fill_(-INFINITY);
+    }
+    if (c.Z == 0 || c.n_q == 0) return results(c);
+    at::Tensor ws;
+    const size_t ws_bytes = fst_attention_chunk_workspace_bytes(&cache.c, int(c.Z), int(c.H), int(c.H_kv), int(c.n_q), int(c.D));
+    if (ws_bytes > 0) ws = empty({int64_t(ws_bytes)}, at::kByte, dev);
+    int32_t *status = static_cast<int32_t *>(status_of(dev, true)->data_ptr());
+    void *stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        rc = fst_attention_chunk(c.q.data_ptr(), c.o.data_ptr(), lse_ptr(c), &cache.c, words(kv_lens), words(q_lens), int(c.Z), int(c.H),
+                                 int(c.H_kv), int(c.n_q), int(c.D), FST_ROW_STRIDES(c.q), FST_ROW_STRIDES(c.o), c.scale, a[11] == Py_True,
+                                 c.dtype, ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, status, stream);
+    }
+    check_status(rc, "fst_attention_chunk");
+    return results(c);
+}
+
 // ---- trees ---------------------------------------------------------------------------------------
 // A cleared status record.  Clearing one per call is a launch (about a microsecond in front of a five
 // microsecond kernel), so a thread takes them from a block that it cleared in one go on the same stream;
@@ -719,7 +937,7 @@ PyMethodDef methods[] = {
     FST_METHOD(attention),      FST_METHOD(attention_ref), FST_METHOD(attention_paged), FST_METHOD(pack),
     FST_METHOD(precompute),     FST_METHOD(new_metadata),  FST_METHOD(dfs_order),
     FST_METHOD(build_tree_topk), FST_METHOD(parents_of_lineage), FST_METHOD(write_self), FST_METHOD(check_tree), FST_METHOD(metadata_of_lineage), FST_METHOD(read_status), FST_METHOD(status_record), FST_METHOD(attention_status),
-    FST_METHOD(splits),         {nullptr, nullptr, 0, nullptr}};
+    FST_METHOD(splits),         FST_METHOD(cache_append),  FST_METHOD(cache_read),     FST_METHOD(attention_chunk), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fst_host", "tensor-level calls into libfstattn_b200.so", -1, methods};
 
 }  // namespace

@@ -326,6 +326,72 @@ int fst_attention_fwd_paged(const void *q, const void *k_tree, const void *v_tre
                             void *workspace, size_t workspace_bytes, int32_t *status, void *stream);
 
 /*
+ * A paged K/V cache.  Row r of sequence z sits in page block_table[z * table_stride + r / page_size] at row
+ * r % page_size; element (page, row, head, d) of a pool at page * stride_page + row * stride_row + head * stride_head + d
+ * (strides in elements, the same for both pools).  page_size is 16, 32, 64 or 128, head_dim 64 or 128.
+ *
+ * With k_scale and v_scale NULL the pools hold 16-bit rows (fp16 or bf16, as the call's dtype says; strides multiples of
+ * 8).  Otherwise they hold e4m3 bytes (strides multiples of 16) and the scales, contiguous
+ * [n_pages][H_kv][page_size] bytes, a biased exponent b (e8m0) for every row and head: the row stands for e4m3 * 2^(b - 127),
+ * for NaN where b is 255.
+ * All addresses are device pointers on 16-byte boundaries (block_table: 4).  The struct itself is read during the call.
+ */
+typedef struct fst_paged_cache {
+    void *k_pool, *v_pool;
+    uint8_t *k_scale, *v_scale;
+    const int32_t *block_table;
+    int table_stride, page_size, n_pages;
+    int64_t stride_page, stride_row, stride_head;
+} fst_paged_cache;
+
+/*
+ * New K/V rows into the pages behind the sequences' ends.  k, v: [Z][H_kv][N][head_dim] by the given strides
+ * (elements, multiples of 8; fp16 or bf16).  Row j < lens[z] of sequence z (lens NULL: all M) goes to position start[z] + j.
+ * rows, when not NULL, is [Z][M]: new row j is row rows[z][j] of k and v - the accepted path of a token tree; otherwise
+ * M = N and it is row j.  An 8-bit cache gets, with a the row's largest magnitude, the smallest e in
+ * [-117, 119] with a <= 448 * 2^e, the values rounded to e4m3(x * 2^-e) (nearest, ties to even, saturating) and
+ * b = e + 127; a row with an element that is not finite gets zeros and b = 255.
+ * A position outside the table, a page number outside [0, n_pages) or an entry of rows outside [0, N) is not written and sets
+ * FST_DEV_INDEX_RANGE.  Two rows of a call must not go to the same place: which of them (and of its halves) stays is not defined.
+ */
+int fst_cache_append(const fst_paged_cache *cache, const void *k, const void *v, const int32_t *start,
+                     const int32_t *lens, const int32_t *rows, int Z, int H_kv, int N, int M, int head_dim,
+                     int64_t k_stride_z, int64_t k_stride_h, int64_t k_stride_n,
+                     int64_t v_stride_z, int64_t v_stride_h, int64_t v_stride_n,
+                     int dtype, int32_t *status, void *stream);
+
+/*
+ * Rows [0, min(lens[z], max_rows)) of every sequence out of the pages into k, v: [Z][H_kv][max_rows][head_dim]
+ * by the given strides; the rows behind them are written as zeros.  An 8-bit cache is expanded to dtype (fp16: values
+ * past 65504 saturate, small ones are rounded; bf16: exact).  A page number outside [0, n_pages) reads as zeros and sets
+ * FST_DEV_INDEX_RANGE, as does a row past the table.
+ */
+int fst_cache_read(const fst_paged_cache *cache, void *k, void *v, const int32_t *lens, int Z, int H_kv, int max_rows,
+                   int head_dim, int64_t k_stride_z, int64_t k_stride_h, int64_t k_stride_n,
+                   int64_t v_stride_z, int64_t v_stride_h, int64_t v_stride_n,
+                   int dtype, int32_t *status, void *stream);
+
+/*
+ * Attention of new tokens over the cache, which holds their own rows too.  q: [Z][H][n_q][head_dim], H a multiple
+ * of H_kv.  Sequence z has kv_lens[z] rows in the cache and q_lens[z] queries (NULL: n_q), its last
+ * q_lens[z] positions: query i attends to rows [0, kv_lens[z] - q_lens[z] + i], or with causal = 0 to all kv_lens[z] rows.
+ * A query that sees no row gets zeros (lse -inf).  Rows i >= q_lens[z] of o and lse are left as they are.  What the
+ * cache holds at rows that a query does not attend to, NaN and infinities included, does not reach it.
+ * lse, when not NULL, is [Z][H][n_q], base-2 log-sum-exp of the scaled scores.  sm_scale must be positive and finite.
+ * workspace: fst_attention_chunk_workspace_bytes() bytes (for the current device), 16-byte aligned, scratch of this call
+ * alone; what is in it before does not matter.  May be NULL where that is 0.
+ * A length that is negative or past the table (or n_q) is cut and sets FST_DEV_INDEX_RANGE, a page number outside
+ * [0, n_pages) reads as zeros and does the same.
+ */
+size_t fst_attention_chunk_workspace_bytes(const fst_paged_cache *cache, int Z, int H, int H_kv, int n_q, int head_dim);
+int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cache *cache, const int32_t *kv_lens,
+                        const int32_t *q_lens, int Z, int H, int H_kv, int n_q, int head_dim,
+                        int64_t q_stride_z, int64_t q_stride_h, int64_t q_stride_n,
+                        int64_t o_stride_z, int64_t o_stride_h, int64_t o_stride_n,
+                        float sm_scale, int causal, int dtype, void *workspace, size_t workspace_bytes,
+                        int32_t *status, void *stream);
+
+/*
  * The same with reference-format metadata, i.e. exactly the arguments of the reference's
  * fst_attention(q, k, v, ancestor_idx, ancestor_mask, leaf_idx, sm_scale, BLOCK_M,
  * MAX_ANCESTORS) (fstattention.py:153).  Index tensors hold absolute K/V rows
