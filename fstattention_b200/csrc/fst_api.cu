@@ -80,8 +80,6 @@ static bool aligned_strides(std::initializer_list<int64_t> strides) {
         if (s & 7) return false;
     return true;
 }
-// rows of a row tile of the kernel that a chunk call goes to
-static int chunk_rows(int n_q, int group) { return (long long)n_q * group <= 16 ? 16 : 32; }
 }  // namespace fst
 
 using namespace fst;
@@ -523,7 +521,9 @@ size_t fst_attention_chunk_workspace_bytes(const fst_paged_cache *cache, int Z, 
     ChunkArgs a = {};
     if (Z <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || n_q <= 0 || open_cache(a.c, cache, head_dim, FST_F16) != FST_OK) return 0;
     if (!chunk_splits(a, 128)) return 0;
-    return size_t(2) * chunk_ctas() * chunk_rows(n_q, H / H_kv) * (head_dim + 2) * sizeof(float);
+    a.n_q = n_q;
+    a.group = H / H_kv;
+    return size_t(2) * chunk_ctas() * chunk_row_tile(a) * (head_dim + 2) * sizeof(float);
 }
 
 int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cache *cache, const int32_t *kv_lens,

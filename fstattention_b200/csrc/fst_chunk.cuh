@@ -55,13 +55,23 @@ struct ChunkLine {
     }
     // at least one key tile, so that rows which see nothing are written too
     __device__ __forceinline__ static int tiles_of(int keys) { return max(1, (keys + KEYS - 1) / KEYS); }
-    // key tiles of one K/V head of a sequence
+    // Key tiles of one K/V head of a sequence: by one lane, or by a whole warp where the row tiles are many (64 row tiles one after
+    // the other take a lane 2 us).
+    __device__ __forceinline__ bool wide() const { return a.causal && row_tiles(a.n_q) > 8; }
     __device__ __forceinline__ long long head_tiles(int kv, int ql) const {
         const int n = row_tiles(ql);
         if (!a.causal) return (long long)n * tiles_of(kv);
         long long s = 0;
 #pragma unroll 1
         for (int qt = 0; qt < n; ++qt) s += tiles_of(keys(kv, ql, qt));
+        return s;
+    }
+    __device__ __forceinline__ long long head_tiles_by_warp(int kv, int ql) const {
+        long long s = 0;
+#pragma unroll 1
+        for (int qt = threadIdx.x & 31, n = row_tiles(ql); qt < n; qt += 32) s += tiles_of(keys(kv, ql, qt));
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
         return s;
     }
 };
@@ -84,47 +94,73 @@ struct ChunkCursor {
     __device__ __forceinline__ static long long total(const ChunkLine<ROWS, KEYS> &line) {
         const int lane = threadIdx.x & 31;
         long long sum = 0;
+        if (line.wide()) {
+#pragma unroll 1
+            for (int z = 0; z < line.a.Z; ++z) sum += line.head_tiles_by_warp(line.kv_len(z), line.q_len(z));
+            return sum * line.a.H_kv;
+        }
 #pragma unroll 1
         for (int z = lane; z < line.a.Z; z += 32) sum += line.head_tiles(line.kv_len(z), line.q_len(z));
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
         return sum * line.a.H_kv;
     }
+    // running sums over the lanes
+    __device__ __forceinline__ static long long scan(long long v) {
+#pragma unroll
+        for (int s = 1; s < 32; s *= 2) {
+            const long long below = __shfl_up_sync(0xffffffffu, v, s);
+            if (int(threadIdx.x & 31) >= s) v += below;
+        }
+        return v;
+    }
     // by a whole warp: to tile `pos` of the line, which has to be in it
     __device__ __forceinline__ void seek(const ChunkLine<ROWS, KEYS> &line, long long pos) {
         const int lane = threadIdx.x & 31;
         long long head = 1;
         z = 0;
+        if (line.wide()) {
 #pragma unroll 1
-        for (int z0 = 0; z0 < line.a.Z; z0 += 32) {
-            const long long mine = z0 + lane < line.a.Z ? line.head_tiles(line.kv_len(z0 + lane), line.q_len(z0 + lane)) : 0;
-            long long upto = mine * line.a.H_kv;
-#pragma unroll
-            for (int s = 1; s < 32; s *= 2) {
-                const long long below = __shfl_up_sync(0xffffffffu, upto, s);
-                if (lane >= s) upto += below;
+            for (;; ++z) {
+                head = line.head_tiles_by_warp(line.kv_len(z), line.q_len(z));
+                if (pos < head * line.a.H_kv || z + 1 == line.a.Z) break;
+                pos -= head * line.a.H_kv;
             }
-            const unsigned past = __ballot_sync(0xffffffffu, pos < upto);
-            if (past != 0u) {
-                const int f = __ffs(past) - 1;
-                z = z0 + f;
-                head = __shfl_sync(0xffffffffu, mine, f);
-                pos -= __shfl_sync(0xffffffffu, upto, f) - head * line.a.H_kv;
-                break;
+        } else {
+#pragma unroll 1
+            for (int z0 = 0; z0 < line.a.Z; z0 += 32) {
+                const long long mine = z0 + lane < line.a.Z ? line.head_tiles(line.kv_len(z0 + lane), line.q_len(z0 + lane)) : 0;
+                const long long upto = scan(mine * line.a.H_kv);
+                const unsigned past = __ballot_sync(0xffffffffu, pos < upto);
+                if (past != 0u) {
+                    const int f = __ffs(past) - 1;
+                    z = z0 + f;
+                    head = __shfl_sync(0xffffffffu, mine, f);
+                    pos -= __shfl_sync(0xffffffffu, upto, f) - head * line.a.H_kv;
+                    break;
+                }
+                pos -= __shfl_sync(0xffffffffu, upto, 31);
             }
-            pos -= __shfl_sync(0xffffffffu, upto, 31);
         }
         open(line);
         h = int(pos / head);
         pos -= h * head;
         qt = 0;
-        at_row_tile(line);
+        if (n_qt > 1) {
 #pragma unroll 1
-        while (pos >= tiles) {
-            pos -= tiles;
-            ++qt;
-            at_row_tile(line);
+            for (int q0 = 0; q0 < n_qt; q0 += 32) {
+                const long long mine = q0 + lane < n_qt ? line.tiles_of(line.keys(kv, ql, q0 + lane)) : 0, upto = scan(mine);
+                const unsigned past = __ballot_sync(0xffffffffu, pos < upto);
+                if (past != 0u) {
+                    const int f = __ffs(past) - 1;
+                    qt = q0 + f;
+                    pos -= __shfl_sync(0xffffffffu, upto - mine, f);
+                    break;
+                }
+                pos -= __shfl_sync(0xffffffffu, upto, 31);
+            }
         }
+        at_row_tile(line);
         tile = int(pos);
     }
     // to the next tile; the last tile of the line has none
@@ -261,6 +297,9 @@ cudaError_t launch_chunk_combine(const ChunkArgs &a, int n_ctas, cudaStream_t st
 
 // CTAs of a call's line: one per SM (a workspace holds two pieces for each).
 inline int chunk_ctas() { return sm_count(); }
+// Which kernel: up to 32 rows the mma.sync one.
+inline bool chunk_many_rows(const ChunkArgs &a) { return a.c.k_scale == nullptr && (long long)a.n_q * a.group > 32; }
+inline int chunk_row_tile(const ChunkArgs &a) { return chunk_many_rows(a) ? 256 : (long long)a.n_q * a.group <= 16 ? 16 : 32; }
 // Whether any piece can be less than an item: not if all that the table can hold is one key tile.
 inline bool chunk_splits(const ChunkArgs &a, int keys) { return ((long long)a.c.width << a.c.page_shift) > keys; }
 

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "fst_chunk_mma.cuh"
+#include "fst_chunk_umma.cuh"
 
 namespace fst {
 
@@ -9,6 +10,10 @@ template <typename T, int D>
 cudaError_t launch_chunk_t(const ChunkArgs &a, int n_ctas, cudaStream_t stream) {
     constexpr bool bf16 = !std::is_same<T, __half>::value;
     alignas(64) CUtensorMap tk, tv;
+    if (chunk_many_rows(a)) {
+        if (!make_pool_maps(&tk, &tv, a.c, bf16, D, a.H_kv, 1 << a.c.page_shift)) return cudaErrorNotSupported;
+        return launch_chunk_umma<T, D>(a, tk, tv, n_ctas, stream);
+    }
     if (!make_pool_maps(&tk, &tv, a.c, bf16, D, a.H_kv, 16)) return cudaErrorNotSupported;
     const bool one = a.n_q * a.group <= 16;
     if (a.c.k_scale != nullptr)
