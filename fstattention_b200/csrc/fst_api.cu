@@ -523,7 +523,7 @@ size_t fst_attention_chunk_workspace_bytes(const fst_paged_cache *cache, int Z, 
     if (!chunk_splits(a, 128)) return 0;
     a.n_q = n_q;
     a.group = H / H_kv;
-    return size_t(2) * chunk_ctas() * chunk_row_tile(a) * (head_dim + 2) * sizeof(float);
+    return chunk_part_bytes(chunk_ctas(), chunk_row_tile(a), head_dim);
 }
 
 int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cache *cache, const int32_t *kv_lens,
@@ -548,7 +548,7 @@ int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cach
     a.os_z = o_stride_z; a.os_h = o_stride_h; a.os_n = o_stride_n;
     a.scale_log2 = sm_scale * 1.4426950408889634f;
     a.causal = causal != 0;
-    a.part = static_cast<float *>(workspace);
+    a.part = need > 0 ? static_cast<float *>(workspace) : nullptr;
     a.status = status;
     const int n_ctas = chunk_ctas();
     cudaStream_t st = static_cast<cudaStream_t>(stream);

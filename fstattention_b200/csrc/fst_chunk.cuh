@@ -31,7 +31,7 @@ struct ChunkArgs {
     int64_t qs_z, qs_h, qs_n, os_z, os_h, os_n;
     float scale_log2;                      // sm_scale * log2(e), positive
     int causal;
-    float *part;                           // pieces: [2 CTAs][rows][D] sums, then [2 CTAs][rows] (exponent, sum)
+    float *part;                           // pieces: [2 CTAs][rows][D] sums, [2 CTAs][rows] (exponent, sum), [CTAs] ChunkCut
     int32_t *status;
 };
 
@@ -184,6 +184,14 @@ struct ChunkCursor {
     }
 };
 
+
+// What the merge has to know of the item that CTA i's last piece begins: its pieces are CTA i's last one and the first ones of the
+// CTAs behind it.
+struct ChunkCut {
+    int z, h, qt, ql, pieces;              // 1 (or 0, a CTA without work): nothing to merge
+    int pad[3];
+};
+
 // CTA i of n takes [first(i), first(i + 1)) of the line
 __device__ __forceinline__ long long chunk_first(long long total, int i, int n) { return total / n * i + min((long long)i, total % n); }
 
@@ -240,48 +248,81 @@ cudaError_t launch_serialised(void (*kernel)(P...), dim3 grid, dim3 block, size_
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// The pieces of the item that CTA x's last piece begins, merged: a warp per row, eight rows of the item per block.
-template <typename T, int D, int ROWS, int KEYS>
+__host__ __device__ inline size_t chunk_stats_at(int n_ctas, int rows, int D) { return size_t(2) * n_ctas * rows * D; }
+__host__ __device__ inline size_t chunk_cuts_at(int n_ctas, int rows, int D) { return chunk_stats_at(n_ctas, rows, D) + size_t(4) * n_ctas * rows; }
+inline size_t chunk_part_bytes(int n_ctas, int rows, int D) { return chunk_cuts_at(n_ctas, rows, D) * sizeof(float) + n_ctas * sizeof(ChunkCut); }
+
+// CTA i's note for the merge, by one thread, `last` being its last tile.  (Every CTA behind it takes `per` tiles or one more, so
+// that the count is a division and at most a step or two.)
+template <int ROWS, int D, int KEYS>
+__device__ __forceinline__ void leave_cut(const ChunkArgs &a, const ChunkCursor<ROWS, KEYS> &last, long long total, int n_tiles) {
+    ChunkCut cut = {};
+    if (n_tiles > 0) {
+        cut.z = last.z;
+        cut.h = last.h;
+        cut.qt = last.qt;
+        cut.ql = last.ql;
+        cut.pieces = 1;
+        const int behind = last.tiles - last.tile - 1;
+        if (behind > 0 && n_tiles > last.tile) {          // it goes on, and began here
+            const int me = blockIdx.x, n = gridDim.x;
+            const long long end = chunk_first(total, me + 1, n) + behind;
+            int c = me + 1 + int((behind - 1) / (total / n + 1));
+            while (c + 1 < n && chunk_first(total, c + 1, n) < end) ++c;
+            cut.pieces = c - me + 1;
+        }
+    }
+    reinterpret_cast<ChunkCut *>(a.part + chunk_cuts_at(gridDim.x, ROWS, D))[blockIdx.x] = cut;
+}
+
+// The pieces of the item that CTA x's last piece begins, merged in their order: a warp per row, eight rows of the item per block.
+// The factors of up to 32 pieces are taken by a lane each, so that nothing but the additions is a chain.
+template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(256)
 chunk_combine_kernel(const ChunkArgs a, int n_ctas) {
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    using Line = ChunkLine<ROWS, KEYS>;
-    using Cursor = ChunkCursor<ROWS, KEYS>;
     constexpr int C = D / 32;                             // columns of a lane
-    const Line line(a);
-    const long long total = Cursor::total(line), lo = chunk_first(total, blockIdx.x, n_ctas), hi = chunk_first(total, blockIdx.x + 1, n_ctas);
-    if (hi == lo || hi == total) return;
-    Cursor it;
-    it.seek(line, hi - 1);
-    const long long start = hi - 1 - it.tile, end = start + it.tiles;
-    if (end == hi || start < lo) return;                  // it ends with the CTA, or began before it
+    const ChunkCut it = reinterpret_cast<const ChunkCut *>(a.part + chunk_cuts_at(n_ctas, ROWS, D))[blockIdx.x];
     const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int r = it.qt * ROWS + row, tok = r / a.group, head = it.h * a.group + (r - tok * a.group);
-    if (tok >= it.ql) return;
-    const float2 *stats = reinterpret_cast<const float2 *>(a.part + size_t(2) * n_ctas * ROWS * D);
+    if (it.pieces <= 1 || tok >= it.ql) return;
+    const float2 *stats = reinterpret_cast<const float2 *>(a.part + chunk_stats_at(n_ctas, ROWS, D));
+    auto slot = [&](int piece) { return (size_t(2) * (blockIdx.x + piece) + (piece == 0 ? 1 : 0)) * ROWS + row; };
     float acc[C] = {}, top = -INFINITY, sum = 0.f;
-    // (both loads of a piece are asked for before the arithmetic of the one ahead)
-#pragma unroll 4
-    for (int c = blockIdx.x; c < n_ctas && (c == int(blockIdx.x) || chunk_first(total, c, n_ctas) < end); ++c) {
-        const size_t at = (size_t(2) * c + (c == int(blockIdx.x) ? 1 : 0)) * ROWS + row;
-        const float2 st = stats[at];
-        float v[C];
-        const float *from = a.part + at * D + lane * C;
-        if constexpr (C == 4) {
-            const float4 x = *reinterpret_cast<const float4 *>(from);
-            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-        } else {
-            const float2 x = *reinterpret_cast<const float2 *>(from);
-            v[0] = x.x; v[1] = x.y;
-        }
-        const float now = fmaxf(top, st.x), to = now == -INFINITY ? 0.f : now;
-        const float w_old = fast_exp2(top - to), w = fast_exp2(st.x - to);
-        const bool none = st.x == -INFINITY && st.y == 0.f;              // the piece saw nothing
-        sum = none ? sum : sum * (top == -INFINITY ? 1.f : w_old) + st.y * (st.x == -INFINITY ? 1.f : w);
+#pragma unroll 1
+    for (int p0 = 0; p0 < it.pieces; p0 += 32) {
+        const int n = min(32, it.pieces - p0);
+        const float2 st = lane < n ? stats[slot(p0 + lane)] : make_float2(-INFINITY, 0.f);
+        float now = st.x;
 #pragma unroll
-        for (int k = 0; k < C; ++k) acc[k] = none ? acc[k] : acc[k] * (top == -INFINITY ? 1.f : w_old) + v[k] * (st.x == -INFINITY ? 1.f : w);
+        for (int s = 16; s > 0; s >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, s));
+        now = fmaxf(now, top);
+        // a piece that saw nothing has no part in it; one whose scores were all NaN has no exponent, but a sum
+        const float w = st.x == -INFINITY ? (st.y == 0.f ? 0.f : 1.f) : fast_exp2(st.x - now);
+        const float w_old = top == -INFINITY ? 1.f : fast_exp2(top - now);
+        float part = st.y * w;
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) part += __shfl_xor_sync(0xffffffffu, part, s);
+        sum = sum * w_old + part;
         top = now;
+#pragma unroll
+        for (int k = 0; k < C; ++k) acc[k] *= w_old;
+#pragma unroll 8
+        for (int p = 0; p < n; ++p) {
+            const float f = __shfl_sync(0xffffffffu, w, p);
+            const float *from = a.part + slot(p0 + p) * D + lane * C;
+            float v[C];
+            if constexpr (C == 4) {
+                const float4 x = *reinterpret_cast<const float4 *>(from);
+                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+            } else {
+                const float2 x = *reinterpret_cast<const float2 *>(from);
+                v[0] = x.x; v[1] = x.y;
+            }
+#pragma unroll
+            for (int k = 0; k < C; ++k) acc[k] = f == 0.f ? acc[k] : fmaf(v[k], f, acc[k]);
+        }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T *dst = static_cast<T *>(a.o) + it.z * a.os_z + head * a.os_h + tok * a.os_n + lane * C;
@@ -290,9 +331,9 @@ chunk_combine_kernel(const ChunkArgs a, int n_ctas) {
     if (a.lse != nullptr && lane == 0) a.lse[(size_t(it.z) * a.H + head) * a.n_q + tok] = sum == 0.f ? -INFINITY : top + log2f(sum);
 }
 
-template <typename T, int D, int ROWS, int KEYS>
+template <typename T, int D, int ROWS>
 cudaError_t launch_chunk_combine(const ChunkArgs &a, int n_ctas, cudaStream_t stream) {
-    return launch_serialised(chunk_combine_kernel<T, D, ROWS, KEYS>, dim3(n_ctas, ROWS / 8), dim3(256), 0, stream, a, n_ctas);
+    return launch_serialised(chunk_combine_kernel<T, D, ROWS>, dim3(n_ctas, ROWS / 8), dim3(256), 0, stream, a, n_ctas);
 }
 
 // CTAs of a call's line: one per SM (a workspace holds two pieces for each).

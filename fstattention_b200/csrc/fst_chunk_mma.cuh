@@ -90,7 +90,10 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
     const Line line(a);
     const long long total = Cursor::total(line), first = chunk_first(total, blockIdx.x, gridDim.x);
     const int n_tiles = int(chunk_first(total, blockIdx.x + 1, gridDim.x) - first);
-    if (n_tiles == 0) return;
+    if (n_tiles == 0) {
+        if (tid == 0 && a.part != nullptr) leave_cut<G::ROWS, D>(a, Cursor{}, total, 0);
+        return;
+    }
 
     // ---- loads, one 16-key group of this warp at a time; the page of the next one is looked up a group ahead
     Cursor ld;
@@ -447,13 +450,14 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
 #pragma unroll
                     for (int k = 0; k < D / 16; k += 4)
                         *reinterpret_cast<float4 *>(a.part + at * D + c0 + k) = make_float4(out[k], out[k + 1], out[k + 2], out[k + 3]);
-                    if (c0 == 0) reinterpret_cast<float2 *>(a.part + size_t(2) * gridDim.x * G::ROWS * D)[at] = make_float2(top, sum);
+                    if (c0 == 0) reinterpret_cast<float2 *>(a.part + chunk_stats_at(gridDim.x, G::ROWS, D))[at] = make_float2(top, sum);
                 }
                 __syncthreads();
             }
         }
-        me.next(line);
+        if (i + 1 < n_tiles) me.next(line);
     }
+    if (tid == 0 && a.part != nullptr) leave_cut<G::ROWS, D>(a, me, total, n_tiles);
     if (!alive) {                                         // a wait ran out: nothing may land after this CTA has left
 #pragma unroll 1
         for (; in_flight > 0; --in_flight) {
@@ -477,7 +481,7 @@ static cudaError_t launch_chunk_mma(const ChunkArgs &a, const CUtensorMap &tk, c
     if (ce != cudaSuccess) return ce;
     const cudaError_t e = launch_serialised(chunk_mma_kernel<T, D, QUANT, MT>, dim3(n_ctas), dim3(256), G::BYTES, stream, a, tk, tv);
     if (e != cudaSuccess || !chunk_splits(a, G::KEYS)) return e;
-    return launch_chunk_combine<T, D, G::ROWS, G::KEYS>(a, n_ctas, stream);
+    return launch_chunk_combine<T, D, G::ROWS>(a, n_ctas, stream);
 }
 
 }  // namespace fst

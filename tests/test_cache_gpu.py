@@ -7,8 +7,8 @@ sm_scale * sum_d |q_d k_d|:
 * the output's own rounding, eps / 2 of its value, eps that of its type (an fp16 result below 2^-14: half of 2^-24);
 * the rounding of the probabilities to 16 bits for the second product, eps / 2 of A (bf16's eps over an 8-bit cache);
 * scores: fp32 sums of D products, D roundings of S (2^-23 each, the tensor cores may truncate), three more for the scale and
-  the distance to the maximum, and the exponential's own 2^-22; numerator and denominator are both off by that
-  share: 2 A (2^-23 (D + 3) S + 2^-22);
+  the distance to the maximum, and the exponential's own error, 2.6e-6 < 2^-18 for the polynomial; numerator and denominator are
+  both off by that share: 2 A (2^-23 (D + 3) S + 2^-18);
 * the sums over T keys in fp32: T + 64 roundings of 2^-23 at the most, of numerator and denominator: 2 A 2^-23 (T + 64).
 """
 import math
@@ -67,11 +67,12 @@ def check(got, lse, want, quantised, T):
     eps = torch.finfo(got.dtype).eps
     p_eps = torch.finfo(torch.bfloat16).eps if quantised else eps
     D = got.shape[-1]
-    share = 2.0 ** -23 * (D + 3) * size[..., None] + 2.0 ** -22
+    share = 2.0 ** -23 * (D + 3) * size[..., None] + 2.0 ** -18
     tol = out.abs() * eps / 2 + mag * (p_eps / 2 + 2 * share + 2 * 2.0 ** -23 * (T + 64)) + 2.0 ** -25
     same = (out == got.double()) | (torch.isnan(out) & torch.isnan(got))
     far = torch.where(same, torch.zeros_like(out), (got.double() - out).abs() - tol)
-    assert not torch.isnan(far).any() and far.max().item() <= 0, (far.max().item(), mag.max().item())
+    worst = float(torch.nan_to_num(far, nan=math.inf).max())
+    assert worst <= 0, worst
     if lse is not None:
         lse = lse.view(ref_lse.shape).double()
         assert torch.equal(torch.isinf(lse), torch.isinf(ref_lse))
