@@ -18,7 +18,7 @@ namespace fst {
 struct CacheArgs {
     void *k_pool, *v_pool;
     uint8_t *k_scale, *v_scale;            // [n_pages][H_kv][page_size] biased exponents (e8m0), null: rows in 16 bits
-    const int32_t *table;                  // [Z][width] page numbers; null: page i of sequence z is z * width + i
+    const int32_t *table;                  // [Z][width] page numbers
     int width, page_shift, n_pages;
     int64_t stride_page, stride_row, stride_head;
 };

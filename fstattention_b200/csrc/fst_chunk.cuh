@@ -215,19 +215,25 @@ __device__ __forceinline__ bool keep_finite(uint32_t &w, int n) {
     }
     return met;
 }
-// out[k] += the elements c0 + k of V in rows [from, to) of a sequence that are not finite
-template <typename T, int N>
+// out[k] += the elements c0 + k of V in rows [from, to) of a sequence that are not finite (of an 8-bit cache: all of a row, as NaN)
+template <typename T, int N, bool QUANT>
 __device__ __forceinline__ void add_not_finite(const ChunkArgs &a, int z, int h, int from, int to, int c0, float (&out)[N]) {
 #pragma unroll 1
     for (int key = from; key < to; ++key) {
         const int idx = key >> a.c.page_shift, off = key & ((1 << a.c.page_shift) - 1);
-        const int page = a.c.table == nullptr ? z * a.c.width + idx : __ldg(a.c.table + size_t(z) * a.c.width + idx);
+        const int page = __ldg(a.c.table + size_t(z) * a.c.width + idx);
         if (unsigned(page) >= unsigned(a.c.n_pages)) continue;
-        const T *v = static_cast<const T *>(a.c.v_pool) + page * a.c.stride_page + off * a.c.stride_row + h * a.c.stride_head + c0;
+        if constexpr (QUANT) {
+            const bool odd = __ldg(a.c.v_scale + ((size_t(page) * a.H_kv + h) << a.c.page_shift) + off) == 255;
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const float x = float(v[k]);
-            out[k] += isfinite(x) ? 0.f : x;
+            for (int k = 0; k < N; ++k) out[k] = odd ? NAN : out[k];
+        } else {
+            const T *v = static_cast<const T *>(a.c.v_pool) + page * a.c.stride_page + off * a.c.stride_row + h * a.c.stride_head + c0;
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const float x = float(v[k]);
+                out[k] += isfinite(x) ? 0.f : x;
+            }
         }
     }
 }
@@ -339,7 +345,7 @@ cudaError_t launch_chunk_combine(const ChunkArgs &a, int n_ctas, cudaStream_t st
 // CTAs of a call's line: one per SM (a workspace holds two pieces for each).
 inline int chunk_ctas() { return sm_count(); }
 // Which kernel: up to 32 rows the mma.sync one.
-inline bool chunk_many_rows(const ChunkArgs &a) { return a.c.k_scale == nullptr && (long long)a.n_q * a.group > 32; }
+inline bool chunk_many_rows(const ChunkArgs &a) { return (long long)a.n_q * a.group > 32; }
 inline int chunk_row_tile(const ChunkArgs &a) { return chunk_many_rows(a) ? 256 : (long long)a.n_q * a.group <= 16 ? 16 : 32; }
 // Whether any piece can be less than an item: not if all that the table can hold is one key tile.
 inline bool chunk_splits(const ChunkArgs &a, int keys) { return ((long long)a.c.width << a.c.page_shift) > keys; }

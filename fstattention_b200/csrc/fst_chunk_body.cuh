@@ -12,7 +12,7 @@ cudaError_t launch_chunk_t(const ChunkArgs &a, int n_ctas, cudaStream_t stream) 
     alignas(64) CUtensorMap tk, tv;
     if (chunk_many_rows(a)) {
         if (!make_pool_maps(&tk, &tv, a.c, bf16, D, a.H_kv, 1 << a.c.page_shift)) return cudaErrorNotSupported;
-        return launch_chunk_umma<T, D>(a, tk, tv, n_ctas, stream);
+        return a.c.k_scale != nullptr ? launch_chunk_umma<T, D, true>(a, tk, tv, n_ctas, stream) : launch_chunk_umma<T, D, false>(a, tk, tv, n_ctas, stream);
     }
     if (!make_pool_maps(&tk, &tv, a.c, bf16, D, a.H_kv, 16)) return cudaErrorNotSupported;
     const bool one = a.n_q * a.group <= 16;

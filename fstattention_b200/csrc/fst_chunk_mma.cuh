@@ -109,7 +109,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
         }
         if (left > 0) {
             const int idx = group_of(ld) >> a.c.page_shift;
-            page = a.c.table == nullptr ? ld.z * a.c.width + idx : __ldg(a.c.table + size_t(ld.z) * a.c.width + idx);
+            page = __ldg(a.c.table + size_t(ld.z) * a.c.width + idx);
         }
     };
     auto load = [&]() {                                   // requests it, then looks for the one behind
@@ -431,7 +431,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                 if (bad && tok < me.ql) {
                     // keys of this piece whose groups were looked through, as far as my row sees them
                     const int keys = a.causal ? min(me.kv, me.kv - me.ql + tok + 1) : me.kv;
-                    add_not_finite<T, D / 16>(a, me.z, me.h, max(max(lim_first, 0) & ~(G::KW - 1), max(0, me.tile - i) * G::KEYS),
+                    add_not_finite<T, D / 16, QUANT>(a, me.z, me.h, max(max(lim_first, 0) & ~(G::KW - 1), max(0, me.tile - i) * G::KEYS),
                                               min(keys, (me.tile + 1) * G::KEYS), c0, out);
                 }
                 if (whole) {

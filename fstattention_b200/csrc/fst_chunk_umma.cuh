@@ -19,48 +19,30 @@
 
 #include "fst_chunk.cuh"
 #include "fst_chunk_map.cuh"
+#include "fst_chunk_mma.cuh"
 #include "fst_umma.cuh"
 
 namespace fst {
 
-template <int D>
+template <int D, bool QUANT>
 struct ChunkUmmaGeo {
     static constexpr int ROWS = 256, KEYS = 128, THREADS = 512;
     static constexpr int TILE = (D / 64) * umma::HALF;              // 128 rows
     static constexpr int QBUF = D == 128 ? 1 : 2;                   // items whose Q is there at a time
-    static constexpr int RING = D == 128 ? 5 : 8;
-    static constexpr int OFF_RING = QBUF * 2 * TILE, OFF_BAR = OFF_RING + RING * TILE;
-    static constexpr int BARS = 3 * RING + 4 * QBUF + 9;
-    static constexpr int OFF_NOTE = OFF_BAR + BARS * 8;             // first item that held values that are not finite; tensor memory's address
-    static constexpr int BYTES = OFF_NOTE + 16 + 1024;              // + alignment
+    static constexpr int RING = QUANT ? (D == 128 ? 4 : 6) : (D == 128 ? 5 : 8);
+    static constexpr int RAW = QUANT ? (D == 128 ? 2 : 4) : 0;      // stages of 8-bit tiles: 128 rows of D bytes
+    static constexpr int OFF_RING = QBUF * 2 * TILE, OFF_RAW = OFF_RING + RING * TILE, OFF_BAR = OFF_RAW + RAW * 128 * D;
+    static constexpr int BARS = 3 * RING + 2 * RAW + 4 * QBUF + 9;
+    static constexpr int OFF_NOTE = (OFF_BAR + BARS * 8 + 15) & ~15;             // first item that held values that are not finite; tensor memory's address
+    static constexpr int OFF_SCALES = OFF_NOTE + 16;                // [raw stage] 128 bytes
+    static constexpr int OFF_PLAN = OFF_SCALES + RAW * 128;         // [stage] what a tile is to the issuing lane, see there
+    static constexpr int OFF_RAW_PLAN = OFF_PLAN + RING * 4;        // [raw stage] the same
+    static constexpr int BYTES = OFF_RAW_PLAN + RAW * 4 + 1024;     // + alignment
     // of 65536 registers a launch of 512 threads gets 128 each; the softmax warps take 192 and leave 64 to the others
     static constexpr int REGS_SOFTMAX = 192, REGS_OTHERS = 64;
 };
 static_assert(256 * 192 + 256 * 64 <= 512 * 128, "the split draws on what the launch was given");
 
-// 2^x for x up to 127, zero from -127 down: Cody and Waite's split x = n + f, f in [-1/2, 1/2], and the polynomial of degree 4 with the smallest
-// relative error on it (Remez' exchange; 2.6e-6), two at a time.
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ void exp2_poly(uint64_t x, float &p0, float &p1) {
-    using namespace umma;
-    const float kRound = 12582912.f;                      // 1.5 * 2^23: adding it leaves round(x) in the low bits
-    float a, b;
-    unpair(x, a, b);
-    x = pair(fmaxf(a, -127.f), fmaxf(b, -127.f));
-    const uint64_t t = add2(x, pair(kRound, kRound)), f = add2(x, fma2(t, pair(-1.f, -1.f), pair(kRound, kRound)));
-    uint64_t r = fma2(f, pair(0.009570102207362652f, 0.009570102207362652f), pair(0.05591785907745361f, 0.05591785907745361f));
-    r = fma2(r, f, pair(0.240247443318367f, 0.240247443318367f));
-    r = fma2(r, f, pair(0.6931217908859253f, 0.6931217908859253f));
-    r = fma2(r, f, pair(0.9999992847442627f, 0.9999992847442627f));
-    float t0, t1;
-    unpair(t, t0, t1);                                    // 2^n by its exponent; that of -127 is zero, and so is the result
-    r = mul2(r, pair(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u)));
-    unpair(r, p0, p1);
-}
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float r;
     asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(x), "f"(y), "f"(z));
@@ -72,16 +54,61 @@ __device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
     constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u, U = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
     return ((w & E) + U) & 0x80008000u;
 }
+// Row r of an 8-bit tile (128 rows of D bytes, swizzled as TMA leaves them) times 2^(b - 127) into row r of a tile of T; zeros if `none`.
 template <typename T, int D>
+__device__ __forceinline__ void widen_row(uint32_t from, uint32_t to, int r, uint32_t b, bool none) {
+    constexpr bool BF16 = !std::is_same<T, __half>::value;
+    // The shortcut: an e4m3's bits under T's exponent are value * 2^-120 (bf16) or value * 2^-8 (fp16); one multiplication by 2^(e + 120)
+    // or 2^(e + 8) gives the value.  It has to be one that T holds, and the product in T's range.
+    const int e = int(b) - 127;
+    const bool quick = BF16 ? e <= 7 : e <= 7 && e >= -22;
+    const uint32_t f = BF16 ? uint32_t(e + 247) << 7 : uint32_t(e + 23) << 10, ff = f | f << 16;
+    const float scale = e8m0_value(b);
+    const uint32_t src = from + r * D;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (!none) w = lds128(src + ((D == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4));
+        const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+        uint32_t out[8];
+        if (quick) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {                 // bytes 2 k, 2 k + 1 at the tops of 16-bit halves
+                const uint32_t x = __byte_perm(in[k >> 1], 0, k & 1 ? 0x3424 : 0x1404);
+                uint32_t y = (x & 0x80008000u) | ((x >> (BF16 ? 4 : 1)) & (BF16 ? 0x07f007f0u : 0x3f803f80u));
+                if constexpr (BF16) asm("mul.rn.bf16x2 %0, %0, %1;\n" : "+r"(y) : "r"(ff));
+                else asm("mul.rn.f16x2 %0, %0, %1;\n" : "+r"(y) : "r"(ff));
+                out[k] = y;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float2 x = e4m3_values(in[k >> 1] >> (k & 1) * 16);
+                out[k] = pack_cache<T>(x.x * scale, x.y * scale);
+            }
+            if (none)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) out[k] = 0;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int chunk = 2 * c + k;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(to + (chunk >> 3) * umma::HALF + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)),
+                         "r"(out[4 * k]), "r"(out[4 * k + 1]), "r"(out[4 * k + 2]), "r"(out[4 * k + 3]) : "memory");
+        }
+    }
+}
+
+template <typename T, int D, bool QUANT>
 __global__ void __launch_bounds__(512, 1)
 chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
     using namespace umma;
-    using G = ChunkUmmaGeo<D>;
+    using G = ChunkUmmaGeo<D, QUANT>;
     using MT = MmaTraits<T>;
     using Line = ChunkLine<G::ROWS, G::KEYS>;
     using Cursor = ChunkCursor<G::ROWS, G::KEYS>;
     constexpr bool BF16 = !std::is_same<T, __half>::value;
-    constexpr int DH = D / 64, TILE = G::TILE, RING = G::RING, QBUF = G::QBUF;
+    constexpr int DH = D / 64, TILE = G::TILE, RING = G::RING, QBUF = G::QBUF, RAW = G::RAW;
 
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     extern __shared__ unsigned char smem_raw[];
@@ -92,8 +119,11 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
     // full / raw (landed, to be looked through) / empty of every stage; Q there / done with, [buffer][group]; S landed, halves of P written,
     // O complete of either group
     const uint32_t bar_full = s_base + G::OFF_BAR, bar_raw = bar_full + RING * 8, bar_empty = bar_raw + RING * 8, bar_q = bar_empty + RING * 8,
-                   bar_qfree = bar_q + QBUF * 16, bar_s = bar_qfree + QBUF * 16, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_end = bar_o + 16;
+                   bar_qfree = bar_q + QBUF * 16, bar_s = bar_qfree + QBUF * 16, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_end = bar_o + 16,
+                   bar_in = bar_end + 8, bar_out = bar_in + RAW * 8;      // 8-bit tiles: landed, widened
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + G::OFF_NOTE + 8);
+    volatile uint32_t *plan = reinterpret_cast<volatile uint32_t *>(smem + G::OFF_PLAN);
+    volatile uint32_t *raw_plan = reinterpret_cast<volatile uint32_t *>(smem + G::OFF_RAW_PLAN);
     volatile int *note = reinterpret_cast<volatile int *>(smem + G::OFF_NOTE);
     if (warp == 8) {
         if (lane == 0) {
@@ -109,6 +139,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
                 mbar_init(bar_o + i * 8, 1);
             }
             mbar_init(bar_end, 1);
+            for (int i = 0; i < 2 * RAW; ++i) mbar_init(bar_in + i * 8, 1);
             *note = 0x7fffffff;
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         }
@@ -151,25 +182,76 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
             const int idx = me.tile * npt + lane;
             page = 0;
             if (lane < npt && idx * ps < me.keys)
-                page = a.c.table == nullptr ? me.z * a.c.width + idx : __ldg(a.c.table + size_t(me.z) * a.c.width + idx);
+                page = __ldg(a.c.table + size_t(me.z) * a.c.width + idx);
         };
+        // The plan of a tile goes into the word of its K's stage: 16-key steps with keys in them (bits 0-3), and of either group whether it
+        // takes part (4, 5), whether the tile is its piece's first (6, 7) or last (8, 9), which buffer holds Q (10); 0: no more tiles.
+        // The issuing lane has to hand over a product every 64 cycles and did not come to it (4400 instead of 2048 cycles a
+        // tile) while it kept the place in the line itself.
+        int tiles0 = 0, tiles1 = 0, item = 0;
         if (n_tiles > 0) look_up();
 #pragma unroll 1
-        for (int i = 0; i < n_tiles && alive; ++i) {
+        for (int i = 0; i <= n_tiles && alive; ++i) {
             const int here = page, key0 = me.tile * G::KEYS, h = me.h, z = me.z;
-            const int pages = (min(G::KEYS, me.keys - key0) + ps - 1) >> a.c.page_shift;      // 0: an item that sees nothing
-            const bool edge = key0 + G::KEYS > first_limit();
-            me.next(line);
-            if (i + 1 < n_tiles) look_up();
-            if (pages <= 0) continue;
+            int pages = 0;                                // 0: an item that sees nothing
+            bool edge = false;
+            uint32_t word = 0;
+            if (i < n_tiles) {
+                const bool begins = i == 0 || me.tile == 0;
+                if (begins) {
+                    if (i > 0) ++item;
+                    tiles0 = group_tiles(0);
+                    tiles1 = group_tiles(1);
+                }
+                pages = (min(G::KEYS, me.keys - key0) + ps - 1) >> a.c.page_shift;
+                edge = key0 + G::KEYS > first_limit();
+                const uint32_t on = (me.tile < tiles0 ? 1u : 0u) | (me.tile < tiles1 ? 2u : 0u);
+                const uint32_t ends = on & (i + 1 == n_tiles ? 3u : (me.tile + 1 == tiles0 ? 1u : 0u) | (me.tile + 1 == tiles1 ? 2u : 0u));
+                word = uint32_t(min(8, (me.keys - key0 + 15) >> 4)) | on << 4 | (begins ? on << 6 : 0u) | ends << 8 | uint32_t(QBUF == 1 ? 0 : item & 1) << 10;
+                me.next(line);
+                if (i + 1 < n_tiles) look_up();
+                if (pages <= 0) continue;
+            }
+            if constexpr (QUANT) {
 #pragma unroll 1
-            for (int v = 0; v < 2; ++v) {
+                for (int v = 0; v < (i < n_tiles ? 2 : 1); ++v) {
+                    const uint32_t bar = bar_in + st * 8;
+                    if (use > 0) alive = __all_sync(0xffffffffu, mbar_wait(bar_out + st * 8, (use - 1) & 1, a.status, where));
+                    if (!alive) break;
+                    const bool bad = lane < pages && unsigned(here) >= unsigned(a.c.n_pages);     // its rows read as zeros
+                    unsigned char *scales = smem + G::OFF_SCALES + st * 128 + lane * ps;
+                    if (bad) {
+                        if (v == 0) report(a.status, FST_DEV_INDEX_RANGE, z, key0 + lane * ps);
+                        for (int k = 0; k < ps; k += 16) *reinterpret_cast<uint4 *>(scales + k) = make_uint4(0, 0, 0, 0);
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    }
+                    const int good = pages - __popc(__ballot_sync(0xffffffffu, bad));
+                    if (lane == 0) {
+                        if (v == 0) raw_plan[st] = word;
+                        mbar_arrive_expect_tx(bar, ((pages * D + good) << a.c.page_shift));
+                    }
+                    __syncwarp();
+                    if (lane < pages) {
+                        tma_load_4d(s_base + G::OFF_RAW + st * 128 * D + lane * ps * D, v ? &tm_v : &tm_k, 0, 0, h, here, bar);
+                        if (!bad) bulk_load(smem_u32(scales), (v ? a.c.v_scale : a.c.k_scale) + ((size_t(here) * a.H_kv + h) << a.c.page_shift), ps, bar);
+                    }
+                    if (++st == RAW) {
+                        st = 0;
+                        ++use;
+                    }
+                }
+            } else {
+#pragma unroll 1
+            for (int v = 0; v < (i < n_tiles ? 2 : 1); ++v) {
                 const uint32_t dst = s_ring + st * TILE, bar = (v && edge ? bar_raw : bar_full) + st * 8;
                 if (use > 0) alive = __all_sync(0xffffffffu, mbar_wait(bar_empty + st * 8, (use - 1) & 1, a.status, where));
                 if (!alive) break;
                 to_raw = (to_raw & ~(1u << st)) | uint32_t(v && edge) << st;
                 raw_fills ^= uint32_t(v && edge) << st;
-                if (lane == 0) mbar_arrive_expect_tx(bar, (pages << a.c.page_shift) * D * 2);
+                if (lane == 0) {
+                    if (v == 0) plan[st] = word;
+                    mbar_arrive_expect_tx(bar, (pages << a.c.page_shift) * D * 2);
+                }
                 __syncwarp();
                 if (lane < pages) {
                     if (unsigned(here) >= unsigned(a.c.n_pages) && v == 0) report(a.status, FST_DEV_INDEX_RANGE, z, key0 + lane * ps);
@@ -181,20 +263,22 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
                     ++use;
                 }
             }
+            }
         }
         // nothing may land after the CTA has left, also when a wait ran out: the last fill of every stage
 #pragma unroll 1
-        for (int s = 0; s < RING; ++s) {
+        for (int s = 0; s < (QUANT ? RAW : RING); ++s) {
             const uint32_t fills = use + (s < st ? 1u : 0u);
-            if (fills > 0) mbar_wait((to_raw >> s & 1 ? bar_raw : bar_full) + s * 8, to_raw >> s & 1 ? (raw_fills >> s & 1) ^ 1u : (fills - 1) & 1, a.status, where);
+            if (QUANT && fills > 0) mbar_wait(bar_in + s * 8, (fills - 1) & 1, a.status, where);
+            else if (fills > 0) mbar_wait((to_raw >> s & 1 ? bar_raw : bar_full) + s * 8, to_raw >> s & 1 ? (raw_fills >> s & 1) ^ 1u : (fills - 1) & 1, a.status, where);
         }
     } else if (warp == 9) {
         // ====== products: for either group O += P V of the tile before, then S of this one ======
-        if (elect_one() && n_tiles > 0) {
+        if (elect_one()) {
             const uint32_t idesc_s = instr_desc(BF16, false, G::KEYS), idesc_pv = instr_desc(BF16, true, D);
             const uint64_t dq = smem_desc(s_base, 16), dk = smem_desc(s_ring, 16), dv = smem_desc(s_ring, HALF);
             int k_st = 0, v_st = 1;                       // stages of the next K and V
-            uint32_t k_ph = 0, v_ph = 0, p_ph = 0, q_ph = 0;                                  // (bit g: group g)
+            uint32_t k_ph = 0, v_ph = 0, p_ph = 0, q_ph = 0;      // (bits: group, or Q's buffer and group)
             auto step2 = [&](int &st, uint32_t &ph) {
                 st += 2;
                 if (st >= RING) {
@@ -203,83 +287,76 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
                 }
             };
             bool alive = true;
-            int item = 0;
-            // of the tile before: 16-key steps with keys in them, and of either group whether it takes part (bit g), whether this was its
-            // piece's first or last tile
-            int steps_b = 0;
-            uint32_t on_b = 0, first_b = 0, last_b = 0;
-            int tiles_g[2] = {0, 0};
+            uint32_t before = 0, now = 0;                 // the plan's words of the tile before and of this one
+            // O += P V of the tile before, without a branch among the products where all of its 128 keys count
+            auto second_product = [&](auto gc) {
+                constexpr int g = decltype(gc)::value;
+                const uint32_t tmem_o = tmem + 256 + g * D, tmem_p = D == 128 ? tmem + g * 128 : tmem + 384 + g * 64;
+                const uint64_t dvs = dv + uint64_t(v_st * (TILE >> 4));
+                const int steps = before & 15u;
+                const bool fresh = before >> (6 + g) & 1u;
+                alive = mbar_wait(bar_p + g * 16, p_ph >> g & 1, a.status, where);
+                if (!alive) return;
+                fence_after_sync();
+                if (steps == 8) {
+                    mma_f16_ts(tmem_o, tmem_p, dvs, idesc_pv, !fresh);
+#pragma unroll
+                    for (int ks = 1; ks < 4; ++ks) mma_f16_ts(tmem_o, tmem_p + ks * 8, dvs + uint64_t((ks * 16 * 128) >> 4), idesc_pv, true);
+                    alive = mbar_wait(bar_p + g * 16 + 8, p_ph >> g & 1, a.status, where);
+                    fence_after_sync();
+#pragma unroll
+                    for (int ks = 4; ks < 8; ++ks) mma_f16_ts(tmem_o, tmem_p + ks * 8, dvs + uint64_t((ks * 16 * 128) >> 4), idesc_pv, true);
+                } else {
+                    alive = mbar_wait(bar_p + g * 16 + 8, p_ph >> g & 1, a.status, where);
+                    fence_after_sync();
 #pragma unroll 1
-            for (int i = 0; i <= n_tiles && alive; ++i) {
-                const bool real = i < n_tiles && me.keys > 0;
-                if (real && (i == 0 || me.tile == 0)) {
-                    tiles_g[0] = group_tiles(0);
-                    tiles_g[1] = group_tiles(1);
+                    for (int ks = 0; ks < steps; ++ks) mma_f16_ts(tmem_o, tmem_p + ks * 8, dvs + uint64_t((ks * 16 * 128) >> 4), idesc_pv, ks > 0 || !fresh);
                 }
-                if (i > 0 && i < n_tiles && me.tile == 0) ++item;
-                const int qbuf = QBUF == 1 ? 0 : item & 1;
-                const int steps = real ? min(8, (me.keys - me.tile * G::KEYS + 15) >> 4) : 0;
-                uint32_t on = 0, first_here = 0, last_here = 0;
-                if (real) {
+                p_ph ^= 1u << g;
+                if (before >> (8 + g) & 1u) mma_commit(bar_o + g * 8);
+                if ((before >> 4 & 3u) >> g == 1u) {      // the last group to read this V
+                    mma_commit(bar_empty + v_st * 8);
+                    step2(v_st, v_ph);
+                }
+            };
+            auto first_product = [&](auto gc) {
+                constexpr int g = decltype(gc)::value;
+                const uint32_t tmem_s = tmem + g * 128, at = (now >> 10 & 1u) * 2 + g;
+                if (now >> (6 + g) & 1u) {
+                    alive = mbar_wait(bar_q + at * 8, q_ph >> at & 1, a.status, where);
+                    q_ph ^= 1u << at;
+                    if (!alive) return;
+                    fence_after_sync();
+                }
+                const uint64_t dqs = dq + uint64_t(at * (TILE >> 4)), dks = dk + uint64_t(k_st * (TILE >> 4));
 #pragma unroll
-                    for (int g = 0; g < 2; ++g)
-                        if (me.tile < tiles_g[g]) {
-                            on |= 1u << g;
-                            if (i == 0 || me.tile == 0) first_here |= 1u << g;
-                            if (me.tile + 1 == tiles_g[g] || i + 1 == n_tiles) last_here |= 1u << g;
-                        }
+                for (int ks = 0; ks < D / 16; ++ks) {
+                    const uint64_t koff = ((ks >> 2) * HALF + (ks & 3) * 32) >> 4;
+                    mma_f16(tmem_s, dqs + koff, dks + koff, idesc_s, ks > 0);
                 }
+                mma_commit(bar_s + g * 8);
+                if (now >> (8 + g) & 1u) mma_commit(bar_qfree + at * 8);
+                if ((now >> 4 & 3u) >> g == 1u) {
+                    mma_commit(bar_empty + k_st * 8);
+                    step2(k_st, k_ph);
+                }
+            };
 #pragma unroll 1
-                for (int g = 0; g < 2 && alive; ++g) {
-                    const uint32_t tmem_s = tmem + g * 128, tmem_o = tmem + 256 + g * D, tmem_p = D == 128 ? tmem_s : tmem + 384 + g * 64;
-                    if (on_b >> g & 1) {
-                        if (g == 0 || on_b == 2) alive = mbar_wait(bar_full + v_st * 8, v_ph, a.status, where);
-                        alive = alive && mbar_wait(bar_p + g * 16, p_ph >> g & 1, a.status, where);
-                        if (!alive) break;
-                        fence_after_sync();
-                        const uint64_t dvs = dv + uint64_t(v_st * (TILE >> 4));
-#pragma unroll
-                        for (int ks = 0; ks < 8; ++ks) {
-                            if (ks == 4) {
-                                alive = mbar_wait(bar_p + g * 16 + 8, p_ph >> g & 1, a.status, where);
-                                fence_after_sync();
-                            }
-                            if (ks < steps_b) mma_f16_ts(tmem_o, tmem_p + ks * 8, dvs + uint64_t((ks * 16 * 128) >> 4), idesc_pv, ks > 0 || !(first_b >> g & 1));
-                        }
-                        p_ph ^= 1u << g;
-                        if (last_b >> g & 1) mma_commit(bar_o + g * 8);
-                        if (on_b >> g == 1) {             // the last group to read this V
-                            mma_commit(bar_empty + v_st * 8);
-                            step2(v_st, v_ph);
-                        }
-                    }
-                    if ((on >> g & 1) && alive) {
-                        if (g == 0 || on == 2) alive = mbar_wait(bar_full + k_st * 8, k_ph, a.status, where);
-                        if (first_here >> g & 1) {
-                            alive = alive && mbar_wait(bar_q + (qbuf * 2 + g) * 8, q_ph >> (qbuf * 2 + g) & 1, a.status, where);
-                            q_ph ^= 1u << (qbuf * 2 + g);
-                        }
-                        if (!alive) break;
-                        fence_after_sync();
-                        const uint64_t dqs = dq + uint64_t((qbuf * 2 + g) * (TILE >> 4)), dks = dk + uint64_t(k_st * (TILE >> 4));
-#pragma unroll
-                        for (int ks = 0; ks < D / 16; ++ks) {
-                            const uint64_t koff = ((ks >> 2) * HALF + (ks & 3) * 32) >> 4;
-                            mma_f16(tmem_s, dqs + koff, dks + koff, idesc_s, ks > 0);
-                        }
-                        mma_commit(bar_s + g * 8);
-                        if (last_here >> g & 1) mma_commit(bar_qfree + (qbuf * 2 + g) * 8);
-                        if (on >> g == 1) {
-                            mma_commit(bar_empty + k_st * 8);
-                            step2(k_st, k_ph);
-                        }
-                    }
+            while (alive) {
+                alive = mbar_wait(bar_full + k_st * 8, k_ph, a.status, where);
+                if (!alive) break;
+                fence_after_sync();
+                now = plan[k_st];
+                if (before != 0u) {
+                    alive = mbar_wait(bar_full + v_st * 8, v_ph, a.status, where);
+                    fence_after_sync();
                 }
-                steps_b = steps;
-                on_b = on;
-                first_b = first_here;
-                last_b = last_here;
-                if (i + 1 < n_tiles) me.next(line);
+                if (alive && (before & 16u)) second_product(std::integral_constant<int, 0>());
+                if (alive && (now & 16u)) first_product(std::integral_constant<int, 0>());
+                if (alive && (before & 32u)) second_product(std::integral_constant<int, 1>());
+                if (alive && (now & 32u)) first_product(std::integral_constant<int, 1>());
+                before = now;
+                if (now == 0u) break;
             }
             mma_commit(bar_end);                          // all products are done before tensor memory is given back
             mbar_wait(bar_end, 0, a.status, where);
@@ -323,8 +400,56 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
             if (i + len < n_tiles) me.next(line);
         }
     } else {
-        // ====== V tiles that not every row attends to all of ======
         const int t128 = tid - 384;
+        if constexpr (QUANT) {
+            // ====== 8-bit tiles into 16-bit ones, a thread per row: a scale each, and rows of a swizzled tile are free of conflicts ======
+            int st = 0, rs = 0, item = 0;
+            uint32_t use = 0, turn = 0;
+            bool alive = true;
+#pragma unroll 1
+            for (int i = 0; i <= n_tiles; ++i) {
+                if (i > 0 && i < n_tiles && me.tile == 0) ++item;
+                const int key0 = me.tile * G::KEYS;
+                if (i == n_tiles || me.keys > 0) {
+                    const bool edge = key0 + G::KEYS > first_limit();
+                    const int have = me.kv - key0;        // V rows behind the sequence's end become zeros
+#pragma unroll 1
+                    for (int v = 0; v < (i < n_tiles ? 2 : 1); ++v) {
+                        if (alive) alive = mbar_wait(bar_in + rs * 8, turn & 1, a.status, where);
+                        if (alive && use > 0) alive = mbar_wait(bar_empty + st * 8, (use - 1) & 1, a.status, where);
+                        if (i < n_tiles) {
+                            const uint32_t b = smem[G::OFF_SCALES + rs * 128 + t128];
+                            bool none = false;            // a V row that is left out
+                            if (v) {
+                                none = t128 >= have;
+                                if (edge && !none && b == 255u) {
+                                    none = true;
+                                    atomicMin_block(const_cast<int *>(note), item);
+                                }
+                            }
+                            widen_row<T, D>(s_base + G::OFF_RAW + rs * 128 * D, s_ring + st * TILE, t128, b, none);
+                            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                        }
+                        asm volatile("bar.sync 2, 128;\n" ::: "memory");
+                        if (t128 == 0) {
+                            if (v == 0) plan[st] = raw_plan[rs];
+                            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar_full + st * 8) : "memory");
+                            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar_out + rs * 8) : "memory");
+                        }
+                        if (++st == RING) {
+                            st = 0;
+                            ++use;
+                        }
+                        if (++rs == RAW) {
+                            rs = 0;
+                            ++turn;
+                        }
+                    }
+                }
+                if (i + 1 < n_tiles) me.next(line);
+            }
+        } else {
+        // ====== V tiles that not every row attends to all of ======
         int st = 1, item = 0;                             // stage of the tile's V
         uint32_t raw_ph = 0;
         bool alive = true;
@@ -377,6 +502,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
             }
             if (i + 1 < n_tiles) me.next(line);
         }
+        }
         if (t128 == 0 && a.part != nullptr) leave_cut<G::ROWS, D>(a, me, total, n_tiles);
     }
     } else {
@@ -390,6 +516,20 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
         uint32_t s_ph = 0, o_ph = 0;
         int item = 0, len;
         bool alive = true;
+        auto announce = [&](uint32_t bar) {
+            tmem_st_wait();
+            fence_before_sync();
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+        };
+        // probabilities of two scores, into the row's sum and as a pair of 16-bit values
+        auto exp2_pair = [&](uint64_t x, uint64_t &sum, uint32_t &out) {
+            float p0, p1;
+            unpair(x, p0, p1);
+            p0 = fast_exp2(p0);
+            p1 = fast_exp2(p1);
+            sum = add2(sum, pair(p0, p1));
+            out = MT::pack(p0, p1);
+        };
 #pragma unroll 1
         for (int i = 0; i < n_tiles; i += len, ++item) {
             len = min(me.tiles - me.tile, n_tiles - i);
@@ -416,17 +556,34 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
                         for (int k = 0; k < 32; ++k)
                             if (c * 32 + k >= n) s[c][k] = 0xff800000u;
                 }
-                float mx4[4];
+                // The exponentials of the first half are taken against the reference that the tiles before left, and the row's maximum in
+                // between (an exponential keeps its unit for 8 cycles, a maximum fits in).  Where a row has outgrown the reference by more
+                // than 2^8 - on a piece's first tile always - it moves, what was summed so far with it, and they are taken again.
+                uint64_t l2[2], scale2 = pair(c2, c2), shift2;
+                uint32_t packed[2][16];
+#pragma unroll 1
+                for (int again = 0;; ++again) {
+                    const float mu = m_ref == -INFINITY ? 0.f : m_ref * c2;
+                    shift2 = pair(-mu, -mu);
+                    float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+                    l2[0] = l2[1] = 0;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    mx4[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
+                    for (int c = 0; c < 2; ++c)
 #pragma unroll
-                    for (int k = 2; k < 32; k += 2) mx4[c] = max3(mx4[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
-                }
-                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                // the reference moves when a row has outgrown it by more than 2^8 (always on its first live tile)
-                const bool up = (mx - m_ref) * c2 > 8.f;
-                if (__any_sync(0xffffffffu, up)) {
+                        for (int k = 0; k < 32; k += 2) {
+                            const float x0 = __uint_as_float(s[c][k]), x1 = __uint_as_float(s[c][k + 1]);
+                            exp2_pair(fma2(pair(x0, x1), scale2, shift2), l2[(k >> 1) & 1], packed[c][k >> 1]);
+                            if ((k >> 1) & 1) {
+                                m0 = max3(m0, x0, x1);
+                                m1 = max3(m1, __uint_as_float(s[c + 2][k]), __uint_as_float(s[c + 2][k + 1]));
+                            } else {
+                                m2 = max3(m2, x0, x1);
+                                m3 = max3(m3, __uint_as_float(s[c + 2][k]), __uint_as_float(s[c + 2][k + 1]));
+                            }
+                        }
+                    const float mx = max3(fmaxf(m0, m1), m2, m3);
+                    const bool up = (mx - m_ref) * c2 > 8.f;
+                    if (again > 0 || !__any_sync(0xffffffffu, up)) break;
                     if (j > 0) {                          // (S of this tile has landed: O += P V of the one before is done)
                         const float alpha = up ? fast_exp2((m_ref - mx) * c2) : 1.f;
 #pragma unroll 1
@@ -442,33 +599,18 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
                     }
                     if (up) m_ref = mx;
                 }
-                const float mu = m_ref == -INFINITY ? 0.f : m_ref * c2;
-                const uint64_t scale2 = pair(c2, c2), shift2 = pair(-mu, -mu);
-                uint64_t l2[2] = {0, 0};
+                tmem_st16(tmem_p, packed[0]);
+                tmem_st16(tmem_p + 16, packed[1]);
+                announce(my_p);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t packed[16];
+                for (int c = 0; c < 2; ++c) {
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        const uint64_t x = fma2(pair(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), scale2, shift2);
-                        float p0, p1;
-                        if ((k >> 1) % 4 == 3) {
-                            exp2_poly(x, p0, p1);
-                        } else {
-                            unpair(x, p0, p1);
-                            p0 = fast_exp2(p0);
-                            p1 = fast_exp2(p1);
-                        }
-                        l2[(k >> 1) & 1] = add2(l2[(k >> 1) & 1], pair(p0, p1));
-                        packed[k >> 1] = MT::pack(p0, p1);
-                    }
-                    tmem_st16(tmem_p + c * 16, packed);
-                    if (c & 1) {
-                        tmem_st_wait();
-                        fence_before_sync();
-                        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(my_p + (c >> 1) * 8) : "memory");
-                    }
+                    for (int k = 0; k < 32; k += 2)
+                        exp2_pair(fma2(pair(__uint_as_float(s[c + 2][k]), __uint_as_float(s[c + 2][k + 1])), scale2, shift2), l2[(k >> 1) & 1],
+                                  packed[c][k >> 1]);
+                    tmem_st16(tmem_p + 32 + c * 16, packed[c]);
                 }
+                announce(my_p + 8);
                 float la, lb;
                 unpair(add2(l2[0], l2[1]), la, lb);
                 l += la + lb;
@@ -496,7 +638,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
                     tmem_ld_wait(w);
 #pragma unroll
                     for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(w[k]);
-                    if (bad) add_not_finite<T, 32>(a, me.z, me.h, look_from, look_to, c0, o);
+                    if (bad) add_not_finite<T, 32, QUANT>(a, me.z, me.h, look_from, look_to, c0, o);
                 } else {
 #pragma unroll
                     for (int k = 0; k < 32; ++k) o[k] = 0.f;
@@ -531,16 +673,16 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool QUANT>
 static cudaError_t launch_chunk_umma(const ChunkArgs &a, const CUtensorMap &tk, const CUtensorMap &tv, int n_ctas, cudaStream_t stream) {
-    using G = ChunkUmmaGeo<D>;
+    using G = ChunkUmmaGeo<D, QUANT>;
     static_assert(G::BYTES <= 227 * 1024, "one CTA's shared memory");
     static DeviceOnce configured;
     const cudaError_t ce = configured.run([&] {
-        return cudaFuncSetAttribute(chunk_umma_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::BYTES);
+        return cudaFuncSetAttribute(chunk_umma_kernel<T, D, QUANT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::BYTES);
     });
     if (ce != cudaSuccess) return ce;
-    const cudaError_t e = launch_serialised(chunk_umma_kernel<T, D>, dim3(n_ctas), dim3(G::THREADS), G::BYTES, stream, a, tk, tv);
+    const cudaError_t e = launch_serialised(chunk_umma_kernel<T, D, QUANT>, dim3(n_ctas), dim3(G::THREADS), G::BYTES, stream, a, tk, tv);
     if (e != cudaSuccess || !chunk_splits(a, G::KEYS)) return e;
     return launch_chunk_combine<T, D, G::ROWS>(a, n_ctas, stream);
 }
