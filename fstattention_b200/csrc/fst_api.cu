@@ -45,6 +45,8 @@ static cudaError_t launch_tree_umma(const AttnArgs &a, int dtype, cudaStream_t s
 }
 
 static int elem_size(int dtype) { return dtype == FST_F32 ? 4 : 2; }
+// TMA reads rows of 128 bytes: off their boundary they cost twice the sectors (503 instead of 900 TFLOP/s)
+static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static bool mma_ok(int dtype, int D, int bm) {
     return (dtype == FST_F16 || dtype == FST_BF16) && (D == 64 || D == 128) &&
@@ -520,10 +522,14 @@ int fst_cache_read(const fst_paged_cache *cache, void *k, void *v, const int32_t
 size_t fst_attention_chunk_workspace_bytes(const fst_paged_cache *cache, int Z, int H, int H_kv, int n_q, int head_dim) {
     ChunkArgs a = {};
     if (Z <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || n_q <= 0 || open_cache(a.c, cache, head_dim, FST_F16) != FST_OK) return 0;
-    if (!chunk_splits(a, 128)) return 0;
+    a.Z = Z;
+    a.H_kv = H_kv;
     a.n_q = n_q;
     a.group = H / H_kv;
-    return chunk_part_bytes(chunk_ctas(), chunk_row_tile(a), head_dim);
+    size_t bytes = chunk_splits(a, 128) ? chunk_part_bytes(chunk_ctas(), chunk_row_tile(a), head_dim) : 0;
+    if (chunk_expands(a, head_dim))                       // behind the pieces: K, V, the table
+        bytes = align256(bytes) + size_t(chunk_expanded_bytes(a, head_dim)) + size_t(Z) * a.c.width * 4;
+    return bytes;
 }
 
 int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cache *cache, const int32_t *kv_lens,
@@ -548,10 +554,24 @@ int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cach
     a.os_z = o_stride_z; a.os_h = o_stride_h; a.os_n = o_stride_n;
     a.scale_log2 = sm_scale * 1.4426950408889634f;
     a.causal = causal != 0;
-    a.part = need > 0 ? static_cast<float *>(workspace) : nullptr;
-    a.status = status;
     const int n_ctas = chunk_ctas();
+    const bool splits = chunk_splits(a, 128);
+    a.part = splits ? static_cast<float *>(workspace) : nullptr;
+    a.status = status;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (chunk_expands(a, head_dim)) {
+        unsigned char *at = static_cast<unsigned char *>(workspace) + (splits ? align256(chunk_part_bytes(n_ctas, chunk_row_tile(a), head_dim)) : 0);
+        const size_t pool = size_t(chunk_expanded_bytes(a, head_dim)) / 2;
+        const ExpandArgs x{a.c, at, at + pool, reinterpret_cast<int32_t *>(at + 2 * pool), kv_lens, Z, H_kv, status};
+        const cudaError_t e = launch_cache_expand(x, dtype, head_dim, st);
+        if (e != cudaSuccess) return cuda_status(e);
+        a.c.k_pool = x.k; a.c.v_pool = x.v; a.c.k_scale = a.c.v_scale = nullptr;
+        a.c.table = x.table;
+        a.c.n_pages = Z * a.c.width;
+        a.c.stride_row = head_dim;
+        a.c.stride_head = int64_t(head_dim) << a.c.page_shift;
+        a.c.stride_page = a.c.stride_head * H_kv;
+    }
     if (dtype == FST_F16)
         return cuda_status(head_dim == 64 ? launch_chunk_f16_d64(a, n_ctas, st) : launch_chunk_f16_d128(a, n_ctas, st));
     return cuda_status(head_dim == 64 ? launch_chunk_bf16_d64(a, n_ctas, st) : launch_chunk_bf16_d128(a, n_ctas, st));

@@ -146,6 +146,69 @@ cache_read_kernel(const ReadArgs a) {
     *reinterpret_cast<uint4 *>(static_cast<T *>(a.v) + z * a.vs_z + h * a.vs_h + r * a.vs_n + col) = v;
 }
 
+// A block takes pages of one head, every gridDim.x-th of all that hold rows; the lengths are read once per 256 sequences.
+template <typename T, int D>
+__global__ void __launch_bounds__(CACHE_THREADS)
+cache_expand_kernel(const ExpandArgs a) {
+    constexpr int LPR = D / 8, RPB = CACHE_THREADS / LPR;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    __shared__ int pages[256];
+    const int col = (threadIdx.x % LPR) * 8, ps = 1 << a.c.page_shift;
+    unsigned skip = blockIdx.x;                           // units ahead of my next one
+#pragma unroll 1
+    for (int z0 = 0; z0 < a.Z; z0 += 256) {
+        __syncthreads();
+        if (z0 + int(threadIdx.x) < a.Z) pages[threadIdx.x] = min((max(__ldg(a.lens + z0 + threadIdx.x), 0) + ps - 1) >> a.c.page_shift, a.c.width);
+        __syncthreads();
+#pragma unroll 1
+        for (int z = z0; z < min(a.Z, z0 + 256); ++z) {
+            const unsigned n = unsigned(pages[z - z0]) * unsigned(a.H_kv);
+#pragma unroll 1
+            for (; skip < n; skip += gridDim.x) {
+                const int idx = int(skip / unsigned(a.H_kv)), h = int(skip - unsigned(idx) * unsigned(a.H_kv));
+                const size_t to_page = size_t(z) * a.c.width + idx;
+                const int page = __ldg(a.c.table + to_page);
+                const bool bad = unsigned(page) >= unsigned(a.c.n_pages);        // its rows read as zeros: no page of the new pool either
+                if (h == 0 && threadIdx.x == 0) {
+                    if (bad) report(a.status, FST_DEV_INDEX_RANGE, z, idx << a.c.page_shift);
+                    a.table[to_page] = bad ? -1 : int(to_page);
+                }
+                if (bad) continue;
+#pragma unroll 2
+                for (int r = threadIdx.x / LPR; r < ps; r += RPB) {
+                    const int64_t from = page * a.c.stride_page + r * a.c.stride_row + h * a.c.stride_head + col;
+                    const size_t at = ((size_t(page) * a.H_kv + h) << a.c.page_shift) + r, to = (((to_page * a.H_kv + h) << a.c.page_shift) + r) * D + col;
+                    const uint2 bk = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.k_pool) + from));
+                    const uint2 bv = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.v_pool) + from));
+                    const float ek = e8m0_value(__ldg(a.c.k_scale + at)), ev = e8m0_value(__ldg(a.c.v_scale + at));
+                    *reinterpret_cast<uint4 *>(static_cast<T *>(a.k) + to) = expand8<T>(bk, ek);
+                    *reinterpret_cast<uint4 *>(static_cast<T *>(a.v) + to) = expand8<T>(bv, ev);
+                }
+            }
+            skip -= n;
+        }
+    }
+}
+
+template <typename T, int D>
+static cudaError_t launch_expand_t(const ExpandArgs &a, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(8 * sm_count());
+    cfg.blockDim = dim3(CACHE_THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, cache_expand_kernel<T, D>, a);
+}
+cudaError_t launch_cache_expand(const ExpandArgs &a, int dtype, int D, cudaStream_t stream) {
+    if (dtype == FST_F16) return D == 128 ? launch_expand_t<__half, 128>(a, stream) : launch_expand_t<__half, 64>(a, stream);
+    return D == 128 ? launch_expand_t<__nv_bfloat16, 128>(a, stream) : launch_expand_t<__nv_bfloat16, 64>(a, stream);
+}
+
 // One lane group per row; launched so that the grid may become resident while the one ahead of it drains.
 template <int D, typename K, typename A>
 static cudaError_t launch_rows(K kernel, const A &a, cudaStream_t stream) {

@@ -77,6 +77,17 @@ struct ReadArgs {
     int Z, H_kv, M;
     int32_t *status;
 };
+// An 8-bit cache as a 16-bit one of the same pages' rows: page i of sequence z is page z * width + i of the pools k, v, contiguous
+// [Z * width][H_kv][page_size][D], as table says, [Z][width].  Only pages with rows are written.
+struct ExpandArgs {
+    CacheArgs c;
+    void *k, *v;
+    int32_t *table;
+    const int32_t *lens;
+    int Z, H_kv;
+    int32_t *status;
+};
+cudaError_t launch_cache_expand(const ExpandArgs &a, int dtype, int D, cudaStream_t stream);
 cudaError_t launch_cache_append(const AppendArgs &a, int dtype, int D, cudaStream_t stream);
 cudaError_t launch_cache_read(const ReadArgs &a, int dtype, int D, cudaStream_t stream);
 

@@ -281,65 +281,86 @@ __device__ __forceinline__ void leave_cut(const ChunkArgs &a, const ChunkCursor<
     reinterpret_cast<ChunkCut *>(a.part + chunk_cuts_at(gridDim.x, ROWS, D))[blockIdx.x] = cut;
 }
 
-// The pieces of the item that CTA x's last piece begins, merged in their order: a warp per row, eight rows of the item per block.
+// The pieces of the item that CTA x's last piece begins, merged in their order: a warp for RPW rows at a time, eight warps a block.
 // The factors of up to 32 pieces are taken by a lane each, so that nothing but the additions is a chain.
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(256)
 chunk_combine_kernel(const ChunkArgs a, int n_ctas) {
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    constexpr int C = D / 32;                             // columns of a lane
+    constexpr int C = D / 32, RPW = ROWS >= 32 ? 4 : 2;   // columns of a lane, rows of a warp
     const ChunkCut it = reinterpret_cast<const ChunkCut *>(a.part + chunk_cuts_at(n_ctas, ROWS, D))[blockIdx.x];
-    const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int r = it.qt * ROWS + row, tok = r / a.group, head = it.h * a.group + (r - tok * a.group);
-    if (it.pieces <= 1 || tok >= it.ql) return;
+    const int row0 = (blockIdx.y * 8 + (threadIdx.x >> 5)) * RPW, lane = threadIdx.x & 31;
+    if (it.pieces <= 1 || it.qt * ROWS + row0 >= it.ql * a.group) return;
     const float2 *stats = reinterpret_cast<const float2 *>(a.part + chunk_stats_at(n_ctas, ROWS, D));
-    auto slot = [&](int piece) { return (size_t(2) * (blockIdx.x + piece) + (piece == 0 ? 1 : 0)) * ROWS + row; };
-    float acc[C] = {}, top = -INFINITY, sum = 0.f;
+    auto slot = [&](int piece) { return (size_t(2) * (blockIdx.x + piece) + (piece == 0 ? 1 : 0)) * ROWS + row0; };
+    float acc[RPW][C] = {}, top[RPW], sum[RPW];
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) {
+        top[i] = -INFINITY;
+        sum[i] = 0.f;
+    }
 #pragma unroll 1
     for (int p0 = 0; p0 < it.pieces; p0 += 32) {
         const int n = min(32, it.pieces - p0);
-        const float2 st = lane < n ? stats[slot(p0 + lane)] : make_float2(-INFINITY, 0.f);
-        float now = st.x;
+        float2 st[RPW];
+        float w[RPW];
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, s));
-        now = fmaxf(now, top);
-        // a piece that saw nothing has no part in it; one whose scores were all NaN has no exponent, but a sum
-        const float w = st.x == -INFINITY ? (st.y == 0.f ? 0.f : 1.f) : fast_exp2(st.x - now);
-        const float w_old = top == -INFINITY ? 1.f : fast_exp2(top - now);
-        float part = st.y * w;
+        for (int i = 0; i < RPW; ++i) st[i] = lane < n ? stats[slot(p0 + lane) + i] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) part += __shfl_xor_sync(0xffffffffu, part, s);
-        sum = sum * w_old + part;
-        top = now;
+        for (int i = 0; i < RPW; ++i) {
+            float now = st[i].x;
 #pragma unroll
-        for (int k = 0; k < C; ++k) acc[k] *= w_old;
-#pragma unroll 8
+            for (int s = 16; s > 0; s >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, s));
+            now = fmaxf(now, top[i]);
+            // a piece that saw nothing has no part in it; one whose scores were all NaN has no exponent, but a sum
+            w[i] = st[i].x == -INFINITY ? (st[i].y == 0.f ? 0.f : 1.f) : fast_exp2(st[i].x - now);
+            const float w_old = top[i] == -INFINITY ? 1.f : fast_exp2(top[i] - now);
+            float part = st[i].y * w[i];
+#pragma unroll
+            for (int s = 16; s > 0; s >>= 1) part += __shfl_xor_sync(0xffffffffu, part, s);
+            sum[i] = sum[i] * w_old + part;
+            top[i] = now;
+#pragma unroll
+            for (int k = 0; k < C; ++k) acc[i][k] *= w_old;
+        }
+#pragma unroll 4
         for (int p = 0; p < n; ++p) {
-            const float f = __shfl_sync(0xffffffffu, w, p);
             const float *from = a.part + slot(p0 + p) * D + lane * C;
-            float v[C];
-            if constexpr (C == 4) {
-                const float4 x = *reinterpret_cast<const float4 *>(from);
-                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-            } else {
-                const float2 x = *reinterpret_cast<const float2 *>(from);
-                v[0] = x.x; v[1] = x.y;
-            }
 #pragma unroll
-            for (int k = 0; k < C; ++k) acc[k] = f == 0.f ? acc[k] : fmaf(v[k], f, acc[k]);
+            for (int i = 0; i < RPW; ++i) {
+                const float f = __shfl_sync(0xffffffffu, w[i], p);
+                float v[C];
+                if constexpr (C == 4) {
+                    const float4 x = *reinterpret_cast<const float4 *>(from + i * D);
+                    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+                } else {
+                    const float2 x = *reinterpret_cast<const float2 *>(from + i * D);
+                    v[0] = x.x; v[1] = x.y;
+                }
+#pragma unroll
+                for (int k = 0; k < C; ++k) acc[i][k] = f == 0.f ? acc[i][k] : fmaf(v[k], f, acc[i][k]);      // (not written where f is zero)
+            }
         }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T *dst = static_cast<T *>(a.o) + it.z * a.os_z + head * a.os_h + tok * a.os_n + lane * C;
-    if constexpr (C == 4) *reinterpret_cast<uint2 *>(dst) = make_uint2(MmaTraits<T>::pack(acc[0] * inv, acc[1] * inv), MmaTraits<T>::pack(acc[2] * inv, acc[3] * inv));
-    else *reinterpret_cast<uint32_t *>(dst) = MmaTraits<T>::pack(acc[0] * inv, acc[1] * inv);
-    if (a.lse != nullptr && lane == 0) a.lse[(size_t(it.z) * a.H + head) * a.n_q + tok] = sum == 0.f ? -INFINITY : top + log2f(sum);
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) {
+        const int r = it.qt * ROWS + row0 + i, tok = r / a.group, head = it.h * a.group + (r - tok * a.group);
+        if (tok >= it.ql) continue;
+        const float inv = sum[i] == 0.f ? 0.f : 1.f / sum[i];
+        T *dst = static_cast<T *>(a.o) + it.z * a.os_z + head * a.os_h + tok * a.os_n + lane * C;
+        if constexpr (C == 4)
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(MmaTraits<T>::pack(acc[i][0] * inv, acc[i][1] * inv), MmaTraits<T>::pack(acc[i][2] * inv, acc[i][3] * inv));
+        else
+            *reinterpret_cast<uint32_t *>(dst) = MmaTraits<T>::pack(acc[i][0] * inv, acc[i][1] * inv);
+        if (a.lse != nullptr && lane == 0) a.lse[(size_t(it.z) * a.H + head) * a.n_q + tok] = sum[i] == 0.f ? -INFINITY : top[i] + log2f(sum[i]);
+    }
 }
 
 template <typename T, int D, int ROWS>
 cudaError_t launch_chunk_combine(const ChunkArgs &a, int n_ctas, cudaStream_t stream) {
-    return launch_serialised(chunk_combine_kernel<T, D, ROWS>, dim3(n_ctas, ROWS / 8), dim3(256), 0, stream, a, n_ctas);
+    constexpr int PER_BLOCK = 8 * (ROWS >= 32 ? 4 : 2);
+    return launch_serialised(chunk_combine_kernel<T, D, ROWS>, dim3(n_ctas, ROWS / PER_BLOCK), dim3(256), 0, stream, a, n_ctas);
 }
 
 // CTAs of a call's line: one per SM (a workspace holds two pieces for each).
@@ -347,6 +368,14 @@ inline int chunk_ctas() { return sm_count(); }
 // Which kernel: up to 32 rows the mma.sync one.
 inline bool chunk_many_rows(const ChunkArgs &a) { return (long long)a.n_q * a.group > 32; }
 inline int chunk_row_tile(const ChunkArgs &a) { return chunk_many_rows(a) ? 256 : (long long)a.n_q * a.group <= 16 ? 16 : 32; }
+// An 8-bit cache under many queries is expanded once, ahead of the call, rather than by every row tile on its way: from two row tiles of
+// a K/V head on that is no slower (512 rows of 8 heads over 16384: 125 us on the way, 126 expanded; 8192 rows over 8192: 410 and
+// ...), but only as long as the copy of all that the tables can hold stays below 2 GB.
+constexpr long long kMostExpanded = 2LL << 30;
+inline long long chunk_expanded_bytes(const ChunkArgs &a, int D) { return 4LL * a.Z * a.c.width * a.H_kv * D << a.c.page_shift; }
+inline bool chunk_expands(const ChunkArgs &a, int D) {
+    return a.c.k_scale != nullptr && (long long)a.n_q * a.group >= 512 && (long long)a.Z * a.c.width < 0x7fffffffLL && chunk_expanded_bytes(a, D) <= kMostExpanded;
+}
 // Whether any piece can be less than an item: not if all that the table can hold is one key tile.
 inline bool chunk_splits(const ChunkArgs &a, int keys) { return ((long long)a.c.width << a.c.page_shift) > keys; }
 
