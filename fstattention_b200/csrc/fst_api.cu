@@ -542,7 +542,7 @@ int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cach
     const int rc = open_cache(a.c, cache, head_dim, dtype);
     if (rc != FST_OK) return rc;
     if ((long long)n_q * (H / H_kv) > 0x7fffffffLL - 1024) return FST_ERR_TOO_LARGE;
-    if (!aligned16(q) || !aligned16(o) || !aligned16(workspace) ||
+    if (!aligned16(q) || !aligned16(o) || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
         !aligned_strides({q_stride_z, q_stride_h, q_stride_n, o_stride_z, o_stride_h, o_stride_n}))
         return FST_ERR_ALIGNMENT;
     const size_t need = fst_attention_chunk_workspace_bytes(cache, Z, H, H_kv, n_q, head_dim);

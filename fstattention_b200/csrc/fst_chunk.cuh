@@ -31,6 +31,7 @@ struct ChunkArgs {
     int64_t qs_z, qs_h, qs_n, os_z, os_h, os_n;
     float scale_log2;                      // sm_scale * log2(e), positive
     int causal;
+    int q_boxes;                           // Q comes as boxes of `group` heads by 128 / group tokens
     float *part;                           // pieces: [2 CTAs][rows][D] sums, [2 CTAs][rows] (exponent, sum), [CTAs] ChunkCut
     int32_t *status;
 };

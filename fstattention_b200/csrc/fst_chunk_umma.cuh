@@ -48,6 +48,11 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
     asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(x), "f"(y), "f"(z));
     return r;
 }
+// 32 bytes to an address on their boundary
+__device__ __forceinline__ void store32(void *to, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n"
+                 ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
 // whether one of the pairs of 16-bit values has an exponent of ones: the top bit of a half that overflows into it
 template <typename T>
 __device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
@@ -118,7 +123,7 @@ __device__ __forceinline__ void widen_row(uint32_t from, uint32_t to, int r, uin
 
 template <typename T, int D, bool QUANT>
 __global__ void __launch_bounds__(512, 1)
-chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
     using namespace umma;
     using G = ChunkUmmaGeo<D, QUANT>;
     using MT = MmaTraits<T>;
@@ -146,7 +151,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
         if (lane == 0) {
             for (int i = 0; i < 3 * RING; ++i) mbar_init(bar_full + i * 8, 1);
             for (int i = 0; i < 2 * QBUF; ++i) {
-                mbar_init(bar_q + i * 8, 64);
+                mbar_init(bar_q + i * 8, a.q_boxes ? 1 : 64);
                 mbar_init(bar_qfree + i * 8, 1);
             }
             for (int i = 0; i < 2; ++i) {
@@ -379,7 +384,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
             mbar_wait(bar_end, 0, a.status, where);
         }
     } else if (warp == 10 || warp == 11) {
-        // ====== rows of Q, an item (D 128) or two ahead of its products' end ======
+        // ====== rows of Q, an item (D 128) or two ahead of its products' end: one box where whole tokens fit a tile (3 us sooner) ======
         const int t64 = tid - 320;
         uint32_t qfree_ph = 0, used = 0;                  // bit: buffer and group
         bool alive = true;
@@ -398,20 +403,31 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
                     qfree_ph ^= 1u << at;
                 }
                 used |= 1u << at;
-                constexpr int CH = D / 8;
+                const int row0 = me.qt * G::ROWS + g * 128, bar = bar_q + at * 8;
+                if (a.q_boxes) {                          // heads of a token side by side, tokens behind the tensor's end as zeros
+                    if (t64 == 0) {
+                        mbar_arrive_expect_tx(bar, TILE);
+#pragma unroll
+                        for (int hf = 0; hf < DH; ++hf) tma_load_4d(s_base + at * TILE + hf * HALF, &tm_q, hf * 64, me.h * a.group, row0 / a.group, me.z, bar);
+                    }
+                    continue;
+                }
+                constexpr int CH = D / 8, STEP = 64 / CH;
                 const int c = t64 % CH;
                 const uint32_t dst = s_base + at * TILE + (c >> 3) * HALF;
+                int tok = (row0 + t64 / CH) / a.group, sub = row0 + t64 / CH - tok * a.group;
 #pragma unroll 4
-                for (int r = t64 / CH; r < 128; r += 64 / CH) {
-                    const int row = me.qt * G::ROWS + g * 128 + r, tok = row / a.group;
+                for (int r = t64 / CH; r < 128; r += STEP) {
                     const bool there = tok < me.ql;
-                    const T *src = static_cast<const T *>(a.q) + me.z * a.qs_z + (me.h * a.group + (row - tok * a.group)) * a.qs_h + tok * a.qs_n + c * 8;
+                    const T *src = static_cast<const T *>(a.q) + me.z * a.qs_z + (me.h * a.group + sub) * a.qs_h + tok * a.qs_n + c * 8;
                     cp_async16(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), there ? src : static_cast<const T *>(a.q), there);
+#pragma unroll 1
+                    for (sub += STEP; sub >= a.group; sub -= a.group) ++tok;
                 }
                 cp_async_commit();
                 cp_async_wait<0>();
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar_q + at * 8) : "memory");
+                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
             }
             me.tile += len - 1;
             if (i + len < n_tiles) me.next(line);
@@ -439,7 +455,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
                             bool none = false;            // a V row that is left out
                             if (v) {
                                 none = t128 >= have;
-                                if (edge && !none && b == 255u) {
+                                if (edge && !none && b == 255u && t128 < ((me.keys - key0 + 15) & ~15)) {
                                     none = true;
                                     atomicMin_block(const_cast<int *>(note), item);
                                 }
@@ -478,25 +494,25 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
                 if (key0 + G::KEYS > first_limit()) {
                     if (alive) alive = mbar_wait(bar_raw + st * 8, raw_ph >> st & 1, a.status, where);
                     raw_ph ^= 1u << st;
-                    // thread: a row's half at D 64, a whole row at D 128; chunks in an order that spreads the rows over the banks
-                    const int have = me.kv - key0;        // rows behind the sequence's end become zeros
-                    constexpr int PER = D / 8;            // chunks of 16 bytes: 128 rows of D / 8 over 128 threads
+                    // Rows that take part, whole 16-key steps of them (what lies behind may be anything, and a look there would find it), and
+                    // rows of the sequence: those behind become zeros.  Neighbouring threads have neighbouring chunks of 16 bytes.
+                    const int rows = (min(G::KEYS, me.keys - key0) + 15) & ~15, have = me.kv - key0;
+                    constexpr int PER = D / 8;            // chunks of a thread
                     unsigned char *tile = smem + G::OFF_RING + st * TILE;
-                    uint32_t odd = 0;
-                    if (have >= G::KEYS) {
+                    uint32_t odd = have < rows;
 #pragma unroll
-                        for (int k = 0; k < PER; ++k) {
-                            const uint4 w = *reinterpret_cast<const uint4 *>(tile + (k * 128 + t128) * 16);
-                            odd |= odd_bits<T>(w.x) | odd_bits<T>(w.y) | odd_bits<T>(w.z) | odd_bits<T>(w.w);
-                        }
-                    } else {
-                        odd = 1u;
+                    for (int k = 0; k < PER; ++k) {
+                        const int at = (k * 128 + t128) * 16;
+                        const uint4 w = *reinterpret_cast<const uint4 *>(tile + at);
+                        const uint32_t bits = odd_bits<T>(w.x) | odd_bits<T>(w.y) | odd_bits<T>(w.z) | odd_bits<T>(w.w);
+                        odd |= at % HALF / 128 < rows ? bits : 0u;
                     }
                     if (odd != 0u) {                      // (the order of a row's chunks does not matter)
                         bool met = false;
 #pragma unroll 1
                         for (int k = 0; k < PER; ++k) {
                             const int at = (k * 128 + t128) * 16, r = at % HALF / 128;
+                            if (r >= rows) continue;
                             uint4 w = *reinterpret_cast<const uint4 *>(tile + at);
                             if (r >= have) {
                                 w = make_uint4(0, 0, 0, 0);
@@ -646,6 +662,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
             const int head = me.h * a.group + (row - tok * a.group);
             const size_t slot = (size_t(2) * blockIdx.x + (me.tile == 0 ? 1 : 0)) * G::ROWS + g * 128 + r;
             T *dst = static_cast<T *>(a.o) + me.z * a.os_z + head * a.os_h + tok * a.os_n;
+            const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
                 float o[32];
@@ -661,15 +678,21 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
                     for (int k = 0; k < 32; ++k) o[k] = 0.f;
                 }
                 if (!there) continue;
-                if (whole) {
+                if (whole) {                              // 32 bytes a store, whole sectors
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8)
-                        *reinterpret_cast<uint4 *>(dst + c0 + k) = make_uint4(MT::pack(o[k] * f, o[k + 1] * f), MT::pack(o[k + 2] * f, o[k + 3] * f),
-                                                                              MT::pack(o[k + 4] * f, o[k + 5] * f), MT::pack(o[k + 6] * f, o[k + 7] * f));
+                    for (int k = 0; k < 32; k += 16) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) w[x] = MT::pack(o[k + 2 * x] * f, o[k + 2 * x + 1] * f);
+                        if (wide) store32(dst + c0 + k, w);
+                        else {
+                            *reinterpret_cast<uint4 *>(dst + c0 + k) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4 *>(dst + c0 + k + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                        }
+                    }
                 } else {
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4)
-                        *reinterpret_cast<float4 *>(a.part + slot * D + c0 + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                    for (int k = 0; k < 32; k += 8) store32(a.part + slot * D + c0 + k, reinterpret_cast<const uint32_t(&)[8]>(o[k]));
                 }
             }
             if (there) {
@@ -691,7 +714,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, c
 }
 
 template <typename T, int D, bool QUANT>
-static cudaError_t launch_chunk_umma(const ChunkArgs &a, const CUtensorMap &tk, const CUtensorMap &tv, int n_ctas, cudaStream_t stream) {
+static cudaError_t launch_chunk_umma(const ChunkArgs &a, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, int n_ctas, cudaStream_t stream) {
     using G = ChunkUmmaGeo<D, QUANT>;
     static_assert(G::BYTES <= 227 * 1024, "one CTA's shared memory");
     static DeviceOnce configured;
@@ -699,7 +722,7 @@ static cudaError_t launch_chunk_umma(const ChunkArgs &a, const CUtensorMap &tk, 
         return cudaFuncSetAttribute(chunk_umma_kernel<T, D, QUANT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::BYTES);
     });
     if (ce != cudaSuccess) return ce;
-    const cudaError_t e = launch_serialised(chunk_umma_kernel<T, D, QUANT>, dim3(n_ctas), dim3(G::THREADS), G::BYTES, stream, a, tk, tv);
+    const cudaError_t e = launch_serialised(chunk_umma_kernel<T, D, QUANT>, dim3(n_ctas), dim3(G::THREADS), G::BYTES, stream, a, tq, tk, tv);
     if (e != cudaSuccess || !chunk_splits(a, G::KEYS)) return e;
     return launch_chunk_combine<T, D, G::ROWS>(a, n_ctas, stream);
 }
