@@ -549,7 +549,8 @@ int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cach
     if (need > 0 && (!workspace || workspace_bytes < need)) return FST_ERR_WORKSPACE;
     a.q = q; a.o = o; a.lse = lse;
     a.kv_lens = kv_lens; a.q_lens = q_lens;
-    a.Z = Z; a.H = H; a.H_kv = H_kv; a.group = H / H_kv; a.n_q = n_q;
+    a.Z = Z; a.H = H; a.H_kv = H_kv; a.n_q = n_q;
+    set_group(a, H / H_kv);
     a.qs_z = q_stride_z; a.qs_h = q_stride_h; a.qs_n = q_stride_n;
     a.os_z = o_stride_z; a.os_h = o_stride_h; a.os_n = o_stride_n;
     a.scale_log2 = sm_scale * 1.4426950408889634f;

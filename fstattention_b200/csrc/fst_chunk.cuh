@@ -29,12 +29,25 @@ struct ChunkArgs {
     const int32_t *kv_lens, *q_lens;       // [Z], q_lens null: n_q everywhere
     int Z, H, H_kv, group, n_q;
     int64_t qs_z, qs_h, qs_n, os_z, os_h, os_n;
+    uint32_t group_mul;                    // x / group = x * group_mul >> group_shift for x in [0, 2^31): see set_group
+    int group_shift;
     float scale_log2;                      // sm_scale * log2(e), positive
     int causal;
     int q_boxes;                           // Q comes as boxes of `group` heads by 128 / group tokens
     float *part;                           // pieces: [2 CTAs][rows][D] sums, [2 CTAs][rows] (exponent, sum), [CTAs] ChunkCut
     int32_t *status;
 };
+
+// With s the smallest number of bits for which 2^s >= d and m = ceil(2^(31 + s) / d), which is below 2^32, m d exceeds 2^(31 + s) by less
+// than 2^s, so x m / 2^(31 + s) exceeds x / d by less than 1 / d for x < 2^31: the same integer.
+inline void set_group(ChunkArgs &a, int group) {
+    a.group = group;
+    int s = 0;
+    while ((1u << s) < unsigned(group)) ++s;
+    a.group_mul = uint32_t(((1ull << (31 + s)) + unsigned(group) - 1) / unsigned(group));
+    a.group_shift = 31 + s;
+}
+__device__ __forceinline__ int by_group(const ChunkArgs &a, int x) { return int(uint64_t(uint32_t(x)) * a.group_mul >> a.group_shift); }
 
 // The line of work for row tiles of ROWS and key tiles of KEYS.
 template <int ROWS, int KEYS>
@@ -51,7 +64,7 @@ struct ChunkLine {
     // keys that the last row of a row tile sees
     __device__ __forceinline__ int keys(int kv, int ql, int qt) const {
         if (!a.causal) return kv;
-        const int last = min(((qt + 1) * ROWS - 1) / a.group, ql - 1);
+        const int last = min(by_group(a, (qt + 1) * ROWS - 1), ql - 1);
         return max(0, min(kv, kv - ql + last + 1));
     }
     // at least one key tile, so that rows which see nothing are written too
@@ -346,7 +359,7 @@ chunk_combine_kernel(const ChunkArgs a, int n_ctas) {
     }
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
-        const int r = it.qt * ROWS + row0 + i, tok = r / a.group, head = it.h * a.group + (r - tok * a.group);
+        const int r = it.qt * ROWS + row0 + i, tok = by_group(a, r), head = it.h * a.group + (r - tok * a.group);
         if (tok >= it.ql) continue;
         const float inv = sum[i] == 0.f ? 0.f : 1.f / sum[i];
         T *dst = static_cast<T *>(a.o) + it.z * a.os_z + head * a.os_h + tok * a.os_n + lane * C;

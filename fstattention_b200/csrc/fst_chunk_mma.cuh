@@ -166,12 +166,12 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
             if (tid == 0 && me.h == 0 && me.qt == 0 && (me.kv != __ldg(a.kv_lens + me.z) || (a.q_lens != nullptr && me.ql != __ldg(a.q_lens + me.z))))
                 report(a.status, FST_DEV_INDEX_RANGE, me.z, __ldg(a.kv_lens + me.z));
             poisoned = false;
-            lim_first = a.causal ? min(me.kv, me.kv - me.ql + me.qt * G::ROWS / a.group + 1) : me.kv;
+            lim_first = a.causal ? min(me.kv, me.kv - me.ql + by_group(a, me.qt * G::ROWS) + 1) : me.kv;
 #pragma unroll
             for (int x = 0; x < MT; ++x) {
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
-                    const int r = me.qt * G::ROWS + x * 16 + hh * 8 + g, tok = r / a.group;
+                    const int r = me.qt * G::ROWS + x * 16 + hh * 8 + g, tok = by_group(a, r);
                     const bool real = tok < me.ql;
                     limit[x][hh] = !real ? 0 : a.causal ? min(me.kv, me.kv - me.ql + tok + 1) : me.kv;
                     m[x][hh] = -INFINITY;
@@ -423,7 +423,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         out[k + 3] += v.w * f;
                     }
                 }
-                const int r = me.qt * G::ROWS + x * 16 + row, tok = r / a.group, head = me.h * a.group + (r - tok * a.group);
+                const int r = me.qt * G::ROWS + x * 16 + row, tok = by_group(a, r), head = me.h * a.group + (r - tok * a.group);
                 if (QUANT) {
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) out[k] *= kTiny;

@@ -29,9 +29,11 @@ struct ChunkUmmaGeo {
     static constexpr int ROWS = 256, KEYS = 128, THREADS = 512;
     static constexpr int TILE = (D / 64) * umma::HALF;              // 128 rows
     static constexpr int QBUF = D == 128 ? 1 : 2;                   // items whose Q is there at a time
-    static constexpr int RING = QUANT ? (D == 128 ? 4 : 6) : (D == 128 ? 5 : 8);
+    static constexpr int RING = QUANT ? (D == 128 ? 3 : 6) : (D == 128 ? 4 : 8);
     static constexpr int RAW = QUANT ? (D == 128 ? 2 : 4) : 0;      // stages of 8-bit tiles: 128 rows of D bytes
-    static constexpr int OFF_RING = QBUF * 2 * TILE, OFF_RAW = OFF_RING + RING * TILE, OFF_BAR = OFF_RAW + RAW * 128 * D;
+    static constexpr int OFF_RING = QBUF * 2 * TILE, OFF_RAW = OFF_RING + RING * TILE;
+    static constexpr int OFF_OUT = OFF_RAW + RAW * 128 * D;         // [softmax warp] 32 rows of 128 bytes on their way out
+    static constexpr int OFF_BAR = OFF_OUT + 8 * 4096;
     static constexpr int BARS = 3 * RING + 2 * RAW + 4 * QBUF + 9;
     static constexpr int OFF_NOTE = (OFF_BAR + BARS * 8 + 15) & ~15;             // first item that held values that are not finite; tensor memory's address
     static constexpr int OFF_SCALES = OFF_NOTE + 16;                // [raw stage] 128 bytes
@@ -47,11 +49,6 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
     float r;
     asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(x), "f"(y), "f"(z));
     return r;
-}
-// 32 bytes to an address on their boundary
-__device__ __forceinline__ void store32(void *to, const uint32_t (&w)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n"
-                 ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 // whether one of the pairs of 16-bit values has an exponent of ones: the top bit of a half that overflows into it
 template <typename T>
@@ -185,10 +182,10 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
     auto group_tiles = [&](int g) {
         if (me.keys == 0 || (g == 1 && me.ql * a.group - me.qt * G::ROWS <= 128)) return 0;
         if (g == 1 || !a.causal) return me.tiles;
-        return line.tiles_of(max(0, min(me.kv, me.kv - me.ql + min((me.qt * G::ROWS + 127) / a.group, me.ql - 1) + 1)));
+        return line.tiles_of(max(0, min(me.kv, me.kv - me.ql + min(by_group(a, me.qt * G::ROWS + 127), me.ql - 1) + 1)));
     };
     // keys that the item's first row sees: tiles past it are not seen whole by every row
-    auto first_limit = [&]() { return a.causal ? min(me.kv, me.kv - me.ql + me.qt * G::ROWS / a.group + 1) : me.kv; };
+    auto first_limit = [&]() { return a.causal ? min(me.kv, me.kv - me.ql + by_group(a, me.qt * G::ROWS) + 1) : me.kv; };
 
     // (Each side asks for its share inside its own branch, since code that both reach gets the lower count; and no function is called
     // there, wait_slow for instance: ptxas then finds no allocation.)
@@ -408,14 +405,14 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                     if (t64 == 0) {
                         mbar_arrive_expect_tx(bar, TILE);
 #pragma unroll
-                        for (int hf = 0; hf < DH; ++hf) tma_load_4d(s_base + at * TILE + hf * HALF, &tm_q, hf * 64, me.h * a.group, row0 / a.group, me.z, bar);
+                        for (int hf = 0; hf < DH; ++hf) tma_load_4d(s_base + at * TILE + hf * HALF, &tm_q, hf * 64, me.h * a.group, by_group(a, row0), me.z, bar);
                     }
                     continue;
                 }
                 constexpr int CH = D / 8, STEP = 64 / CH;
                 const int c = t64 % CH;
                 const uint32_t dst = s_base + at * TILE + (c >> 3) * HALF;
-                int tok = (row0 + t64 / CH) / a.group, sub = row0 + t64 / CH - tok * a.group;
+                int tok = by_group(a, row0 + t64 / CH), sub = row0 + t64 / CH - tok * a.group;
 #pragma unroll 4
                 for (int r = t64 / CH; r < 128; r += STEP) {
                     const bool there = tok < me.ql;
@@ -567,7 +564,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
         for (int i = 0; i < n_tiles; i += len, ++item) {
             len = min(me.tiles - me.tile, n_tiles - i);
             const int mine = min(max(group_tiles(g) - me.tile, 0), len);         // tiles of the piece that my group takes
-            const int row = me.qt * G::ROWS + g * 128 + r, tok = row / a.group;
+            const int row = me.qt * G::ROWS + g * 128 + r, tok = by_group(a, row);
             const int limit = tok >= me.ql ? 0 : a.causal ? min(me.kv, me.kv - me.ql + tok + 1) : me.kv;
             float m_ref = -INFINITY, l = 0.f;
             // keys of the tile that I see, and that every row sees
@@ -591,9 +588,20 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                 }
                 // The exponentials of the first half are taken against the reference that the tiles before left, and the row's maximum in
                 // between (an exponential keeps its unit for 8 cycles, a maximum fits in).  Where a row has outgrown the reference by more
-                // than 2^8 - on a piece's first tile always - it moves, what was summed so far with it, and they are taken again.
+                // than 2^8 it moves, what was summed so far with it, and they are taken again.  On a piece's first tile the maximum comes first.
                 uint64_t l2[2], scale2 = pair(c2, c2), shift2;
                 uint32_t packed[2][16];
+                if (j == 0) {
+                    float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) {
+                            m0 = max3(m0, __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
+                            m1 = max3(m1, __uint_as_float(s[c][k + 2]), __uint_as_float(s[c][k + 3]));
+                        }
+                    m_ref = fmaxf(m0, m1);
+                }
 #pragma unroll 1
                 for (int again = 0;; ++again) {
                     const float mu = m_ref == -INFINITY ? 0.f : m_ref * c2;
@@ -616,20 +624,19 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                         }
                     const float mx = max3(fmaxf(m0, m1), m2, m3);
                     const bool up = (mx - m_ref) * c2 > 8.f;
-                    if (again > 0 || !__any_sync(0xffffffffu, up)) break;
-                    if (j > 0) {                          // (S of this tile has landed: O += P V of the one before is done)
-                        const float alpha = up ? fast_exp2((m_ref - mx) * c2) : 1.f;
+                    if (again > 0 || j == 0 || !__any_sync(0xffffffffu, up)) break;
+                    // (S of this tile has landed: O += P V of the one before is done)
+                    const float alpha = up ? fast_exp2((m_ref - mx) * c2) : 1.f;
 #pragma unroll 1
-                        for (int c0 = 0; c0 < D; c0 += 16) {
-                            uint32_t o[16];
-                            tmem_ld16(o, tmem_o + c0);
+                    for (int c0 = 0; c0 < D; c0 += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o, tmem_o + c0);
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-                            tmem_st16(tmem_o + c0, o);
-                        }
-                        tmem_st_wait();
-                        l *= alpha;
+                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                        tmem_st16(tmem_o + c0, o);
                     }
+                    tmem_st_wait();
+                    l *= alpha;
                     if (up) m_ref = mx;
                 }
                 tmem_st16(tmem_p, packed[0]);
@@ -661,39 +668,52 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
             const float f = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l, mu = m_ref == -INFINITY ? -INFINITY : m_ref * c2;
             const int head = me.h * a.group + (row - tok * a.group);
             const size_t slot = (size_t(2) * blockIdx.x + (me.tile == 0 ? 1 : 0)) * G::ROWS + g * 128 + r;
-            T *dst = static_cast<T *>(a.o) + me.z * a.os_z + head * a.os_h + tok * a.os_n;
-            const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
+            // The rows leave through shared memory, four whole lines of 128 bytes a store: by 16 or 32 bytes of 32 rows at a time a piece took
+            // 5 us to write, by lines ...
+            const uint32_t out_at = s_base + G::OFF_OUT + warp * 4096;
+            const unsigned long long to = reinterpret_cast<unsigned long long>(
+                whole ? static_cast<void *>(static_cast<T *>(a.o) + me.z * a.os_z + head * a.os_h + tok * a.os_n) : static_cast<void *>(a.part + slot * D));
+            const unsigned rows_there = __ballot_sync(0xffffffffu, there);
+            const int width = whole ? 64 : 32;            // columns in 128 bytes
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
-                float o[32];
-                if (mine > 0) {
-                    uint32_t w[32];
-                    tmem_ld32(w, tmem_o + c0);
-                    tmem_ld_wait(w);
+            for (int c0 = 0; c0 < D; c0 += width) {
+#pragma unroll 1
+                for (int c1 = 0; c1 < width; c1 += 32) {
+                    float o[32];
+                    if (mine > 0) {
+                        uint32_t w[32];
+                        tmem_ld32(w, tmem_o + c0 + c1);
+                        tmem_ld_wait(w);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(w[k]);
-                    if (bad) add_not_finite<T, 32, QUANT>(a, me.z, me.h, look_from, look_to, c0, o);
-                } else {
+                        for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(w[k]);
+                        if (bad) add_not_finite<T, 32, QUANT>(a, me.z, me.h, look_from, look_to, c0 + c1, o);
+                    } else {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = 0.f;
-                }
-                if (!there) continue;
-                if (whole) {                              // 32 bytes a store, whole sectors
-#pragma unroll
-                    for (int k = 0; k < 32; k += 16) {
-                        uint32_t w[8];
-#pragma unroll
-                        for (int x = 0; x < 8; ++x) w[x] = MT::pack(o[k + 2 * x] * f, o[k + 2 * x + 1] * f);
-                        if (wide) store32(dst + c0 + k, w);
-                        else {
-                            *reinterpret_cast<uint4 *>(dst + c0 + k) = make_uint4(w[0], w[1], w[2], w[3]);
-                            *reinterpret_cast<uint4 *>(dst + c0 + k + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-                        }
+                        for (int k = 0; k < 32; ++k) o[k] = 0.f;
                     }
-                } else {
+                    auto put = [&](int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(out_at + lane * 128 + ((chunk ^ (lane & 7)) << 4)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+                    };
+                    if (whole) {
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8) store32(a.part + slot * D + c0 + k, reinterpret_cast<const uint32_t(&)[8]>(o[k]));
+                        for (int k = 0; k < 32; k += 8)
+                            put((c1 + k) >> 3, MT::pack(o[k] * f, o[k + 1] * f), MT::pack(o[k + 2] * f, o[k + 3] * f), MT::pack(o[k + 4] * f, o[k + 5] * f),
+                                MT::pack(o[k + 6] * f, o[k + 7] * f));
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4)
+                            put(k >> 2, __float_as_uint(o[k]), __float_as_uint(o[k + 1]), __float_as_uint(o[k + 2]), __float_as_uint(o[k + 3]));
+                    }
                 }
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int from = k * 4 + (lane >> 3), chunk = lane & 7;
+                    const uint4 v = lds128(out_at + from * 128 + ((chunk ^ (from & 7)) << 4));
+                    unsigned char *dst = reinterpret_cast<unsigned char *>(__shfl_sync(0xffffffffu, to, from));
+                    if (rows_there >> from & 1u) *reinterpret_cast<uint4 *>(dst + c0 * (whole ? 2 : 4) + chunk * 16) = v;
+                }
+                __syncwarp();
             }
             if (there) {
                 if (!whole) reinterpret_cast<float2 *>(a.part + chunk_stats_at(gridDim.x, G::ROWS, D))[slot] = make_float2(mu, l);
