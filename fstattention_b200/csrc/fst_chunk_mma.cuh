@@ -1,8 +1,8 @@
 // Chunk attention of few rows on mma.sync: decode steps and drafted tokens.
 //
-// A tile is 16 or 32 rows and 128 keys; a call like that reads each key and value once for a handful of products, so HBM bounds it
+// A tile is 16 or 32 rows and 128 or 256 keys; a call like that reads each key and value once for a handful of products, so HBM bounds it
 // and the tensor cores' rate does not matter.  What matters is bytes in flight and that nobody waits for anybody: each of the
-// eight warps has 16 keys of a tile, a ring of its own that TMA fills (boxes of 16 rows; a page holds 16 or more), and an accumulator of its
+// eight warps has 16 or 32 keys of a tile, a ring of its own that TMA fills (boxes of 16 rows; a page holds 16 or more), and an accumulator of its
 // own for all rows, so the loop has no barrier among warps.  They meet once per item, to add up.
 //
 // 8-bit rows become matrix fragments in registers.  The order of the summed index is free as long as both operands agree, so
@@ -23,13 +23,15 @@ namespace fst {
 
 template <int D, bool QUANT, int MT>
 struct ChunkMmaGeo {
-    static constexpr int WARPS = 8, KW = 16, KEYS = WARPS * KW, ROWS = 16 * MT;
-    static constexpr int TILE = KW * D * (QUANT ? 1 : 2);           // bytes of 16 rows of K or V
-    static constexpr int STAGES = (D == 128 ? 2 : 4) * (QUANT ? 2 : 1);
+    static constexpr int WARPS = 8, KW = !QUANT && D == 128 ? 16 : 32, KEYS = WARPS * KW, ROWS = 16 * MT;
+    static constexpr int TILE = KW * D * (QUANT ? 1 : 2);           // bytes of a warp's rows of K or V
+    static constexpr int STAGES = QUANT && D == 64 ? 4 : 2;
+    static constexpr bool Q_SHARED = D == 128 && MT == 2;           // fragments of Q in shared memory: registers would not hold them
     static constexpr int OFF_MERGE = WARPS * STAGES * 2 * TILE;     // [warp][16 rows][D + 4] fp32
     static constexpr int OFF_STATS = OFF_MERGE + WARPS * 16 * (D + 4) * 4;      // [warp][ROWS] (exponent, sum)
-    static constexpr int OFF_SCALES = OFF_STATS + WARPS * ROWS * 8; // [warp][stage] 16 bytes of K, 16 of V
-    static constexpr int OFF_BAR = OFF_SCALES + WARPS * STAGES * 32;
+    static constexpr int OFF_SCALES = OFF_STATS + WARPS * ROWS * 8; // [warp][stage] KW bytes of K, KW of V
+    static constexpr int OFF_Q = OFF_SCALES + WARPS * STAGES * 2 * KW;    // [row tile][step][lane] 16 bytes
+    static constexpr int OFF_BAR = OFF_Q + (Q_SHARED ? MT * D / 16 * 512 : 0);
     static constexpr int BYTES = OFF_BAR + WARPS * STAGES * 8 + 16 + 1024;      // + alignment
 };
 
@@ -71,7 +73,8 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
     using Cursor = ChunkCursor<G::ROWS, G::KEYS>;
     constexpr bool BF16 = !std::is_same<T, __half>::value;
     constexpr int KS = D / 16, ND = D / 8;               // steps of the first product, column tiles of the second
-    constexpr int HALF_BYTES = 16 * 128;                 // 16 rows of 64 columns of 16 bits
+    constexpr int KW = G::KW, NK = KW / 8, SUBS = KW / 16;
+    constexpr int HALF_BYTES = 16 * 128, SUB_BYTES = 16 * D * 2;      // 16 rows of 64 columns of 16 bits, of all
 
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     extern __shared__ unsigned char smem_raw[];
@@ -79,7 +82,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
     unsigned char *smem = smem_raw + (s_base - smem_u32(smem_raw));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t ring = s_base + warp * G::STAGES * 2 * G::TILE, bars = s_base + G::OFF_BAR + warp * G::STAGES * 8;
-    unsigned char *scales = smem + G::OFF_SCALES + warp * G::STAGES * 32;
+    unsigned char *scales = smem + G::OFF_SCALES + warp * G::STAGES * 2 * KW;
     if (lane == 0) {
         for (int i = 0; i < G::STAGES; ++i) mbar_init(bars + i * 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -95,51 +98,50 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
         return;
     }
 
-    // ---- loads, one 16-key group of this warp at a time; the page of the next one is looked up a group ahead
+    // ---- loads, one group of KW keys of this warp at a time, 16 of them by a lane; the pages of the next one are looked up a group ahead
     Cursor ld;
     ld.seek(line, first);
     Cursor me = ld;
     int left = n_tiles, page = 0, slot_in = 0, in_flight = 0;
-    auto group_of = [&](const Cursor &c) { return c.tile * G::KEYS + warp * G::KW; };
+    auto group_of = [&](const Cursor &c) { return c.tile * G::KEYS + warp * KW; };
     auto look_up = [&]() {                                // the next group that has keys, if any
 #pragma unroll 1
         while (left > 0 && group_of(ld) >= ld.keys) {
             ld.next(line);
             --left;
         }
-        if (left > 0) {
-            const int idx = group_of(ld) >> a.c.page_shift;
-            page = __ldg(a.c.table + size_t(ld.z) * a.c.width + idx);
-        }
+        const int key = group_of(ld) + lane * 16;
+        if (left > 0 && lane < SUBS && key < ld.keys) page = __ldg(a.c.table + size_t(ld.z) * a.c.width + (key >> a.c.page_shift));
     };
     auto load = [&]() {                                   // requests it, then looks for the one behind
         if (left <= 0) return;
-        if (lane == 0) {
-            const int off = group_of(ld) & ((1 << a.c.page_shift) - 1);
-            const uint32_t bar = bars + slot_in * 8, dst = ring + slot_in * 2 * G::TILE;
-            const bool bad = unsigned(page) >= unsigned(a.c.n_pages);    // the boxes then read as zeros
-            if (bad) report(a.status, FST_DEV_INDEX_RANGE, ld.z, group_of(ld));
+        const int key = group_of(ld) + lane * 16, off = key & ((1 << a.c.page_shift) - 1);
+        const bool mine = lane < SUBS && key < ld.keys, bad = mine && unsigned(page) >= unsigned(a.c.n_pages);    // bad: the boxes read as zeros
+        const uint32_t bar = bars + slot_in * 8, dst = ring + slot_in * 2 * G::TILE;
+        const uint32_t all = __ballot_sync(0xffffffffu, mine), wrong = __ballot_sync(0xffffffffu, bad);
+        if (bad) report(a.status, FST_DEV_INDEX_RANGE, ld.z, key);
+        uint4 *sc = reinterpret_cast<uint4 *>(scales + slot_in * 2 * KW);
+        if (QUANT && bad) {
+            sc[lane] = sc[SUBS + lane] = make_uint4(0, 0, 0, 0);
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(bar, __popc(all) * 2 * (G::TILE / SUBS) + (QUANT ? 32 * __popc(all & ~wrong) : 0));
+        __syncwarp();
+        if (mine) {
             if constexpr (QUANT) {
-                const size_t at = ((size_t(bad ? 0 : page) * a.H_kv + ld.h) << a.c.page_shift) + off;
-                const uint4 zero = make_uint4(0, 0, 0, 0);
-                uint4 *sc = reinterpret_cast<uint4 *>(scales + slot_in * 32);
-                if (bad) {
-                    sc[0] = sc[1] = zero;
-                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                }
-                mbar_arrive_expect_tx(bar, 2 * G::TILE + (bad ? 0 : 32));
                 if (!bad) {
-                    bulk_load(smem_u32(sc), a.c.k_scale + at, 16, bar);
-                    bulk_load(smem_u32(sc + 1), a.c.v_scale + at, 16, bar);
+                    const size_t at = ((size_t(page) * a.H_kv + ld.h) << a.c.page_shift) + off;
+                    bulk_load(smem_u32(sc + lane), a.c.k_scale + at, 16, bar);
+                    bulk_load(smem_u32(sc + SUBS + lane), a.c.v_scale + at, 16, bar);
                 }
-                tma_load_4d(dst, &tm_k, 0, off, ld.h, page, bar);
-                tma_load_4d(dst + G::TILE, &tm_v, 0, off, ld.h, page, bar);
+                tma_load_4d(dst + lane * 16 * D, &tm_k, 0, off, ld.h, page, bar);
+                tma_load_4d(dst + G::TILE + lane * 16 * D, &tm_v, 0, off, ld.h, page, bar);
             } else {
-                mbar_arrive_expect_tx(bar, 2 * G::TILE);
 #pragma unroll
-                for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(dst + hf * HALF_BYTES, &tm_k, hf * 64, off, ld.h, page, bar);
+                for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(dst + lane * SUB_BYTES + hf * HALF_BYTES, &tm_k, hf * 64, off, ld.h, page, bar);
 #pragma unroll
-                for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(dst + G::TILE + hf * HALF_BYTES, &tm_v, hf * 64, off, ld.h, page, bar);
+                for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(dst + G::TILE + lane * SUB_BYTES + hf * HALF_BYTES, &tm_v, hf * 64, off, ld.h, page, bar);
             }
         }
         if (++slot_in == G::STAGES) slot_in = 0;
@@ -154,7 +156,18 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
 
     // ---- products
     const float c2 = a.scale_log2 * (QUANT ? (BF16 ? kTiny : 256.f) : 1.f);
-    uint32_t qf[MT][KS][4];
+    uint32_t qf[G::Q_SHARED ? 1 : MT][G::Q_SHARED ? 1 : KS][4];
+    const uint32_t q_at = s_base + G::OFF_Q + lane * 16;
+    // fragment of step st of row tile x
+    auto q_frag = [&](int x, int st, uint32_t (&f)[4]) {
+        if constexpr (G::Q_SHARED) {
+            const uint4 v = lds128(q_at + (x * KS + st) * 512);
+            f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[k] = qf[x][st][k];
+        }
+    };
     float acc[MT][ND][4], m[MT][2], l[MT][2];
     int limit[MT][2], lim_first = 0, slot = 0;
     uint32_t parity = 0;
@@ -177,31 +190,53 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     m[x][hh] = -INFINITY;
                     l[x][hh] = 0.f;
                     const T *src = static_cast<const T *>(a.q) + me.z * a.qs_z + (me.h * a.group + (r - tok * a.group)) * a.qs_h + tok * a.qs_n;
-                    if constexpr (QUANT) {                // D / 4 contiguous values of the row, in the order of the K bytes
+                    // two of the four registers of the row tile's fragments: the row's part of two steps in an 8-bit cache's order, or of one
+                    auto two_steps = [&](int s2, uint32_t (&f)[4]) {         // steps 2 s2 and 2 s2 + 1: D / 4 contiguous values, K's bytes' order
+                        uint4 w = real ? __ldg(reinterpret_cast<const uint4 *>(src + t * (D / 4) + s2 * 8)) : make_uint4(0, 0, 0, 0);
+                        if constexpr (BF16) {
+                            const __nv_bfloat162 by = __float2bfloat162_rn(kTiny);
+                            uint32_t *p = &w.x;
 #pragma unroll
-                        for (int s = 0; s < KS / 2; ++s) {
-                            uint4 w = real ? __ldg(reinterpret_cast<const uint4 *>(src + t * (D / 4) + s * 8)) : make_uint4(0, 0, 0, 0);
-                            if constexpr (BF16) {
-                                const __nv_bfloat162 f = __float2bfloat162_rn(kTiny);
-                                uint32_t *p = &w.x;
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    const __nv_bfloat162 y = __hmul2(*reinterpret_cast<__nv_bfloat162 *>(p + k), f);
-                                    p[k] = *reinterpret_cast<const uint32_t *>(&y);
-                                }
+                            for (int k = 0; k < 4; ++k) {
+                                const __nv_bfloat162 y = __hmul2(*reinterpret_cast<__nv_bfloat162 *>(p + k), by);
+                                p[k] = *reinterpret_cast<const uint32_t *>(&y);
                             }
-                            // widen() gives bytes (0, 2) and (1, 3): Q's pairs to match
-                            qf[x][2 * s][hh] = __byte_perm(w.x, w.y, 0x5410);
-                            qf[x][2 * s][2 + hh] = __byte_perm(w.x, w.y, 0x7632);
-                            qf[x][2 * s + 1][hh] = __byte_perm(w.z, w.w, 0x5410);
-                            qf[x][2 * s + 1][2 + hh] = __byte_perm(w.z, w.w, 0x7632);
+                        }
+                        // widen() gives bytes (0, 2) and (1, 3): Q's pairs to match
+                        f[0] = __byte_perm(w.x, w.y, 0x5410);
+                        f[1] = __byte_perm(w.x, w.y, 0x7632);
+                        f[2] = __byte_perm(w.z, w.w, 0x5410);
+                        f[3] = __byte_perm(w.z, w.w, 0x7632);
+                    };
+                    auto one_step = [&](int st, uint32_t &lo, uint32_t &hi) {
+                        lo = real ? __ldg(reinterpret_cast<const uint32_t *>(src + st * 16 + 2 * t)) : 0u;
+                        hi = real ? __ldg(reinterpret_cast<const uint32_t *>(src + st * 16 + 8 + 2 * t)) : 0u;
+                    };
+                    if constexpr (G::Q_SHARED) {          // every warp brings a step (KS = 8 warps)
+                        uint32_t lo, hi;
+                        if constexpr (QUANT) {
+                            uint32_t f[4];
+                            two_steps(warp >> 1, f);
+                            lo = warp & 1 ? f[2] : f[0];
+                            hi = warp & 1 ? f[3] : f[1];
+                        } else {
+                            one_step(warp, lo, hi);
+                        }
+                        asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(q_at + (x * KS + warp) * 512 + hh * 4), "r"(lo) : "memory");
+                        asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(q_at + (x * KS + warp) * 512 + 8 + hh * 4), "r"(hi) : "memory");
+                    } else if constexpr (QUANT) {
+#pragma unroll
+                        for (int s2 = 0; s2 < KS / 2; ++s2) {
+                            uint32_t f[4];
+                            two_steps(s2, f);
+                            qf[x][2 * s2][hh] = f[0];
+                            qf[x][2 * s2][2 + hh] = f[1];
+                            qf[x][2 * s2 + 1][hh] = f[2];
+                            qf[x][2 * s2 + 1][2 + hh] = f[3];
                         }
                     } else {
 #pragma unroll
-                        for (int s = 0; s < KS; ++s) {
-                            qf[x][s][hh] = real ? __ldg(reinterpret_cast<const uint32_t *>(src + s * 16 + 2 * t)) : 0u;
-                            qf[x][s][2 + hh] = real ? __ldg(reinterpret_cast<const uint32_t *>(src + s * 16 + 8 + 2 * t)) : 0u;
-                        }
+                        for (int st = 0; st < KS; ++st) one_step(st, qf[x][st][hh], qf[x][st][2 + hh]);
                     }
                 }
 #pragma unroll
@@ -209,46 +244,42 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
 #pragma unroll
                     for (int k = 0; k < 4; ++k) acc[x][n][k] = 0.f;
             }
+            if constexpr (G::Q_SHARED) __syncthreads();
         }
 
         const int key0 = group_of(me);
         if (key0 < me.keys && alive) {
             const uint32_t k_at = ring + slot * 2 * G::TILE, v_at = k_at + G::TILE;
-            const bool edge = key0 + G::KW > lim_first;   // not every row attends to all of the group
+            const bool edge = key0 + KW > lim_first;      // not every row attends to all of the group
             alive = __all_sync(0xffffffffu, mbar_wait(bars + slot * 8, parity, a.status, blockIdx.x));
-            float s[MT][2][4];
+            float s[MT][NK][4];
 #pragma unroll
             for (int x = 0; x < MT; ++x)
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < NK; ++n)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) s[x][n][k] = 0.f;
-            float ks[2][2], vs[2][2];                     // scales of my four keys: 8 n + 2 t + k
             if constexpr (QUANT) {
-                const uint16_t *sc = reinterpret_cast<const uint16_t *>(scales + slot * 32);
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const uint32_t bk = sc[4 * n + t], bv = sc[8 + 4 * n + t];
-                    ks[n][0] = e8m0_value(bk & 255u) * c2;
-                    ks[n][1] = e8m0_value(bk >> 8) * c2;
-                    vs[n][0] = e8m0_value(bv & 255u) * kTiny;
-                    vs[n][1] = e8m0_value(bv >> 8) * kTiny;
-                }
                 // K: key 8 n + g, bytes D/4 t ..
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const int row = 8 * n + g;
+                for (int c = 0; c < D / 64; ++c) {        // 16 bytes: four steps
+                    uint4 b[NK];
 #pragma unroll
-                    for (int c = 0; c < D / 64; ++c) {    // 16 bytes: four steps
-                        const int chunk = D == 128 ? ((2 * t + c) ^ (row & 7)) : (t ^ ((row >> 1) & 3));
-                        const uint4 b = lds128(k_at + row * D + chunk * 16);
-                        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+                    for (int n = 0; n < NK; ++n) {
+                        const int row = 8 * n + g, chunk = D == 128 ? ((2 * t + c) ^ (row & 7)) : (t ^ ((row >> 1) & 3));
+                        b[n] = lds128(k_at + row * D + chunk * 16);
+                    }
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t q[MT][4];
+#pragma unroll
+                        for (int x = 0; x < MT; ++x) q_frag(x, c * 4 + k, q[x]);
+#pragma unroll
+                        for (int n = 0; n < NK; ++n) {
                             uint32_t b0, b1;
-                            widen<BF16>(w[k], b0, b1);
+                            widen<BF16>(k == 0 ? b[n].x : k == 1 ? b[n].y : k == 2 ? b[n].z : b[n].w, b0, b1);
 #pragma unroll
-                            for (int x = 0; x < MT; ++x) MT_::mma(s[x][n], qf[x][c * 4 + k], b0, b1);
+                            for (int x = 0; x < MT; ++x) MT_::mma(s[x][n], q[x], b0, b1);
                         }
                     }
                 }
@@ -257,40 +288,57 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
 #pragma unroll
                 for (int st = 0; st < KS; ++st) {
                     const int chunk = 2 * st + ((lane >> 3) & 1);
-                    uint32_t b[4];
-                    ldmatrix_x4(b, k_at + (chunk >> 3) * HALF_BYTES + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+                    uint32_t q[MT][4];
 #pragma unroll
-                    for (int x = 0; x < MT; ++x) {
-                        MT_::mma(s[x][0], qf[x][st], b[0], b[1]);
-                        MT_::mma(s[x][1], qf[x][st], b[2], b[3]);
+                    for (int x = 0; x < MT; ++x) q_frag(x, st, q[x]);
+#pragma unroll
+                    for (int sub = 0; sub < SUBS; ++sub) {
+                        uint32_t b[4];
+                        ldmatrix_x4(b, k_at + sub * SUB_BYTES + (chunk >> 3) * HALF_BYTES + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+#pragma unroll
+                        for (int x = 0; x < MT; ++x) {
+                            MT_::mma(s[x][2 * sub], q[x], b[0], b[1]);
+                            MT_::mma(s[x][2 * sub + 1], q[x], b[2], b[3]);
+                        }
                     }
                 }
             }
             // ---- softmax of the group: scores in base-2 units against the row's running maximum
-            uint32_t pf[MT][4];
+            uint32_t pf[MT][SUBS][4];
+            float mx[MT][2];
 #pragma unroll
-            for (int x = 0; x < MT; ++x) {
-                float mx[2] = {-INFINITY, -INFINITY};
+            for (int x = 0; x < MT; ++x) mx[x][0] = mx[x][1] = -INFINITY;
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NK; ++n) {
+                float ks[2] = {c2, c2};                   // of my keys 8 n + 2 t + k
+                if constexpr (QUANT) {
+                    const uint32_t b = *reinterpret_cast<const uint16_t *>(scales + slot * 2 * KW + 8 * n + 2 * t);
+                    ks[0] = e8m0_value(b & 255u) * c2;
+                    ks[1] = e8m0_value(b >> 8) * c2;
+                }
+#pragma unroll
+                for (int x = 0; x < MT; ++x)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        float v = s[x][n][k] * (QUANT ? ks[n][k & 1] : c2);
+                        float v = s[x][n][k] * ks[k & 1];
                         if (edge && key0 + 8 * n + 2 * t + (k & 1) >= limit[x][k >> 1]) v = -INFINITY;
                         s[x][n][k] = v;
-                        mx[k >> 1] = fmaxf(mx[k >> 1], v);
+                        mx[x][k >> 1] = fmaxf(mx[x][k >> 1], v);
                     }
+            }
+#pragma unroll
+            for (int x = 0; x < MT; ++x) {
                 bool up = false;
-                float alpha[2], ref[2];
+                float alpha[2];
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
-                    mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 1));
-                    mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 2));
-                    const float now = fmaxf(m[x][hh], mx[hh]);
+                    mx[x][hh] = fmaxf(mx[x][hh], __shfl_xor_sync(0xffffffffu, mx[x][hh], 1));
+                    mx[x][hh] = fmaxf(mx[x][hh], __shfl_xor_sync(0xffffffffu, mx[x][hh], 2));
+                    const float now = fmaxf(m[x][hh], mx[x][hh]);
                     up = up || now > m[x][hh];
                     alpha[hh] = now == -INFINITY ? 1.f : fast_exp2(m[x][hh] - now);
                     m[x][hh] = now;
-                    ref[hh] = now == -INFINITY ? 0.f : now;
+                    mx[x][hh] = now == -INFINITY ? 0.f : now;
                 }
                 if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -303,63 +351,75 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     l[x][0] *= alpha[0];
                     l[x][1] *= alpha[1];
                 }
-                float p[2][4];
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        p[n][k] = fast_exp2(s[x][n][k] - ref[k >> 1]);
-                        l[x][k >> 1] += p[n][k];
-                        // the row's scale; what a masked key holds, NaN too, stays out
-                        if constexpr (QUANT) p[n][k] = s[x][n][k] == -INFINITY ? 0.f : p[n][k] * vs[n][k & 1];
-                    }
-                pf[x][0] = MP::pack(p[0][0], p[0][1]);
-                pf[x][1] = MP::pack(p[0][2], p[0][3]);
-                pf[x][2] = MP::pack(p[1][0], p[1][1]);
-                pf[x][3] = MP::pack(p[1][2], p[1][3]);
             }
-            // ---- second product
-            if constexpr (QUANT) {
-                // V: keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9, bytes D/8 g ..: column tile j holds columns D/8 n + j
-                uint32_t w[4][D / 32];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int row = 2 * t + (k & 1) + (k >> 1) * 8;
-                    if constexpr (D == 128) {
-                        const uint4 b = lds128(v_at + row * 128 + ((g ^ (row & 7)) << 4));
-                        w[k][0] = b.x; w[k][1] = b.y; w[k][2] = b.z; w[k][3] = b.w;
-                    } else {
-                        const uint2 b = lds64(v_at + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8);
-                        w[k][0] = b.x; w[k][1] = b.y;
-                    }
+            for (int n = 0; n < NK; ++n) {
+                float vs[2] = {1.f, 1.f};
+                if constexpr (QUANT) {
+                    const uint32_t b = *reinterpret_cast<const uint16_t *>(scales + slot * 2 * KW + KW + 8 * n + 2 * t);
+                    vs[0] = e8m0_value(b & 255u) * kTiny;
+                    vs[1] = e8m0_value(b >> 8) * kTiny;
                 }
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c)
+                for (int x = 0; x < MT; ++x) {
+                    float p[4];
 #pragma unroll
-                    for (int hl = 0; hl < 2; ++hl) {      // two column tiles from bytes 2 hl, 2 hl + 1 of either key
-                        uint32_t b0[2], b1[2];
-                        widen<true>(__byte_perm(w[0][c], w[1][c], hl ? 0x7632 : 0x5410), b0[0], b0[1]);
-                        widen<true>(__byte_perm(w[2][c], w[3][c], hl ? 0x7632 : 0x5410), b1[0], b1[1]);
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-#pragma unroll
-                            for (int x = 0; x < MT; ++x) MP::mma(acc[x][c * 4 + hl * 2 + k], pf[x], b0[k], b1[k]);
+                    for (int k = 0; k < 4; ++k) {
+                        p[k] = fast_exp2(s[x][n][k] - mx[x][k >> 1]);
+                        l[x][k >> 1] += p[k];
+                        // the row's scale; what a masked key holds, NaN too, stays out
+                        if constexpr (QUANT) p[k] = s[x][n][k] == -INFINITY ? 0.f : p[k] * vs[k & 1];
                     }
-            } else {
-                const int row = (lane & 7) + ((lane >> 3) & 1) * 8, here = min(me.kv - key0, G::KW);
+                    pf[x][n >> 1][(n & 1) * 2] = MP::pack(p[0], p[1]);
+                    pf[x][n >> 1][(n & 1) * 2 + 1] = MP::pack(p[2], p[3]);
+                }
+            }
+            // ---- second product
+            const int here = min(me.kv, (me.keys + 15) & ~15) - key0;     // rows of V that were fetched and are the sequence's
 #pragma unroll
-                for (int j = 0; j < ND / 2; ++j) {
-                    const int chunk = 2 * j + (lane >> 4);
-                    uint32_t b[4];
-                    ldmatrix_x4_trans(b, v_at + (chunk >> 3) * HALF_BYTES + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
-                    if (edge) {                           // zero times what is not finite would be NaN
+            for (int sub = 0; sub < SUBS; ++sub) {
+                if constexpr (QUANT) {
+                    // V: keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9, bytes D/8 g ..: column tile j holds columns D/8 n + j
+                    uint32_t w[4][D / 32];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) poisoned = keep_finite<T>(b[k], here - (k & 1) * 8 - 2 * t) || poisoned;
+                    for (int k = 0; k < 4; ++k) {
+                        const int row = sub * 16 + 2 * t + (k & 1) + (k >> 1) * 8;
+                        if constexpr (D == 128) {
+                            const uint4 b = lds128(v_at + row * 128 + ((g ^ (row & 7)) << 4));
+                            w[k][0] = b.x; w[k][1] = b.y; w[k][2] = b.z; w[k][3] = b.w;
+                        } else {
+                            const uint2 b = lds64(v_at + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8);
+                            w[k][0] = b.x; w[k][1] = b.y;
+                        }
                     }
 #pragma unroll
-                    for (int x = 0; x < MT; ++x) {
-                        MP::mma(acc[x][2 * j], pf[x], b[0], b[1]);
-                        MP::mma(acc[x][2 * j + 1], pf[x], b[2], b[3]);
+                    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                        for (int hl = 0; hl < 2; ++hl) {  // two column tiles from bytes 2 hl, 2 hl + 1 of either key
+                            uint32_t b0[2], b1[2];
+                            widen<true>(__byte_perm(w[0][c], w[1][c], hl ? 0x7632 : 0x5410), b0[0], b0[1]);
+                            widen<true>(__byte_perm(w[2][c], w[3][c], hl ? 0x7632 : 0x5410), b1[0], b1[1]);
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                                for (int x = 0; x < MT; ++x) MP::mma(acc[x][c * 4 + hl * 2 + k], pf[x][sub], b0[k], b1[k]);
+                        }
+                } else {
+                    const int row = (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+                    for (int j = 0; j < ND / 2; ++j) {
+                        const int chunk = 2 * j + (lane >> 4);
+                        uint32_t b[4];
+                        ldmatrix_x4_trans(b, v_at + sub * SUB_BYTES + (chunk >> 3) * HALF_BYTES + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+                        if (edge) {                       // zero times what is not finite would be NaN
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) poisoned = keep_finite<T>(b[k], here - sub * 16 - (k & 1) * 8 - 2 * t) || poisoned;
+                        }
+#pragma unroll
+                        for (int x = 0; x < MT; ++x) {
+                            MP::mma(acc[x][2 * j], pf[x][sub], b[0], b[1]);
+                            MP::mma(acc[x][2 * j + 1], pf[x][sub], b[2], b[3]);
+                        }
                     }
                 }
             }
@@ -431,7 +491,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                 if (bad && tok < me.ql) {
                     // keys of this piece whose groups were looked through, as far as my row sees them
                     const int keys = a.causal ? min(me.kv, me.kv - me.ql + tok + 1) : me.kv;
-                    add_not_finite<T, D / 16, QUANT>(a, me.z, me.h, max(max(lim_first, 0) & ~(G::KW - 1), max(0, me.tile - i) * G::KEYS),
+                    add_not_finite<T, D / 16, QUANT>(a, me.z, me.h, max(max(lim_first, 0) & ~(KW - 1), max(0, me.tile - i) * G::KEYS),
                                               min(keys, (me.tile + 1) * G::KEYS), c0, out);
                 }
                 if (whole) {
