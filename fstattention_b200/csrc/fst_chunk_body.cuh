@@ -19,7 +19,7 @@ cudaError_t launch_chunk_t(const ChunkArgs &a, int n_ctas, cudaStream_t stream) 
             return cudaErrorNotSupported;
         return a.c.k_scale != nullptr ? launch_chunk_umma<T, D, true>(b, tq, tk, tv, n_ctas, stream) : launch_chunk_umma<T, D, false>(b, tq, tk, tv, n_ctas, stream);
     }
-    if (!make_pool_maps(&tk, &tv, a.c, bf16, D, a.H_kv, 16)) return cudaErrorNotSupported;
+    if (!make_pool_maps(&tk, &tv, a.c, bf16, D, a.H_kv, 1 << a.c.page_shift)) return cudaErrorNotSupported;
     const bool one = a.n_q * a.group <= 16;
     if (a.c.k_scale != nullptr)
         return one ? launch_chunk_mma<T, D, true, 1>(a, tk, tv, n_ctas, stream) : launch_chunk_mma<T, D, true, 2>(a, tk, tv, n_ctas, stream);

@@ -1,9 +1,9 @@
 // Chunk attention of few rows on mma.sync: decode steps and drafted tokens.
 //
 // A tile is 16 or 32 rows and 128 or 256 keys; a call like that reads each key and value once for a handful of products, so HBM bounds it
-// and the tensor cores' rate does not matter.  What matters is bytes in flight and that nobody waits for anybody: each of the
-// eight warps has 16 or 32 keys of a tile, a ring of its own that TMA fills (boxes of 16 rows; a page holds 16 or more), and an accumulator of its
-// own for all rows, so the loop has no barrier among warps.  They meet once per item, to add up.
+// and the tensor cores' rate does not matter.  What matters is bytes in flight and that the warps seldom wait: a ninth warp has TMA
+// fill a ring of tiles, each of the eight others takes 16 or 32 keys of a tile and has an accumulator of its own for all rows, so
+// that nothing but the ring's barriers lies between them.  They meet once per item, to add up.
 //
 // 8-bit rows become matrix fragments in registers.  The order of the summed index is free as long as both operands agree, so
 // lane (g, t) of a K fragment takes the contiguous bytes D/4 t .. of key g, and Q is loaded in the same order;
@@ -24,15 +24,18 @@ namespace fst {
 template <int D, bool QUANT, int MT>
 struct ChunkMmaGeo {
     static constexpr int WARPS = 8, KW = !QUANT && D == 128 ? 16 : 32, KEYS = WARPS * KW, ROWS = 16 * MT;
-    static constexpr int TILE = KW * D * (QUANT ? 1 : 2);           // bytes of a warp's rows of K or V
+    static constexpr int THREADS = WARPS * 32 + 128;                // and a loading warp, in a warpgroup that gives its registers away
+    static constexpr int REGS = 224, REGS_LOADS = 56;
+    static_assert(256 * REGS + 128 * REGS_LOADS <= THREADS * 168, "the split draws on what the launch was given");
+    static constexpr int TILE = KEYS * D * (QUANT ? 1 : 2);         // bytes of a tile of K or V: 64-column halves of KEYS rows, or rows of bytes
     static constexpr int STAGES = QUANT && D == 64 ? 4 : 2;
     static constexpr bool Q_SHARED = D == 128 && MT == 2;           // fragments of Q in shared memory: registers would not hold them
-    static constexpr int OFF_MERGE = WARPS * STAGES * 2 * TILE;     // [warp][16 rows][D + 4] fp32
+    static constexpr int OFF_MERGE = STAGES * 2 * TILE;             // [warp][16 rows][D + 4] fp32
     static constexpr int OFF_STATS = OFF_MERGE + WARPS * 16 * (D + 4) * 4;      // [warp][ROWS] (exponent, sum)
-    static constexpr int OFF_SCALES = OFF_STATS + WARPS * ROWS * 8; // [warp][stage] KW bytes of K, KW of V
-    static constexpr int OFF_Q = OFF_SCALES + WARPS * STAGES * 2 * KW;    // [row tile][step][lane] 16 bytes
+    static constexpr int OFF_SCALES = OFF_STATS + WARPS * ROWS * 8; // [stage] KEYS bytes of K, KEYS of V
+    static constexpr int OFF_Q = OFF_SCALES + (QUANT ? STAGES * 2 * KEYS : 0);  // [row tile][step][lane] 16 bytes
     static constexpr int OFF_BAR = OFF_Q + (Q_SHARED ? MT * D / 16 * 512 : 0);
-    static constexpr int BYTES = OFF_BAR + WARPS * STAGES * 8 + 16 + 1024;      // + alignment
+    static constexpr int BYTES = OFF_BAR + 2 * STAGES * 8 + 1024;   // + alignment
 };
 
 constexpr float kTiny = 1.152921504606846976e18f;        // 2^60, half of what a bf16 made of an e4m3's bits lacks
@@ -64,7 +67,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, int byt
 }
 
 template <typename T, int D, bool QUANT, int MT>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(384, 1)
 chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
     using G = ChunkMmaGeo<D, QUANT, MT>;
     using MT_ = MmaTraits<T>;
@@ -74,21 +77,23 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
     constexpr bool BF16 = !std::is_same<T, __half>::value;
     constexpr int KS = D / 16, ND = D / 8;               // steps of the first product, column tiles of the second
     constexpr int KW = G::KW, NK = KW / 8, SUBS = KW / 16;
-    constexpr int HALF_BYTES = 16 * 128, SUB_BYTES = 16 * D * 2;      // 16 rows of 64 columns of 16 bits, of all
+    constexpr int HALF_BYTES = G::KEYS * 128, SUB_BYTES = 16 * (QUANT ? D : 128);         // a tile's half of 64 columns of 16 bits, 16 rows in it
 
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     extern __shared__ unsigned char smem_raw[];
     const uint32_t s_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char *smem = smem_raw + (s_base - smem_u32(smem_raw));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t ring = s_base + warp * G::STAGES * 2 * G::TILE, bars = s_base + G::OFF_BAR + warp * G::STAGES * 8;
-    unsigned char *scales = smem + G::OFF_SCALES + warp * G::STAGES * 2 * KW;
-    if (lane == 0) {
-        for (int i = 0; i < G::STAGES; ++i) mbar_init(bars + i * 8, 1);
+    const uint32_t bar_full = s_base + G::OFF_BAR, bar_empty = bar_full + G::STAGES * 8;
+    if (tid == 0) {
+        for (int i = 0; i < G::STAGES; ++i) {
+            mbar_init(bar_full + i * 8, 1);
+            mbar_init(bar_empty + i * 8, G::WARPS);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    __syncwarp();
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    __syncthreads();
 
     const Line line(a);
     const long long total = Cursor::total(line), first = chunk_first(total, blockIdx.x, gridDim.x);
@@ -97,62 +102,81 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
         if (tid == 0 && a.part != nullptr) leave_cut<G::ROWS, D>(a, Cursor{}, total, 0);
         return;
     }
+    Cursor me;
+    me.seek(line, first);
 
-    // ---- loads, one group of KW keys of this warp at a time, 16 of them by a lane; the pages of the next one are looked up a group ahead
-    Cursor ld;
-    ld.seek(line, first);
-    Cursor me = ld;
-    int left = n_tiles, page = 0, slot_in = 0, in_flight = 0;
-    auto group_of = [&](const Cursor &c) { return c.tile * G::KEYS + warp * KW; };
-    auto look_up = [&]() {                                // the next group that has keys, if any
+    // (each side asks inside its own branch, see chunk_umma_kernel)
+    if (warp >= G::WARPS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(G::REGS_LOADS));
+        if (warp > G::WARPS) return;
+        // ====== loads: a box per page and 64 columns, by one lane; the page numbers are looked up a tile ahead ======
+        // (While each warp fetched its own 16 rows, asking for them took it as long as computing with them.)
+        const int ps = 1 << a.c.page_shift;
+        int st = 0, page = 0;
+        uint32_t use = 0;
+        auto look_up = [&]() {
+            const int key = me.tile * G::KEYS + lane * ps;
+            page = lane * ps < G::KEYS && key < me.keys ? __ldg(a.c.table + size_t(me.z) * a.c.width + (key >> a.c.page_shift)) : 0;
+        };
+        look_up();
 #pragma unroll 1
-        while (left > 0 && group_of(ld) >= ld.keys) {
-            ld.next(line);
-            --left;
-        }
-        const int key = group_of(ld) + lane * 16;
-        if (left > 0 && lane < SUBS && key < ld.keys) page = __ldg(a.c.table + size_t(ld.z) * a.c.width + (key >> a.c.page_shift));
-    };
-    auto load = [&]() {                                   // requests it, then looks for the one behind
-        if (left <= 0) return;
-        const int key = group_of(ld) + lane * 16, off = key & ((1 << a.c.page_shift) - 1);
-        const bool mine = lane < SUBS && key < ld.keys, bad = mine && unsigned(page) >= unsigned(a.c.n_pages);    // bad: the boxes read as zeros
-        const uint32_t bar = bars + slot_in * 8, dst = ring + slot_in * 2 * G::TILE;
-        const uint32_t all = __ballot_sync(0xffffffffu, mine), wrong = __ballot_sync(0xffffffffu, bad);
-        if (bad) report(a.status, FST_DEV_INDEX_RANGE, ld.z, key);
-        uint4 *sc = reinterpret_cast<uint4 *>(scales + slot_in * 2 * KW);
-        if (QUANT && bad) {
-            sc[lane] = sc[SUBS + lane] = make_uint4(0, 0, 0, 0);
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(bar, __popc(all) * 2 * (G::TILE / SUBS) + (QUANT ? 32 * __popc(all & ~wrong) : 0));
-        __syncwarp();
-        if (mine) {
-            if constexpr (QUANT) {
-                if (!bad) {
-                    const size_t at = ((size_t(page) * a.H_kv + ld.h) << a.c.page_shift) + off;
-                    bulk_load(smem_u32(sc + lane), a.c.k_scale + at, 16, bar);
-                    bulk_load(smem_u32(sc + SUBS + lane), a.c.v_scale + at, 16, bar);
+        for (int i = 0; i < n_tiles; ++i) {
+            const int here = page, key0 = me.tile * G::KEYS, h = me.h, z = me.z;
+            const int pages = (min(G::KEYS, me.keys - key0) + ps - 1) >> a.c.page_shift;         // 0: an item that sees nothing
+            me.next(line);
+            if (i + 1 < n_tiles) look_up();
+            if (pages <= 0) continue;
+            if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(bar_empty + st * 8, (use - 1) & 1, a.status, blockIdx.x))) break;
+            const bool bad = lane < pages && unsigned(here) >= unsigned(a.c.n_pages);            // the boxes then read as zeros
+            const uint32_t wrong = __ballot_sync(0xffffffffu, bad), bar = bar_full + st * 8, k_at = s_base + st * 2 * G::TILE, v_at = k_at + G::TILE;
+            unsigned char *scales = smem + G::OFF_SCALES + st * 2 * G::KEYS;
+            if (bad) {
+                report(a.status, FST_DEV_INDEX_RANGE, z, key0 + lane * ps);
+                if constexpr (QUANT) {
+                    for (int k = 0; k < ps; k += 16)
+                        *reinterpret_cast<uint4 *>(scales + lane * ps + k) = *reinterpret_cast<uint4 *>(scales + G::KEYS + lane * ps + k) = make_uint4(0, 0, 0, 0);
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 }
-                tma_load_4d(dst + lane * 16 * D, &tm_k, 0, off, ld.h, page, bar);
-                tma_load_4d(dst + G::TILE + lane * 16 * D, &tm_v, 0, off, ld.h, page, bar);
-            } else {
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive_expect_tx(bar, (pages << a.c.page_shift) * D * (QUANT ? 2 : 4) + (QUANT ? (pages - __popc(wrong)) * 2 * ps : 0));
+            __syncwarp();
+#pragma unroll 1
+            for (int p = 0; p < pages; ++p) {
+                const int pg = __shfl_sync(0xffffffffu, here, p), row = p * ps;
+                if (umma::elect_one()) {
+                    if constexpr (QUANT) {
+                        tma_load_4d(k_at + row * D, &tm_k, 0, 0, h, pg, bar);
+                        tma_load_4d(v_at + row * D, &tm_v, 0, 0, h, pg, bar);
+                        if (!(wrong >> p & 1u)) {
+                            const size_t at = (size_t(pg) * a.H_kv + h) << a.c.page_shift;
+                            bulk_load(smem_u32(scales + row), a.c.k_scale + at, ps, bar);
+                            bulk_load(smem_u32(scales + G::KEYS + row), a.c.v_scale + at, ps, bar);
+                        }
+                    } else {
 #pragma unroll
-                for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(dst + lane * SUB_BYTES + hf * HALF_BYTES, &tm_k, hf * 64, off, ld.h, page, bar);
+                        for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(k_at + hf * HALF_BYTES + row * 128, &tm_k, hf * 64, 0, h, pg, bar);
 #pragma unroll
-                for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(dst + G::TILE + lane * SUB_BYTES + hf * HALF_BYTES, &tm_v, hf * 64, off, ld.h, page, bar);
+                        for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(v_at + hf * HALF_BYTES + row * 128, &tm_v, hf * 64, 0, h, pg, bar);
+                    }
+                }
+            }
+            if (++st == G::STAGES) {
+                st = 0;
+                ++use;
             }
         }
-        if (++slot_in == G::STAGES) slot_in = 0;
-        ++in_flight;
-        ld.next(line);
-        --left;
-        look_up();
-    };
-    look_up();
+        // nothing may land after the CTA has left, also when a wait ran out: the last fill of every stage
 #pragma unroll 1
-    for (int i = 0; i < G::STAGES; ++i) load();
+        for (int s = 0; s < G::STAGES; ++s) {
+            const uint32_t fills = use + (s < st ? 1u : 0u);
+            if (fills > 0) mbar_wait(bar_full + s * 8, (fills - 1) & 1, a.status, blockIdx.x);
+        }
+        return;
+    }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(G::REGS));
+    auto meet = [&]() { asm volatile("bar.sync 1, 256;\n" ::: "memory"); };     // the computing warps
+    auto group_of = [&](const Cursor &c) { return c.tile * G::KEYS + warp * KW; };
 
     // ---- products
     const float c2 = a.scale_log2 * (QUANT ? (BF16 ? kTiny : 256.f) : 1.f);
@@ -244,14 +268,15 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
 #pragma unroll
                     for (int k = 0; k < 4; ++k) acc[x][n][k] = 0.f;
             }
-            if constexpr (G::Q_SHARED) __syncthreads();
+            if constexpr (G::Q_SHARED) meet();
         }
 
         const int key0 = group_of(me);
+        if (me.keys > 0 && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_full + slot * 8, parity, a.status, blockIdx.x));
         if (key0 < me.keys && alive) {
-            const uint32_t k_at = ring + slot * 2 * G::TILE, v_at = k_at + G::TILE;
+            const uint32_t k_at = s_base + slot * 2 * G::TILE + warp * SUBS * SUB_BYTES, v_at = k_at + G::TILE;      // my rows
+            const unsigned char *scales = smem + G::OFF_SCALES + slot * 2 * G::KEYS + warp * KW;
             const bool edge = key0 + KW > lim_first;      // not every row attends to all of the group
-            alive = __all_sync(0xffffffffu, mbar_wait(bars + slot * 8, parity, a.status, blockIdx.x));
             float s[MT][NK][4];
 #pragma unroll
             for (int x = 0; x < MT; ++x)
@@ -312,7 +337,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
             for (int n = 0; n < NK; ++n) {
                 float ks[2] = {c2, c2};                   // of my keys 8 n + 2 t + k
                 if constexpr (QUANT) {
-                    const uint32_t b = *reinterpret_cast<const uint16_t *>(scales + slot * 2 * KW + 8 * n + 2 * t);
+                    const uint32_t b = *reinterpret_cast<const uint16_t *>(scales + 8 * n + 2 * t);
                     ks[0] = e8m0_value(b & 255u) * c2;
                     ks[1] = e8m0_value(b >> 8) * c2;
                 }
@@ -356,7 +381,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
             for (int n = 0; n < NK; ++n) {
                 float vs[2] = {1.f, 1.f};
                 if constexpr (QUANT) {
-                    const uint32_t b = *reinterpret_cast<const uint16_t *>(scales + slot * 2 * KW + KW + 8 * n + 2 * t);
+                    const uint32_t b = *reinterpret_cast<const uint16_t *>(scales + G::KEYS + 8 * n + 2 * t);
                     vs[0] = e8m0_value(b & 255u) * kTiny;
                     vs[1] = e8m0_value(b >> 8) * kTiny;
                 }
@@ -423,9 +448,10 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     }
                 }
             }
-            __syncwarp();                                 // everybody is done with the slot
-            --in_flight;
-            if (alive) load();
+        }
+        if (me.keys > 0) {                                // done with the stage
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar_empty + slot * 8) : "memory");
             if (++slot == G::STAGES) {
                 slot = 0;
                 parity ^= 1u;
@@ -435,7 +461,9 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
         if (me.tile + 1 == me.tiles || i + 1 == n_tiles) {
             // ---- the warps' results of this piece: 16 rows at a time through shared memory
             const bool from_start = i >= me.tile, whole = from_start && me.tile + 1 == me.tiles;
-            const bool bad = __syncthreads_or(poisoned) != 0;
+            uint32_t bad;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, 1, 256, q;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+                         : "=r"(bad) : "r"(uint32_t(poisoned)) : "memory");
             float2 *stats = reinterpret_cast<float2 *>(smem + G::OFF_STATS);
             float *rows = reinterpret_cast<float *>(smem + G::OFF_MERGE);
 #pragma unroll
@@ -460,7 +488,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                             *reinterpret_cast<float2 *>(to + n * 8 + 2 * t) = make_float2(acc[x][n][2 * hh], acc[x][n][2 * hh + 1]);
                     }
                 }
-                __syncthreads();
+                meet();
                 // sixteen threads a row, D / 16 columns each
                 const int row = tid >> 4, c0 = (tid & 15) * (D / 16);
                 float top = -INFINITY, sum = 0.f, out[D / 16];
@@ -488,7 +516,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) out[k] *= kTiny;
                 }
-                if (bad && tok < me.ql) {
+                if (bad != 0u && tok < me.ql) {
                     // keys of this piece whose groups were looked through, as far as my row sees them
                     const int keys = a.causal ? min(me.kv, me.kv - me.ql + tok + 1) : me.kv;
                     add_not_finite<T, D / 16, QUANT>(a, me.z, me.h, max(max(lim_first, 0) & ~(KW - 1), max(0, me.tile - i) * G::KEYS),
@@ -512,22 +540,12 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         *reinterpret_cast<float4 *>(a.part + at * D + c0 + k) = make_float4(out[k], out[k + 1], out[k + 2], out[k + 3]);
                     if (c0 == 0) reinterpret_cast<float2 *>(a.part + chunk_stats_at(gridDim.x, G::ROWS, D))[at] = make_float2(top, sum);
                 }
-                __syncthreads();
+                meet();
             }
         }
         if (i + 1 < n_tiles) me.next(line);
     }
     if (tid == 0 && a.part != nullptr) leave_cut<G::ROWS, D>(a, me, total, n_tiles);
-    if (!alive) {                                         // a wait ran out: nothing may land after this CTA has left
-#pragma unroll 1
-        for (; in_flight > 0; --in_flight) {
-            mbar_wait(bars + slot * 8, parity, a.status, blockIdx.x);
-            if (++slot == G::STAGES) {
-                slot = 0;
-                parity ^= 1u;
-            }
-        }
-    }
 }
 
 template <typename T, int D, bool QUANT, int MT>
@@ -539,7 +557,7 @@ static cudaError_t launch_chunk_mma(const ChunkArgs &a, const CUtensorMap &tk, c
         return cudaFuncSetAttribute(chunk_mma_kernel<T, D, QUANT, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::BYTES);
     });
     if (ce != cudaSuccess) return ce;
-    const cudaError_t e = launch_serialised(chunk_mma_kernel<T, D, QUANT, MT>, dim3(n_ctas), dim3(256), G::BYTES, stream, a, tk, tv);
+    const cudaError_t e = launch_serialised(chunk_mma_kernel<T, D, QUANT, MT>, dim3(n_ctas), dim3(G::THREADS), G::BYTES, stream, a, tk, tv);
     if (e != cudaSuccess || !chunk_splits(a, G::KEYS)) return e;
     return launch_chunk_combine<T, D, G::ROWS>(a, n_ctas, stream);
 }
