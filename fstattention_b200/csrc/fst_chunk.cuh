@@ -49,8 +49,10 @@ inline void set_group(ChunkArgs &a, int group) {
 }
 __device__ __forceinline__ int by_group(const ChunkArgs &a, int x) { return int(uint64_t(uint32_t(x)) * a.group_mul >> a.group_shift); }
 
-// The line of work for row tiles of ROWS and key tiles of KEYS.
-template <int ROWS, int KEYS>
+// The line of work for row tiles of ROWS and key tiles of KEYS.  An item is OVER units longer than it has key tiles: its own start and end
+// cost a CTA as much as that many tiles (a CTA that got seven items of two tiles each ended at 51 us, the others at 30).  They lie
+// before its first tile; a place among them means that tile.
+template <int ROWS, int KEYS, int OVER>
 struct ChunkLine {
     const ChunkArgs &a;
     __device__ __forceinline__ explicit ChunkLine(const ChunkArgs &args) : a(args) {}
@@ -69,21 +71,21 @@ struct ChunkLine {
     }
     // at least one key tile, so that rows which see nothing are written too
     __device__ __forceinline__ static int tiles_of(int keys) { return max(1, (keys + KEYS - 1) / KEYS); }
-    // Key tiles of one K/V head of a sequence: by one lane, or by a whole warp where the row tiles are many (64 row tiles one after
+    // Units of one K/V head of a sequence: by one lane, or by a whole warp where the row tiles are many (64 row tiles one after
     // the other take a lane 2 us).
     __device__ __forceinline__ bool wide() const { return a.causal && row_tiles(a.n_q) > 8; }
-    __device__ __forceinline__ long long head_tiles(int kv, int ql) const {
+    __device__ __forceinline__ long long head_units(int kv, int ql) const {
         const int n = row_tiles(ql);
-        if (!a.causal) return (long long)n * tiles_of(kv);
+        if (!a.causal) return (long long)n * (tiles_of(kv) + OVER);
         long long s = 0;
 #pragma unroll 1
-        for (int qt = 0; qt < n; ++qt) s += tiles_of(keys(kv, ql, qt));
+        for (int qt = 0; qt < n; ++qt) s += tiles_of(keys(kv, ql, qt)) + OVER;
         return s;
     }
-    __device__ __forceinline__ long long head_tiles_by_warp(int kv, int ql) const {
+    __device__ __forceinline__ long long head_units_by_warp(int kv, int ql) const {
         long long s = 0;
 #pragma unroll 1
-        for (int qt = threadIdx.x & 31, n = row_tiles(ql); qt < n; qt += 32) s += tiles_of(keys(kv, ql, qt));
+        for (int qt = threadIdx.x & 31, n = row_tiles(ql); qt < n; qt += 32) s += tiles_of(keys(kv, ql, qt)) + OVER;
 #pragma unroll
         for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
         return s;
@@ -91,30 +93,31 @@ struct ChunkLine {
 };
 
 // A place in the line; the same in all lanes of a warp.
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, int OVER>
 struct ChunkCursor {
+    using Line = ChunkLine<ROWS, KEYS, OVER>;
     int z, h, qt, tile, tiles, keys, kv, ql, n_qt;
 
-    __device__ __forceinline__ void at_row_tile(const ChunkLine<ROWS, KEYS> &line) {
+    __device__ __forceinline__ void at_row_tile(const Line &line) {
         keys = line.keys(kv, ql, qt);
         tiles = line.tiles_of(keys);
     }
-    __device__ __forceinline__ void open(const ChunkLine<ROWS, KEYS> &line) {
+    __device__ __forceinline__ void open(const Line &line) {
         kv = line.kv_len(z);
         ql = line.q_len(z);
         n_qt = line.row_tiles(ql);
     }
     // by a whole warp: length of the line
-    __device__ __forceinline__ static long long total(const ChunkLine<ROWS, KEYS> &line) {
+    __device__ __forceinline__ static long long total(const Line &line) {
         const int lane = threadIdx.x & 31;
         long long sum = 0;
         if (line.wide()) {
 #pragma unroll 1
-            for (int z = 0; z < line.a.Z; ++z) sum += line.head_tiles_by_warp(line.kv_len(z), line.q_len(z));
+            for (int z = 0; z < line.a.Z; ++z) sum += line.head_units_by_warp(line.kv_len(z), line.q_len(z));
             return sum * line.a.H_kv;
         }
 #pragma unroll 1
-        for (int z = lane; z < line.a.Z; z += 32) sum += line.head_tiles(line.kv_len(z), line.q_len(z));
+        for (int z = lane; z < line.a.Z; z += 32) sum += line.head_units(line.kv_len(z), line.q_len(z));
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
         return sum * line.a.H_kv;
@@ -128,26 +131,34 @@ struct ChunkCursor {
         }
         return v;
     }
-    // by a whole warp: to tile `pos` of the line, which has to be in it
-    __device__ __forceinline__ void seek(const ChunkLine<ROWS, KEYS> &line, long long pos) {
+    // by a whole warp: to the tile at or behind unit `pos` of the line, which has to be in it; the tiles of the line ahead of that one
+    __device__ __forceinline__ long long seek(const Line &line, long long pos) {
         const int lane = threadIdx.x & 31;
-        long long head = 1;
+        const long long at = pos;
+        long long head = 1, items = 0;                    // of the sequences ahead
         z = 0;
         if (line.wide()) {
 #pragma unroll 1
             for (;; ++z) {
-                head = line.head_tiles_by_warp(line.kv_len(z), line.q_len(z));
+                head = line.head_units_by_warp(line.kv_len(z), line.q_len(z));
                 if (pos < head * line.a.H_kv || z + 1 == line.a.Z) break;
                 pos -= head * line.a.H_kv;
+                items += line.row_tiles(line.q_len(z));
             }
         } else {
 #pragma unroll 1
             for (int z0 = 0; z0 < line.a.Z; z0 += 32) {
-                const long long mine = z0 + lane < line.a.Z ? line.head_tiles(line.kv_len(z0 + lane), line.q_len(z0 + lane)) : 0;
+                const bool real = z0 + lane < line.a.Z;
+                const int mine_q = real ? line.q_len(z0 + lane) : 0;
+                const long long mine = real ? line.head_units(line.kv_len(z0 + lane), mine_q) : 0;
                 const long long upto = scan(mine * line.a.H_kv);
                 const unsigned past = __ballot_sync(0xffffffffu, pos < upto);
+                const int f = past != 0u ? __ffs(past) - 1 : 32;
+                long long n = lane < f ? line.row_tiles(mine_q) : 0;
+#pragma unroll
+                for (int s = 16; s > 0; s >>= 1) n += __shfl_xor_sync(0xffffffffu, n, s);
+                items += n;
                 if (past != 0u) {
-                    const int f = __ffs(past) - 1;
                     z = z0 + f;
                     head = __shfl_sync(0xffffffffu, mine, f);
                     pos -= __shfl_sync(0xffffffffu, upto, f) - head * line.a.H_kv;
@@ -163,7 +174,7 @@ struct ChunkCursor {
         if (n_qt > 1) {
 #pragma unroll 1
             for (int q0 = 0; q0 < n_qt; q0 += 32) {
-                const long long mine = q0 + lane < n_qt ? line.tiles_of(line.keys(kv, ql, q0 + lane)) : 0, upto = scan(mine);
+                const long long mine = q0 + lane < n_qt ? line.tiles_of(line.keys(kv, ql, q0 + lane)) + OVER : 0, upto = scan(mine);
                 const unsigned past = __ballot_sync(0xffffffffu, pos < upto);
                 if (past != 0u) {
                     const int f = __ffs(past) - 1;
@@ -175,10 +186,11 @@ struct ChunkCursor {
             }
         }
         at_row_tile(line);
-        tile = int(pos);
+        tile = max(0, int(pos) - OVER);
+        return at - pos - OVER * (items * line.a.H_kv + (long long)h * n_qt + qt) + tile;
     }
     // to the next tile; the last tile of the line has none
-    __device__ __forceinline__ void next(const ChunkLine<ROWS, KEYS> &line) {
+    __device__ __forceinline__ void next(const Line &line) {
         if (++tile < tiles) return;
         tile = 0;
         if (++qt == n_qt) {
@@ -199,15 +211,45 @@ struct ChunkCursor {
 };
 
 
+// CTA i of n takes the tiles of units [first(i), first(i + 1)) of the line
+__device__ __forceinline__ long long chunk_first(long long total, int i, int n) { return total / n * i + min((long long)i, total % n); }
+
+// A CTA's piece of the line, found by two of its warps for all (in shared memory).
+template <int ROWS, int KEYS, int OVER>
+struct ChunkPiece {
+    ChunkCursor<ROWS, KEYS, OVER> from;
+    long long total, before, upto;         // units of the line; tiles ahead of my first one, ahead of the next CTA's
+    __device__ __forceinline__ int tiles() const { return int(upto - before); }
+    // by the CTA's first two warps, ahead of a barrier
+    __device__ __forceinline__ void find(const ChunkLine<ROWS, KEYS, OVER> &line) {
+        const int warp = threadIdx.x >> 5;
+        if (warp > 1) return;
+        ChunkCursor<ROWS, KEYS, OVER> c;
+        const long long all = c.total(line), lo = chunk_first(all, blockIdx.x, gridDim.x), hi = chunk_first(all, blockIdx.x + 1, gridDim.x);
+        const bool lead = (threadIdx.x & 31) == 0;
+        if (hi == lo) {
+            if (lead && warp == 0) before = 0;
+            if (lead && warp == 1) upto = 0;
+        } else if (warp == 0) {
+            const long long n = c.seek(line, lo);
+            if (lead) {
+                from = c;
+                before = n;
+                total = all;
+            }
+        } else {
+            const long long n = hi == all ? c.seek(line, hi - 1) + 1 : c.seek(line, hi);         // (the line ends with a tile)
+            if (lead) upto = n;
+        }
+    }
+};
+
 // What the merge has to know of the item that CTA i's last piece begins: its pieces are CTA i's last one and the first ones of the
 // CTAs behind it.
 struct ChunkCut {
     int z, h, qt, ql, pieces;              // 1 (or 0, a CTA without work): nothing to merge
     int pad[3];
 };
-
-// CTA i of n takes [first(i), first(i + 1)) of the line
-__device__ __forceinline__ long long chunk_first(long long total, int i, int n) { return total / n * i + min((long long)i, total % n); }
 
 // ---- values that are not finite where not every row of a tile attends to them.  The second product multiplies a masked
 // key's V by a probability of zero, and zero times NaN or infinity is NaN.  In key groups that some row does not see, such elements
@@ -274,8 +316,8 @@ inline size_t chunk_part_bytes(int n_ctas, int rows, int D) { return chunk_cuts_
 
 // CTA i's note for the merge, by one thread, `last` being its last tile.  (Every CTA behind it takes `per` tiles or one more, so
 // that the count is a division and at most a step or two.)
-template <int ROWS, int D, int KEYS>
-__device__ __forceinline__ void leave_cut(const ChunkArgs &a, const ChunkCursor<ROWS, KEYS> &last, long long total, int n_tiles) {
+template <int D, int ROWS, int KEYS, int OVER>
+__device__ __forceinline__ void leave_cut(const ChunkArgs &a, const ChunkCursor<ROWS, KEYS, OVER> &last, long long total, int n_tiles) {
     ChunkCut cut = {};
     if (n_tiles > 0) {
         cut.z = last.z;
@@ -284,7 +326,7 @@ __device__ __forceinline__ void leave_cut(const ChunkArgs &a, const ChunkCursor<
         cut.ql = last.ql;
         cut.pieces = 1;
         const int behind = last.tiles - last.tile - 1;
-        if (behind > 0 && n_tiles > last.tile) {          // it goes on, and began here
+        if (behind > 0 && n_tiles > last.tile) {          // it goes on (then its next tile is the next CTA's first unit), and began here
             const int me = blockIdx.x, n = gridDim.x;
             const long long end = chunk_first(total, me + 1, n) + behind;
             int c = me + 1 + int((behind - 1) / (total / n + 1));

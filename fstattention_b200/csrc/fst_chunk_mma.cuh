@@ -23,7 +23,7 @@ namespace fst {
 
 template <int D, bool QUANT, int MT>
 struct ChunkMmaGeo {
-    static constexpr int WARPS = 8, KW = !QUANT && D == 128 ? 16 : 32, KEYS = WARPS * KW, ROWS = 16 * MT;
+    static constexpr int WARPS = 8, KW = !QUANT && D == 128 ? 16 : 32, KEYS = WARPS * KW, ROWS = 16 * MT, OVER = 2;
     static constexpr int THREADS = WARPS * 32 + 128;                // and a loading warp, in a warpgroup that gives its registers away
     static constexpr int REGS = 224, REGS_LOADS = 56;
     static_assert(256 * REGS + 128 * REGS_LOADS <= THREADS * 168, "the split draws on what the launch was given");
@@ -72,8 +72,8 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
     using G = ChunkMmaGeo<D, QUANT, MT>;
     using MT_ = MmaTraits<T>;
     using MP = MmaTraits<typename std::conditional<QUANT, __nv_bfloat16, T>::type>;      // of the second product
-    using Line = ChunkLine<G::ROWS, G::KEYS>;
-    using Cursor = ChunkCursor<G::ROWS, G::KEYS>;
+    using Line = ChunkLine<G::ROWS, G::KEYS, G::OVER>;
+    using Cursor = ChunkCursor<G::ROWS, G::KEYS, G::OVER>;
     constexpr bool BF16 = !std::is_same<T, __half>::value;
     constexpr int KS = D / 16, ND = D / 8;               // steps of the first product, column tiles of the second
     constexpr int KW = G::KW, NK = KW / 8, SUBS = KW / 16;
@@ -93,17 +93,17 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    __syncthreads();
-
     const Line line(a);
-    const long long total = Cursor::total(line), first = chunk_first(total, blockIdx.x, gridDim.x);
-    const int n_tiles = int(chunk_first(total, blockIdx.x + 1, gridDim.x) - first);
+    __shared__ ChunkPiece<G::ROWS, G::KEYS, G::OVER> piece;
+    piece.find(line);
+    __syncthreads();
+    Cursor me = piece.from;
+    const long long total = piece.total;
+    const int n_tiles = piece.tiles();
     if (n_tiles == 0) {
-        if (tid == 0 && a.part != nullptr) leave_cut<G::ROWS, D>(a, Cursor{}, total, 0);
+        if (tid == 0 && a.part != nullptr) leave_cut<D>(a, me, total, 0);
         return;
     }
-    Cursor me;
-    me.seek(line, first);
 
     // (each side asks inside its own branch, see chunk_umma_kernel)
     if (warp >= G::WARPS) {
@@ -545,7 +545,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
         }
         if (i + 1 < n_tiles) me.next(line);
     }
-    if (tid == 0 && a.part != nullptr) leave_cut<G::ROWS, D>(a, me, total, n_tiles);
+    if (tid == 0 && a.part != nullptr) leave_cut<D>(a, me, total, n_tiles);
 }
 
 template <typename T, int D, bool QUANT, int MT>

@@ -26,7 +26,7 @@ namespace fst {
 
 template <int D, bool QUANT>
 struct ChunkUmmaGeo {
-    static constexpr int ROWS = 256, KEYS = 128, THREADS = 512;
+    static constexpr int ROWS = 256, KEYS = 128, THREADS = 512, OVER = 3;
     static constexpr int TILE = (D / 64) * umma::HALF;              // 128 rows
     static constexpr int QBUF = D == 128 ? 1 : 2;                   // items whose Q is there at a time
     static constexpr int RING = QUANT ? (D == 128 ? 3 : 6) : (D == 128 ? 4 : 8);
@@ -124,8 +124,8 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
     using namespace umma;
     using G = ChunkUmmaGeo<D, QUANT>;
     using MT = MmaTraits<T>;
-    using Line = ChunkLine<G::ROWS, G::KEYS>;
-    using Cursor = ChunkCursor<G::ROWS, G::KEYS>;
+    using Line = ChunkLine<G::ROWS, G::KEYS, G::OVER>;
+    using Cursor = ChunkCursor<G::ROWS, G::KEYS, G::OVER>;
     constexpr bool BF16 = !std::is_same<T, __half>::value;
     constexpr int DH = D / 64, TILE = G::TILE, RING = G::RING, QBUF = G::QBUF, RAW = G::RAW;
 
@@ -168,15 +168,14 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
         fence_before_sync();
     }
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    const Line line(a);
+    __shared__ ChunkPiece<G::ROWS, G::KEYS, G::OVER> piece;
+    piece.find(line);
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = *tmem_slot;
-
-    const Line line(a);
-    const long long total = Cursor::total(line), first = chunk_first(total, blockIdx.x, gridDim.x);
-    const int n_tiles = int(chunk_first(total, blockIdx.x + 1, gridDim.x) - first);
-    Cursor me;
-    if (n_tiles > 0) me.seek(line, first);
+    Cursor me = piece.from;
+    const int n_tiles = piece.tiles();
     const int where = blockIdx.x;
     // key tiles of the item that group g takes part in: none where it has no rows, and the first group sees less than the second
     auto group_tiles = [&](int g) {
@@ -533,7 +532,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
             if (i + 1 < n_tiles) me.next(line);
         }
         }
-        if (t128 == 0 && a.part != nullptr) leave_cut<G::ROWS, D>(a, me, total, n_tiles);
+        if (t128 == 0 && a.part != nullptr) leave_cut<D>(a, me, piece.total, n_tiles);
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(G::REGS_SOFTMAX));
