@@ -10,6 +10,7 @@
 namespace fst {
 
 constexpr int CACHE_THREADS = 256;
+constexpr int CACHE_ROWS = 2;          // rows of a thread where there are many: 8192 rows of 8 heads quantised, 1: 12.9 us, 2: 11.0, 4: 12.0; 30011 read, 36.8, 33.2, 37.1
 
 template <typename T>
 __device__ __forceinline__ float2 two_floats(uint32_t w) {
@@ -17,86 +18,98 @@ __device__ __forceinline__ float2 two_floats(uint32_t w) {
     else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w));
 }
 
-// Eight values of a row that D / 8 neighbouring lanes hold: the row's largest magnitude is taken over them.
+// Eight values of a row that D / 8 neighbouring lanes hold: the row's largest magnitude is taken over them.  Magnitudes are compared as
+// integers, two at a time, where NaN and infinity are the largest (instructions bound large appends: 12.9 us with floats, 11.2 so).
 template <typename T, int D>
 __device__ __forceinline__ uint2 quantise8(uint4 in, uint32_t &biased) {
+    constexpr bool HALF = std::is_same<T, __half>::value;
     const uint32_t w[4] = {in.x, in.y, in.z, in.w};
-    float x[8], a = 0.f;
-    bool finite = true;
+    uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 p = two_floats<T>(w[i]);
-        x[2 * i] = p.x;
-        x[2 * i + 1] = p.y;
-        a = fmaxf(a, fmaxf(fabsf(p.x), fabsf(p.y)));
-        finite = finite && !isnan(p.x) && !isnan(p.y);    // (a maximum passes over them)
-    }
-    if (!finite) a = INFINITY;
-#pragma unroll
-    for (int s = 1; s < D / 8; s *= 2) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, s));
-    if (a == INFINITY) {
+    for (int s = 1; s < D / 8; s *= 2) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, s));
+    top = max(top & 0xffffu, top >> 16);
+    if (top >= (HALF ? 0x7c00u : 0x7f80u)) {
         biased = 255u;
         return make_uint2(0u, 0u);
     }
-    const int e = e4m3_exponent(a);
+    const int e = e4m3_exponent(two_floats<T>(top).x);
     const float f = pow2f(-e);
     biased = uint32_t(e + 127);
     uint32_t b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = e4m3_pair(x[2 * i] * f, x[2 * i + 1] * f);
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = two_floats<T>(w[i]);
+        b[i] = e4m3_pair(x.x * f, x.y * f);
+    }
     return make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
 }
 
-template <typename T, int D, bool QUANT>
+// Rows j of head h of sequence z, neighbours in the source and in a page by neighbouring threads.  R = 1: all (z, h, j) in one line.  R > 1: a block has
+// R * RPB rows of one head, so that nothing is divided and a thread has R rows on their way.
+template <typename T, int D, bool QUANT, int R>
 __global__ void __launch_bounds__(CACHE_THREADS)
 cache_append_kernel(const AppendArgs a) {
     constexpr int LPR = D / 8, RPB = CACHE_THREADS / LPR;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    // unit: row j of head h of sequence z, j fastest (neighbouring rows of the source, and of a page)
-    const unsigned unit = blockIdx.x * RPB + threadIdx.x / LPR, col = (threadIdx.x % LPR) * 8;
-    const unsigned zh = unit / unsigned(a.M), j = unit - zh * unsigned(a.M), z = zh / unsigned(a.H_kv), h = zh - z * unsigned(a.H_kv);
-    bool live = z < unsigned(a.Z);
-    uint4 k = make_uint4(0, 0, 0, 0), v = k;
-    int64_t pos = 0;
-    if (live) {
-        int row = a.rows != nullptr ? __ldg(a.rows + size_t(z) * a.M + j) : int(j);
+    const unsigned first = blockIdx.x * (RPB * R) + threadIdx.x / LPR, col = (threadIdx.x % LPR) * 8;
+    uint4 k[R], v[R];
+    int64_t pos[R];
+    int page[R];
+    unsigned head[R];
+    bool live[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        unsigned j = first + i * RPB, z = blockIdx.z, h = blockIdx.y;
+        if constexpr (R == 1) {
+            const unsigned zh = j / unsigned(a.M);
+            j -= zh * unsigned(a.M);
+            z = zh / unsigned(a.H_kv);
+            h = zh - z * unsigned(a.H_kv);
+        }
+        live[i] = R == 1 ? z < unsigned(a.Z) : j < unsigned(a.M);
+        k[i] = v[i] = make_uint4(0, 0, 0, 0);
+        pos[i] = 0;
+        page[i] = 0;
+        head[i] = h;
+        if (!live[i]) continue;
+        const int row = a.rows != nullptr ? __ldg(a.rows + size_t(z) * a.M + j) : int(j);
         const int count = a.lens != nullptr ? __ldg(a.lens + z) : a.M;
-        pos = int64_t(__ldg(a.start + z)) + j;
-        live = int(j) < count;
-        if (live && (row < 0 || row >= a.N || pos < 0 || (pos >> a.c.page_shift) >= a.c.width)) {
+        pos[i] = int64_t(__ldg(a.start + z)) + j;
+        live[i] = int(j) < count;
+        if (live[i] && (row < 0 || row >= a.N || pos[i] < 0 || (pos[i] >> a.c.page_shift) >= a.c.width)) {
             if (col == 0) report(a.status, FST_DEV_INDEX_RANGE, int(z), int(j));
-            live = false;
+            live[i] = false;
         }
-        if (live) {
-            k = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.k) + z * a.ks_z + h * a.ks_h + row * a.ks_n + col));
-            v = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.v) + z * a.vs_z + h * a.vs_h + row * a.vs_n + col));
+        if (live[i]) {
+            k[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.k) + z * a.ks_z + h * a.ks_h + row * a.ks_n + col));
+            v[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.v) + z * a.vs_z + h * a.vs_h + row * a.vs_n + col));
+            page[i] = __ldg(a.c.table + size_t(z) * a.c.width + (pos[i] >> a.c.page_shift));
+            if (unsigned(page[i]) >= unsigned(a.c.n_pages)) {
+                if (col == 0) report(a.status, FST_DEV_INDEX_RANGE, int(z), int(j));
+                live[i] = false;
+            }
         }
     }
-    int page = 0;
-    if (live) {
-        page = __ldg(a.c.table + size_t(z) * a.c.width + (pos >> a.c.page_shift));
-        if (unsigned(page) >= unsigned(a.c.n_pages)) {
-            if (col == 0) report(a.status, FST_DEV_INDEX_RANGE, int(z), int(j));
-            live = false;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int off = int(pos[i]) & ((1 << a.c.page_shift) - 1);
+        const int64_t to = page[i] * a.c.stride_page + off * a.c.stride_row + head[i] * a.c.stride_head + col;
+        if constexpr (QUANT) {
+            uint32_t ek, ev;                              // (all lanes take part in the maximum)
+            const uint2 qk = quantise8<T, D>(k[i], ek), qv = quantise8<T, D>(v[i], ev);
+            if (!live[i]) continue;
+            *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(a.c.k_pool) + to) = qk;
+            *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(a.c.v_pool) + to) = qv;
+            if (col == 0) {
+                const size_t at = ((size_t(page[i]) * a.H_kv + head[i]) << a.c.page_shift) + off;
+                a.c.k_scale[at] = uint8_t(ek);
+                a.c.v_scale[at] = uint8_t(ev);
+            }
+        } else if (live[i]) {
+            *reinterpret_cast<uint4 *>(static_cast<T *>(a.c.k_pool) + to) = k[i];
+            *reinterpret_cast<uint4 *>(static_cast<T *>(a.c.v_pool) + to) = v[i];
         }
-    }
-    const int off = int(pos) & ((1 << a.c.page_shift) - 1);
-    const int64_t to = page * a.c.stride_page + off * a.c.stride_row + h * a.c.stride_head + col;
-    if constexpr (QUANT) {
-        uint32_t ek, ev;                                  // (all lanes take part in the maximum)
-        const uint2 qk = quantise8<T, D>(k, ek), qv = quantise8<T, D>(v, ev);
-        if (!live) return;
-        *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(a.c.k_pool) + to) = qk;
-        *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(a.c.v_pool) + to) = qv;
-        if (col == 0) {
-            const size_t at = ((size_t(page) * a.H_kv + h) << a.c.page_shift) + off;
-            a.c.k_scale[at] = uint8_t(ek);
-            a.c.v_scale[at] = uint8_t(ev);
-        }
-    } else if (live) {
-        *reinterpret_cast<uint4 *>(static_cast<T *>(a.c.k_pool) + to) = k;
-        *reinterpret_cast<uint4 *>(static_cast<T *>(a.c.v_pool) + to) = v;
     }
 }
 
@@ -112,38 +125,65 @@ __device__ __forceinline__ uint4 expand8(uint2 b, float scale) {
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-template <typename T, int D, bool QUANT>
+// Eight values a lane, so that the lanes of a row write it as a whole.  R as above; a block that lies behind its sequence's end only writes.
+template <typename T, int D, bool QUANT, int R>
 __global__ void __launch_bounds__(CACHE_THREADS)
 cache_read_kernel(const ReadArgs a) {
     constexpr int LPR = D / 8, RPB = CACHE_THREADS / LPR;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    const unsigned unit = blockIdx.x * RPB + threadIdx.x / LPR, col = (threadIdx.x % LPR) * 8;
-    const unsigned zh = unit / unsigned(a.M), r = unit - zh * unsigned(a.M), z = zh / unsigned(a.H_kv), h = zh - z * unsigned(a.H_kv);
-    if (z >= unsigned(a.Z)) return;
-    uint4 k = make_uint4(0, 0, 0, 0), v = k;
-    if (int(r) < __ldg(a.lens + z)) {                     // (rows behind a sequence's end are zeros)
+    const unsigned first = blockIdx.x * (RPB * R) + threadIdx.x / LPR, col = (threadIdx.x % LPR) * 8;
+    uint4 k[R], v[R];
+    float ek[R], ev[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        unsigned r = first + i * RPB, z = blockIdx.z, h = blockIdx.y;
+        if constexpr (R == 1) {
+            const unsigned zh = r / unsigned(a.M);
+            r -= zh * unsigned(a.M);
+            z = zh / unsigned(a.H_kv);
+            h = zh - z * unsigned(a.H_kv);
+        }
+        k[i] = v[i] = make_uint4(0, 0, 0, 0);             // (rows behind a sequence's end are zeros)
+        ek[i] = ev[i] = 0.f;
+        if ((R == 1 ? z >= unsigned(a.Z) : r >= unsigned(a.M)) || int(r) >= __ldg(a.lens + z)) continue;
         const int idx = int(r >> a.c.page_shift), page = idx < a.c.width ? __ldg(a.c.table + size_t(z) * a.c.width + idx) : -1;
         if (unsigned(page) >= unsigned(a.c.n_pages)) {
             if (col == 0) report(a.status, FST_DEV_INDEX_RANGE, int(z), int(r));
+            continue;
+        }
+        const int off = int(r) & ((1 << a.c.page_shift) - 1);
+        const int64_t from = page * a.c.stride_page + off * a.c.stride_row + h * a.c.stride_head + col;
+        if constexpr (QUANT) {
+            const size_t at = ((size_t(page) * a.H_kv + h) << a.c.page_shift) + off;
+            const uint2 bk = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.k_pool) + from));
+            const uint2 bv = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.v_pool) + from));
+            k[i] = make_uint4(bk.x, bk.y, 0, 0);
+            v[i] = make_uint4(bv.x, bv.y, 0, 0);
+            ek[i] = e8m0_value(__ldg(a.c.k_scale + at));
+            ev[i] = e8m0_value(__ldg(a.c.v_scale + at));
         } else {
-            const int off = int(r) & ((1 << a.c.page_shift) - 1);
-            const int64_t from = page * a.c.stride_page + off * a.c.stride_row + h * a.c.stride_head + col;
-            if constexpr (QUANT) {
-                const size_t at = ((size_t(page) * a.H_kv + h) << a.c.page_shift) + off;
-                const uint2 bk = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.k_pool) + from));
-                const uint2 bv = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.v_pool) + from));
-                const float ek = e8m0_value(__ldg(a.c.k_scale + at)), ev = e8m0_value(__ldg(a.c.v_scale + at));
-                k = expand8<T>(bk, ek);
-                v = expand8<T>(bv, ev);
-            } else {
-                k = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.c.k_pool) + from));
-                v = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.c.v_pool) + from));
-            }
+            k[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.c.k_pool) + from));
+            v[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.c.v_pool) + from));
         }
     }
-    *reinterpret_cast<uint4 *>(static_cast<T *>(a.k) + z * a.ks_z + h * a.ks_h + r * a.ks_n + col) = k;
-    *reinterpret_cast<uint4 *>(static_cast<T *>(a.v) + z * a.vs_z + h * a.vs_h + r * a.vs_n + col) = v;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        unsigned r = first + i * RPB, z = blockIdx.z, h = blockIdx.y;
+        if constexpr (R == 1) {
+            const unsigned zh = r / unsigned(a.M);
+            r -= zh * unsigned(a.M);
+            z = zh / unsigned(a.H_kv);
+            h = zh - z * unsigned(a.H_kv);
+        }
+        if (R == 1 ? z >= unsigned(a.Z) : r >= unsigned(a.M)) continue;
+        if constexpr (QUANT) {
+            k[i] = expand8<T>(make_uint2(k[i].x, k[i].y), ek[i]);
+            v[i] = expand8<T>(make_uint2(v[i].x, v[i].y), ev[i]);
+        }
+        *reinterpret_cast<uint4 *>(static_cast<T *>(a.k) + z * a.ks_z + h * a.ks_h + r * a.ks_n + col) = k[i];
+        *reinterpret_cast<uint4 *>(static_cast<T *>(a.v) + z * a.vs_z + h * a.vs_h + r * a.vs_n + col) = v[i];
+    }
 }
 
 // A block takes pages of one head, every gridDim.x-th of all that hold rows; the lengths are read once per 256 sequences.
@@ -209,14 +249,11 @@ cudaError_t launch_cache_expand(const ExpandArgs &a, int dtype, int D, cudaStrea
     return D == 128 ? launch_expand_t<__nv_bfloat16, 128>(a, stream) : launch_expand_t<__nv_bfloat16, 64>(a, stream);
 }
 
-// One lane group per row; launched so that the grid may become resident while the one ahead of it drains.
-template <int D, typename K, typename A>
-static cudaError_t launch_rows(K kernel, const A &a, cudaStream_t stream) {
-    constexpr int RPB = CACHE_THREADS / (D / 8);
-    const long long units = (long long)a.Z * a.H_kv * a.M;
-    if (units > 0x7fffffffLL - RPB) return cudaErrorInvalidConfiguration;
+// Launched so that the grid may become resident while the one ahead of it drains.
+template <typename K, typename A>
+static cudaError_t launch_rows(K kernel, const A &a, dim3 grid, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned((units + RPB - 1) / RPB));
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(CACHE_THREADS);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -226,16 +263,31 @@ static cudaError_t launch_rows(K kernel, const A &a, cudaStream_t stream) {
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
+// The one-row kernel where rows are few or would not fill blocks of R * RPB of one head, else the R-row one.
+template <int R, int RPB, typename K1, typename KR, typename A>
+static cudaError_t launch_rows(K1 one, KR several, const A &a, cudaStream_t stream) {
+    const long long units = (long long)a.Z * a.H_kv * a.M;
+    if (a.M >= 2 * R * RPB && units >= 8LL * R * RPB * sm_count() && a.H_kv <= 65535 && a.Z <= 65535)
+        return launch_rows(several, a, dim3((a.M + R * RPB - 1) / (R * RPB), a.H_kv, a.Z), stream);
+    if (units > 0x7fffffffLL - RPB) return cudaErrorInvalidConfiguration;
+    return launch_rows(one, a, dim3(unsigned((units + RPB - 1) / RPB)), stream);
+}
 
+template <typename T, int D, bool QUANT>
+static cudaError_t launch_append_t(const AppendArgs &a, cudaStream_t stream) {
+    return launch_rows<CACHE_ROWS, CACHE_THREADS / (D / 8)>(cache_append_kernel<T, D, QUANT, 1>, cache_append_kernel<T, D, QUANT, CACHE_ROWS>, a, stream);
+}
+template <typename T, int D, bool QUANT>
+static cudaError_t launch_read_t(const ReadArgs &a, cudaStream_t stream) {
+    return launch_rows<CACHE_ROWS, CACHE_THREADS / (D / 8)>(cache_read_kernel<T, D, QUANT, 1>, cache_read_kernel<T, D, QUANT, CACHE_ROWS>, a, stream);
+}
 template <typename T, int D>
 static cudaError_t launch_append_t(const AppendArgs &a, cudaStream_t stream) {
-    return a.c.k_scale != nullptr ? launch_rows<D>(cache_append_kernel<T, D, true>, a, stream)
-                                  : launch_rows<D>(cache_append_kernel<T, D, false>, a, stream);
+    return a.c.k_scale != nullptr ? launch_append_t<T, D, true>(a, stream) : launch_append_t<T, D, false>(a, stream);
 }
 template <typename T, int D>
 static cudaError_t launch_read_t(const ReadArgs &a, cudaStream_t stream) {
-    return a.c.k_scale != nullptr ? launch_rows<D>(cache_read_kernel<T, D, true>, a, stream)
-                                  : launch_rows<D>(cache_read_kernel<T, D, false>, a, stream);
+    return a.c.k_scale != nullptr ? launch_read_t<T, D, true>(a, stream) : launch_read_t<T, D, false>(a, stream);
 }
 
 cudaError_t launch_cache_append(const AppendArgs &a, int dtype, int D, cudaStream_t stream) {

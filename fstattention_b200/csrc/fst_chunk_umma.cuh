@@ -39,7 +39,8 @@ struct ChunkUmmaGeo {
     static constexpr int OFF_SCALES = OFF_NOTE + 16;                // [raw stage] 128 bytes
     static constexpr int OFF_PLAN = OFF_SCALES + RAW * 128;         // [stage] what a tile is to the issuing lane, see there
     static constexpr int OFF_RAW_PLAN = OFF_PLAN + RING * 4;        // [raw stage] the same
-    static constexpr int BYTES = OFF_RAW_PLAN + RAW * 4 + 1024;     // + alignment
+    static constexpr int OFF_PIECE = (OFF_RAW_PLAN + RAW * 4 + 15) & ~15;       // ChunkPiece
+    static constexpr int BYTES = OFF_PIECE + 96 + 1024;             // + alignment
     // of 65536 registers a launch of 512 threads gets 128 each; the softmax warps take 192 and leave 64 to the others
     static constexpr int REGS_SOFTMAX = 192, REGS_OTHERS = 64;
 };
@@ -169,7 +170,9 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
     }
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const Line line(a);
-    __shared__ ChunkPiece<G::ROWS, G::KEYS, G::OVER> piece;
+    using Piece = ChunkPiece<G::ROWS, G::KEYS, G::OVER>;
+    static_assert(sizeof(Piece) <= 96, "its place");
+    Piece &piece = *reinterpret_cast<Piece *>(smem + G::OFF_PIECE);
     piece.find(line);
     __syncthreads();
     fence_after_sync();
@@ -589,7 +592,6 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                 // between (an exponential keeps its unit for 8 cycles, a maximum fits in).  Where a row has outgrown the reference by more
                 // than 2^8 it moves, what was summed so far with it, and they are taken again.  On a piece's first tile the maximum comes first.
                 uint64_t l2[2], scale2 = pair(c2, c2), shift2;
-                uint32_t packed[2][16];
                 if (j == 0) {
                     float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
@@ -608,11 +610,12 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                     float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
                     l2[0] = l2[1] = 0;
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t packed[16];
 #pragma unroll
                         for (int k = 0; k < 32; k += 2) {
                             const float x0 = __uint_as_float(s[c][k]), x1 = __uint_as_float(s[c][k + 1]);
-                            exp2_pair(fma2(pair(x0, x1), scale2, shift2), l2[(k >> 1) & 1], packed[c][k >> 1]);
+                            exp2_pair(fma2(pair(x0, x1), scale2, shift2), l2[(k >> 1) & 1], packed[k >> 1]);
                             if ((k >> 1) & 1) {
                                 m0 = max3(m0, x0, x1);
                                 m1 = max3(m1, __uint_as_float(s[c + 2][k]), __uint_as_float(s[c + 2][k + 1]));
@@ -621,6 +624,8 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                                 m3 = max3(m3, __uint_as_float(s[c + 2][k]), __uint_as_float(s[c + 2][k + 1]));
                             }
                         }
+                        tmem_st16(tmem_p + c * 16, packed);       // (nobody reads it before it is announced)
+                    }
                     const float mx = max3(fmaxf(m0, m1), m2, m3);
                     const bool up = (mx - m_ref) * c2 > 8.f;
                     if (again > 0 || j == 0 || !__any_sync(0xffffffffu, up)) break;
@@ -638,16 +643,14 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                     l *= alpha;
                     if (up) m_ref = mx;
                 }
-                tmem_st16(tmem_p, packed[0]);
-                tmem_st16(tmem_p + 16, packed[1]);
                 announce(my_p);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
+                    uint32_t packed[16];
 #pragma unroll
                     for (int k = 0; k < 32; k += 2)
-                        exp2_pair(fma2(pair(__uint_as_float(s[c + 2][k]), __uint_as_float(s[c + 2][k + 1])), scale2, shift2), l2[(k >> 1) & 1],
-                                  packed[c][k >> 1]);
-                    tmem_st16(tmem_p + 32 + c * 16, packed[c]);
+                        exp2_pair(fma2(pair(__uint_as_float(s[c + 2][k]), __uint_as_float(s[c + 2][k + 1])), scale2, shift2), l2[(k >> 1) & 1], packed[k >> 1]);
+                    tmem_st16(tmem_p + 32 + c * 16, packed);
                 }
                 announce(my_p + 8);
                 float la, lb;
