@@ -5,14 +5,14 @@
 // fill a ring of tiles, each of the eight others takes 16 or 32 keys of a tile and has an accumulator of its own for all rows, so
 // that nothing but the ring's barriers lies between them.  They meet once per item, to add up.
 //
-// 8-bit rows become matrix fragments in registers.  The order of the summed index is free as long as both operands agree, so
-// lane (g, t) of a K fragment takes the contiguous bytes D/4 t .. of key g, and Q is loaded in the same order;
-// of V it takes bytes D/8 g .. of its four keys, which only permutes the columns of the result.  A byte
-// becomes a 16-bit float by moving its seven low bits under the format's exponent: bf16 holds value * 2^-120, fp16
-// value * 2^-8 (subnormals included), and the missing power of two goes where a multiplication is made anyway: for K into Q (2^60,
-// bf16) and into the score's factor with the key's own scale, for V into the probability with the row's scale (2^60) and
-// the final division.  Probabilities and V are bf16 for an 8-bit cache under fp16 queries too: 2^e of a row and its probability need the
-// range, and V has four significant bits.
+// 8-bit rows become matrix fragments in registers, without their scales.  The order of the summed index is free as long as both operands
+// agree, so lane (g, t) of a K fragment takes the contiguous bytes D/4 t .. of key g, and Q is loaded in the same order; of V it
+// takes bytes D/8 g .. of its four keys, which only permutes the columns of the result.  K is fp16, by the conversion instruction, and a
+// key's scale multiplies its score.  bf16 queries become fp16 times a power of two per row, with the row's largest value next to 2^15:
+// what fp16 loses then is 2^-39 of that.  V is bf16, as a row's scale goes into its probability and needs the range: a byte's seven
+// low bits moved under bf16's exponent are its value * 2^-120, half of which comes back with the scale and half at the end.
+// (Two sequences of 115000 rows: K by its bits as well 118 us; V as fp16 by the instruction, the scales in the exponents of weights
+// of their own, 108 us, but 47 instead of 41 with 28 rows a tile; as it is ...)
 #pragma once
 
 #include "fst_chunk.cuh"
@@ -40,14 +40,17 @@ struct ChunkMmaGeo {
 
 constexpr float kTiny = 1.152921504606846976e18f;        // 2^60, half of what a bf16 made of an e4m3's bits lacks
 
-// four e4m3 bytes -> two pairs of 16-bit floats (bytes 0 and 2, bytes 1 and 3), smaller by 2^120 (bf16) or 2^8 (fp16)
-template <bool BF16>
-__device__ __forceinline__ void widen(uint32_t w, uint32_t &even, uint32_t &odd) {
-    constexpr int S = BF16 ? 4 : 1;
-    constexpr uint32_t M = BF16 ? 0x07f007f0u : 0x3f803f80u;
-    odd = (w & 0x80008000u) | ((w >> S) & M);
+// four e4m3 bytes -> two pairs of bf16 (bytes 0 and 2, bytes 1 and 3), smaller by 2^120
+__device__ __forceinline__ void e4m3_bits(uint32_t w, uint32_t &even, uint32_t &odd) {
+    odd = (w & 0x80008000u) | ((w >> 4) & 0x07f007f0u);
     const uint32_t u = w << 8;
-    even = (u & 0x80008000u) | ((u >> S) & M);
+    even = (u & 0x80008000u) | ((u >> 4) & 0x07f007f0u);
+}
+// two e4m3 bytes (the low ones, the high ones) -> a pair of fp16
+__device__ __forceinline__ uint32_t e4m3_halves(uint32_t w, bool high) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(r) : "h"(uint16_t(high ? w >> 16 : w)));
+    return r;
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -71,7 +74,8 @@ __global__ void __launch_bounds__(384, 1)
 chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
     using G = ChunkMmaGeo<D, QUANT, MT>;
     using MT_ = MmaTraits<T>;
-    using MP = MmaTraits<typename std::conditional<QUANT, __nv_bfloat16, T>::type>;      // of the second product
+    using MK = MmaTraits<typename std::conditional<QUANT, __half, T>::type>;     // of the first product, of the second
+    using MP = MmaTraits<typename std::conditional<QUANT, __nv_bfloat16, T>::type>;
     using Line = ChunkLine<G::ROWS, G::KEYS, G::OVER>;
     using Cursor = ChunkCursor<G::ROWS, G::KEYS, G::OVER>;
     constexpr bool BF16 = !std::is_same<T, __half>::value;
@@ -179,7 +183,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
     auto group_of = [&](const Cursor &c) { return c.tile * G::KEYS + warp * KW; };
 
     // ---- products
-    const float c2 = a.scale_log2 * (QUANT ? (BF16 ? kTiny : 256.f) : 1.f);
+    const float c2 = a.scale_log2;
     uint32_t qf[G::Q_SHARED ? 1 : MT][G::Q_SHARED ? 1 : KS][4];
     const uint32_t q_at = s_base + G::OFF_Q + lane * 16;
     // fragment of step st of row tile x
@@ -193,6 +197,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
         }
     };
     float acc[MT][ND][4], m[MT][2], l[MT][2];
+    float row_c2[QUANT ? MT : 1][2];                      // an 8-bit cache: c2 over the row's factor
     int limit[MT][2], lim_first = 0, slot = 0;
     uint32_t parity = 0;
     bool poisoned = false, alive = true;                  // a V that is not finite was met where not every row attends to it
@@ -214,23 +219,31 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     m[x][hh] = -INFINITY;
                     l[x][hh] = 0.f;
                     const T *src = static_cast<const T *>(a.q) + me.z * a.qs_z + (me.h * a.group + (r - tok * a.group)) * a.qs_h + tok * a.qs_n;
-                    // two of the four registers of the row tile's fragments: the row's part of two steps in an 8-bit cache's order, or of one
-                    auto two_steps = [&](int s2, uint32_t (&f)[4]) {         // steps 2 s2 and 2 s2 + 1: D / 4 contiguous values, K's bytes' order
-                        uint4 w = real ? __ldg(reinterpret_cast<const uint4 *>(src + t * (D / 4) + s2 * 8)) : make_uint4(0, 0, 0, 0);
+                    // two of the four registers of a row tile's fragments: the row's part of two steps in an 8-bit cache's order, or of one
+                    float by = 1.f;                       // the row's factor
+                    if constexpr (QUANT) {
                         if constexpr (BF16) {
-                            const __nv_bfloat162 by = __float2bfloat162_rn(kTiny);
-                            uint32_t *p = &w.x;
+                            uint32_t top = 0;
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const __nv_bfloat162 y = __hmul2(*reinterpret_cast<__nv_bfloat162 *>(p + k), by);
-                                p[k] = *reinterpret_cast<const uint32_t *>(&y);
+                            for (int s2 = 0; s2 < KS / 2; ++s2) {
+                                const uint4 w = real ? __ldg(reinterpret_cast<const uint4 *>(src + t * (D / 4) + s2 * 8)) : make_uint4(0, 0, 0, 0);
+                                top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
                             }
+                            top = max(top & 0xffffu, top >> 16);
+                            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                            // exponent of the largest magnitude to 14; rows of zeros, and of what is not finite, as they are
+                            if (top >= 0x80u && top < 0x7f80u) by = pow2f(min(141 - int(top >> 7), 126));
                         }
-                        // widen() gives bytes (0, 2) and (1, 3): Q's pairs to match
-                        f[0] = __byte_perm(w.x, w.y, 0x5410);
-                        f[1] = __byte_perm(w.x, w.y, 0x7632);
-                        f[2] = __byte_perm(w.z, w.w, 0x5410);
-                        f[3] = __byte_perm(w.z, w.w, 0x7632);
+                        row_c2[x][hh] = c2 / by;
+                    }
+                    auto two_steps = [&](int s2, uint32_t (&f)[4]) {         // steps 2 s2 and 2 s2 + 1: D / 4 contiguous values
+                        const uint4 w = real ? __ldg(reinterpret_cast<const uint4 *>(src + t * (D / 4) + s2 * 8)) : make_uint4(0, 0, 0, 0);
+                        f[0] = w.x; f[1] = w.y; f[2] = w.z; f[3] = w.w;
+                        if constexpr (BF16) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) f[k] = MK::pack(__uint_as_float(f[k] << 16) * by, __uint_as_float(f[k] & 0xffff0000u) * by);
+                        }
                     };
                     auto one_step = [&](int st, uint32_t &lo, uint32_t &hi) {
                         lo = real ? __ldg(reinterpret_cast<const uint32_t *>(src + st * 16 + 2 * t)) : 0u;
@@ -301,10 +314,10 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         for (int x = 0; x < MT; ++x) q_frag(x, c * 4 + k, q[x]);
 #pragma unroll
                         for (int n = 0; n < NK; ++n) {
-                            uint32_t b0, b1;
-                            widen<BF16>(k == 0 ? b[n].x : k == 1 ? b[n].y : k == 2 ? b[n].z : b[n].w, b0, b1);
+                            const uint32_t w = k == 0 ? b[n].x : k == 1 ? b[n].y : k == 2 ? b[n].z : b[n].w;
+                            const uint32_t b0 = e4m3_halves(w, false), b1 = e4m3_halves(w, true);
 #pragma unroll
-                            for (int x = 0; x < MT; ++x) MT_::mma(s[x][n], q[x], b0, b1);
+                            for (int x = 0; x < MT; ++x) MK::mma(s[x][n], q[x], b0, b1);
                         }
                     }
                 }
@@ -335,17 +348,17 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
             for (int x = 0; x < MT; ++x) mx[x][0] = mx[x][1] = -INFINITY;
 #pragma unroll
             for (int n = 0; n < NK; ++n) {
-                float ks[2] = {c2, c2};                   // of my keys 8 n + 2 t + k
+                float ks[2] = {1.f, 1.f};                 // of my keys 8 n + 2 t + k
                 if constexpr (QUANT) {
                     const uint32_t b = *reinterpret_cast<const uint16_t *>(scales + 8 * n + 2 * t);
-                    ks[0] = e8m0_value(b & 255u) * c2;
-                    ks[1] = e8m0_value(b >> 8) * c2;
+                    ks[0] = e8m0_value(b & 255u);
+                    ks[1] = e8m0_value(b >> 8);
                 }
 #pragma unroll
                 for (int x = 0; x < MT; ++x)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        float v = s[x][n][k] * ks[k & 1];
+                        float v = s[x][n][k] * (QUANT ? ks[k & 1] * row_c2[x][k >> 1] : c2);
                         if (edge && key0 + 8 * n + 2 * t + (k & 1) >= limit[x][k >> 1]) v = -INFINITY;
                         s[x][n][k] = v;
                         mx[x][k >> 1] = fmaxf(mx[x][k >> 1], v);
@@ -422,8 +435,8 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
 #pragma unroll
                         for (int hl = 0; hl < 2; ++hl) {  // two column tiles from bytes 2 hl, 2 hl + 1 of either key
                             uint32_t b0[2], b1[2];
-                            widen<true>(__byte_perm(w[0][c], w[1][c], hl ? 0x7632 : 0x5410), b0[0], b0[1]);
-                            widen<true>(__byte_perm(w[2][c], w[3][c], hl ? 0x7632 : 0x5410), b1[0], b1[1]);
+                            e4m3_bits(__byte_perm(w[0][c], w[1][c], hl ? 0x7632 : 0x5410), b0[0], b0[1]);
+                            e4m3_bits(__byte_perm(w[2][c], w[3][c], hl ? 0x7632 : 0x5410), b1[0], b1[1]);
 #pragma unroll
                             for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -511,11 +524,11 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         out[k + 3] += v.w * f;
                     }
                 }
-                const int r = me.qt * G::ROWS + x * 16 + row, tok = by_group(a, r), head = me.h * a.group + (r - tok * a.group);
                 if (QUANT) {
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) out[k] *= kTiny;
                 }
+                const int r = me.qt * G::ROWS + x * 16 + row, tok = by_group(a, r), head = me.h * a.group + (r - tok * a.group);
                 if (bad != 0u && tok < me.ql) {
                     // keys of this piece whose groups were looked through, as far as my row sees them
                     const int keys = a.causal ? min(me.kv, me.kv - me.ql + tok + 1) : me.kv;
