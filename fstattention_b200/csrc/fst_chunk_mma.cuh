@@ -28,12 +28,12 @@ struct ChunkMmaGeo {
     static constexpr int REGS = 224, REGS_LOADS = 56;
     static_assert(256 * REGS + 128 * REGS_LOADS <= THREADS * 168, "the split draws on what the launch was given");
     static constexpr int TILE = KEYS * D * (QUANT ? 1 : 2);         // bytes of a tile of K or V: 64-column halves of KEYS rows, or rows of bytes
-    static constexpr int STAGES = QUANT && D == 64 ? 4 : 2;
+    static constexpr int STAGES = QUANT && D == 64 ? 8 : 4;         // of a tile of K or of V, which take turns
     static constexpr bool Q_SHARED = D == 128 && MT == 2;           // fragments of Q in shared memory: registers would not hold them
-    static constexpr int OFF_MERGE = STAGES * 2 * TILE;             // [warp][16 rows][D + 4] fp32
+    static constexpr int OFF_MERGE = STAGES * TILE;             // [warp][16 rows][D + 4] fp32
     static constexpr int OFF_STATS = OFF_MERGE + WARPS * 16 * (D + 4) * 4;      // [warp][ROWS] (exponent, sum)
-    static constexpr int OFF_SCALES = OFF_STATS + WARPS * ROWS * 8; // [stage] KEYS bytes of K, KEYS of V
-    static constexpr int OFF_Q = OFF_SCALES + (QUANT ? STAGES * 2 * KEYS : 0);  // [row tile][step][lane] 16 bytes
+    static constexpr int OFF_SCALES = OFF_STATS + WARPS * ROWS * 8; // [stage] KEYS bytes
+    static constexpr int OFF_Q = OFF_SCALES + (QUANT ? STAGES * KEYS : 0);  // [row tile][step][lane] 16 bytes
     static constexpr int OFF_BAR = OFF_Q + (Q_SHARED ? MT * D / 16 * 512 : 0);
     static constexpr int BYTES = OFF_BAR + 2 * STAGES * 8 + 1024;   // + alignment
 };
@@ -118,6 +118,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
         const int ps = 1 << a.c.page_shift;
         int st = 0, page = 0;
         uint32_t use = 0;
+        bool alive = true;
         auto look_up = [&]() {
             const int key = me.tile * G::KEYS + lane * ps;
             page = lane * ps < G::KEYS && key < me.keys ? __ldg(a.c.table + size_t(me.z) * a.c.width + (key >> a.c.page_shift)) : 0;
@@ -130,45 +131,44 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
             me.next(line);
             if (i + 1 < n_tiles) look_up();
             if (pages <= 0) continue;
-            if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(bar_empty + st * 8, (use - 1) & 1, a.status, blockIdx.x))) break;
             const bool bad = lane < pages && unsigned(here) >= unsigned(a.c.n_pages);            // the boxes then read as zeros
-            const uint32_t wrong = __ballot_sync(0xffffffffu, bad), bar = bar_full + st * 8, k_at = s_base + st * 2 * G::TILE, v_at = k_at + G::TILE;
-            unsigned char *scales = smem + G::OFF_SCALES + st * 2 * G::KEYS;
-            if (bad) {
-                report(a.status, FST_DEV_INDEX_RANGE, z, key0 + lane * ps);
-                if constexpr (QUANT) {
-                    for (int k = 0; k < ps; k += 16)
-                        *reinterpret_cast<uint4 *>(scales + lane * ps + k) = *reinterpret_cast<uint4 *>(scales + G::KEYS + lane * ps + k) = make_uint4(0, 0, 0, 0);
-                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                }
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive_expect_tx(bar, (pages << a.c.page_shift) * D * (QUANT ? 2 : 4) + (QUANT ? (pages - __popc(wrong)) * 2 * ps : 0));
-            __syncwarp();
+            const uint32_t wrong = __ballot_sync(0xffffffffu, bad);
+            if (bad) report(a.status, FST_DEV_INDEX_RANGE, z, key0 + lane * ps);
 #pragma unroll 1
-            for (int p = 0; p < pages; ++p) {
-                const int pg = __shfl_sync(0xffffffffu, here, p), row = p * ps;
-                if (umma::elect_one()) {
-                    if constexpr (QUANT) {
-                        tma_load_4d(k_at + row * D, &tm_k, 0, 0, h, pg, bar);
-                        tma_load_4d(v_at + row * D, &tm_v, 0, 0, h, pg, bar);
-                        if (!(wrong >> p & 1u)) {
-                            const size_t at = (size_t(pg) * a.H_kv + h) << a.c.page_shift;
-                            bulk_load(smem_u32(scales + row), a.c.k_scale + at, ps, bar);
-                            bulk_load(smem_u32(scales + G::KEYS + row), a.c.v_scale + at, ps, bar);
+            for (int v = 0; v < 2; ++v) {
+                if (use > 0 && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_empty + st * 8, (use - 1) & 1, a.status, blockIdx.x));
+                if (!alive) break;
+                const CUtensorMap *map = v ? &tm_v : &tm_k;
+                const uint32_t bar = bar_full + st * 8, to = s_base + st * G::TILE;
+                unsigned char *scales = smem + G::OFF_SCALES + st * G::KEYS;
+                if constexpr (QUANT) {
+                    if (bad) {
+                        for (int k = 0; k < ps; k += 16) *reinterpret_cast<uint4 *>(scales + lane * ps + k) = make_uint4(0, 0, 0, 0);
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    }
+                    __syncwarp();
+                }
+                if (lane == 0) mbar_arrive_expect_tx(bar, (pages << a.c.page_shift) * D * (QUANT ? 1 : 2) + (QUANT ? (pages - __popc(wrong)) * ps : 0));
+                __syncwarp();
+#pragma unroll 1
+                for (int p = 0; p < pages; ++p) {
+                    const int pg = __shfl_sync(0xffffffffu, here, p), row = p * ps;
+                    if (umma::elect_one()) {
+                        if constexpr (QUANT) {
+                            tma_load_4d(to + row * D, map, 0, 0, h, pg, bar);
+                            if (!(wrong >> p & 1u)) bulk_load(smem_u32(scales + row), (v ? a.c.v_scale : a.c.k_scale) + ((size_t(pg) * a.H_kv + h) << a.c.page_shift), ps, bar);
+                        } else {
+#pragma unroll
+                            for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(to + hf * HALF_BYTES + row * 128, map, hf * 64, 0, h, pg, bar);
                         }
-                    } else {
-#pragma unroll
-                        for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(k_at + hf * HALF_BYTES + row * 128, &tm_k, hf * 64, 0, h, pg, bar);
-#pragma unroll
-                        for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(v_at + hf * HALF_BYTES + row * 128, &tm_v, hf * 64, 0, h, pg, bar);
                     }
                 }
+                if (++st == G::STAGES) {
+                    st = 0;
+                    ++use;
+                }
             }
-            if (++st == G::STAGES) {
-                st = 0;
-                ++use;
-            }
+            if (!alive) break;
         }
         // nothing may land after the CTA has left, also when a wait ran out: the last fill of every stage
 #pragma unroll 1
@@ -286,9 +286,14 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
 
         const int key0 = group_of(me);
         if (me.keys > 0 && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_full + slot * 8, parity, a.status, blockIdx.x));
+        bool k_held = me.keys > 0;
+        auto done_with = [&](int stage) {
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar_empty + stage * 8) : "memory");
+        };
         if (key0 < me.keys && alive) {
-            const uint32_t k_at = s_base + slot * 2 * G::TILE + warp * SUBS * SUB_BYTES, v_at = k_at + G::TILE;      // my rows
-            const unsigned char *scales = smem + G::OFF_SCALES + slot * 2 * G::KEYS + warp * KW;
+            const uint32_t k_at = s_base + slot * G::TILE + warp * SUBS * SUB_BYTES, v_at = k_at + G::TILE;          // my rows
+            const unsigned char *scales = smem + G::OFF_SCALES + slot * G::KEYS + warp * KW;
             const bool edge = key0 + KW > lim_first;      // not every row attends to all of the group
             float s[MT][NK][4];
 #pragma unroll
@@ -341,6 +346,10 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     }
                 }
             }
+            if constexpr (!QUANT) {                       // (an 8-bit tile's scales are still to be read)
+                done_with(slot);
+                k_held = false;
+            }
             // ---- softmax of the group: scores in base-2 units against the row's running maximum
             uint32_t pf[MT][SUBS][4];
             float mx[MT][2];
@@ -363,6 +372,10 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         s[x][n][k] = v;
                         mx[x][k >> 1] = fmaxf(mx[x][k >> 1], v);
                     }
+            }
+            if constexpr (QUANT) {
+                done_with(slot);
+                k_held = false;
             }
 #pragma unroll
             for (int x = 0; x < MT; ++x) {
@@ -390,6 +403,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     l[x][1] *= alpha[1];
                 }
             }
+            alive = __all_sync(0xffffffffu, mbar_wait(bar_full + (slot + 1) * 8, parity, a.status, blockIdx.x));     // V
 #pragma unroll
             for (int n = 0; n < NK; ++n) {
                 float vs[2] = {1.f, 1.f};
@@ -462,10 +476,11 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                 }
             }
         }
-        if (me.keys > 0) {                                // done with the stage
-            __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar_empty + slot * 8) : "memory");
-            if (++slot == G::STAGES) {
+        if (me.keys > 0) {
+            if (k_held) done_with(slot);
+            done_with(slot + 1);
+            slot += 2;
+            if (slot == G::STAGES) {
                 slot = 0;
                 parity ^= 1u;
             }
