@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(256)
 chunk_combine_kernel(const ChunkArgs a, int n_ctas) {
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    constexpr int C = D / 32, RPW = ROWS >= 32 ? 4 : 2;   // columns of a lane, rows of a warp
+    constexpr int C = D / 32, RPW = ROWS >= 32 ? 4 : ROWS / 8;   // columns of a lane, rows of a warp
     const ChunkCut it = reinterpret_cast<const ChunkCut *>(a.part + chunk_cuts_at(n_ctas, ROWS, D))[blockIdx.x];
     const int row0 = (blockIdx.y * 8 + (threadIdx.x >> 5)) * RPW, lane = threadIdx.x & 31;
     if (it.pieces <= 1 || it.qt * ROWS + row0 >= it.ql * a.group) return;
@@ -415,15 +415,18 @@ chunk_combine_kernel(const ChunkArgs a, int n_ctas) {
 
 template <typename T, int D, int ROWS>
 cudaError_t launch_chunk_combine(const ChunkArgs &a, int n_ctas, cudaStream_t stream) {
-    constexpr int PER_BLOCK = 8 * (ROWS >= 32 ? 4 : 2);
+    constexpr int PER_BLOCK = 8 * (ROWS >= 32 ? 4 : ROWS / 8);
     return launch_serialised(chunk_combine_kernel<T, D, ROWS>, dim3(n_ctas, ROWS / PER_BLOCK), dim3(256), 0, stream, a, n_ctas);
 }
 
 // CTAs of a call's line: one per SM (a workspace holds two pieces for each).
 inline int chunk_ctas() { return sm_count(); }
-// Which kernel: up to 32 rows the mma.sync one.
+// Which kernel: up to 32 rows those on mma.sync.
 inline bool chunk_many_rows(const ChunkArgs &a) { return (long long)a.n_q * a.group > 32; }
-inline int chunk_row_tile(const ChunkArgs &a) { return chunk_many_rows(a) ? 256 : (long long)a.n_q * a.group <= 16 ? 16 : 32; }
+inline int chunk_row_tile(const ChunkArgs &a) {
+    const long long rows = (long long)a.n_q * a.group;
+    return chunk_many_rows(a) ? 256 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+}
 // An 8-bit cache under many queries is expanded once, ahead of the call, rather than by every row tile on its way: from two row tiles of
 // a K/V head on that is no slower (512 rows of 8 heads over 16384: 125 us on the way, 126 expanded; 8192 rows over 8192: 410 and
 // ...), but only as long as the copy of all that the tables can hold stays below 2 GB.

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "fst_chunk_mma.cuh"
+#include "fst_chunk_token.cuh"
 #include "fst_chunk_umma.cuh"
 
 namespace fst {
@@ -20,7 +21,9 @@ cudaError_t launch_chunk_t(const ChunkArgs &a, int n_ctas, cudaStream_t stream) 
         return a.c.k_scale != nullptr ? launch_chunk_umma<T, D, true>(b, tq, tk, tv, n_ctas, stream) : launch_chunk_umma<T, D, false>(b, tq, tk, tv, n_ctas, stream);
     }
     if (!make_pool_maps(&tk, &tv, a.c, bf16, D, a.H_kv, 1 << a.c.page_shift)) return cudaErrorNotSupported;
-    const bool one = a.n_q * a.group <= 16;
+    if (chunk_row_tile(a) == 8)
+        return a.c.k_scale != nullptr ? launch_chunk_token<T, D, true>(a, tk, tv, n_ctas, stream) : launch_chunk_token<T, D, false>(a, tk, tv, n_ctas, stream);
+    const bool one = chunk_row_tile(a) == 16;
     if (a.c.k_scale != nullptr)
         return one ? launch_chunk_mma<T, D, true, 1>(a, tk, tv, n_ctas, stream) : launch_chunk_mma<T, D, true, 2>(a, tk, tv, n_ctas, stream);
     return one ? launch_chunk_mma<T, D, false, 1>(a, tk, tv, n_ctas, stream) : launch_chunk_mma<T, D, false, 2>(a, tk, tv, n_ctas, stream);

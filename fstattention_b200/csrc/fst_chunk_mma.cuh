@@ -15,9 +15,7 @@
 // of their own, 108 us, but 47 instead of 41 with 28 rows a tile; as it is ...)
 #pragma once
 
-#include "fst_chunk.cuh"
-#include "fst_chunk_map.cuh"
-#include "fst_umma.cuh"
+#include "fst_chunk_load.cuh"
 
 namespace fst {
 
@@ -46,29 +44,6 @@ __device__ __forceinline__ void e4m3_bits(uint32_t w, uint32_t &even, uint32_t &
     const uint32_t u = w << 8;
     even = (u & 0x80008000u) | ((u >> 4) & 0x07f007f0u);
 }
-// two e4m3 bytes (the low ones, the high ones) -> a pair of fp16
-__device__ __forceinline__ uint32_t e4m3_halves(uint32_t w, bool high) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(r) : "h"(uint16_t(high ? w >> 16 : w)));
-    return r;
-}
-
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-    uint2 v;
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-    return v;
-}
-// `bytes` (a multiple of 16) contiguous bytes of global memory into shared memory
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, int bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-
 template <typename T, int D, bool QUANT, int MT>
 __global__ void __launch_bounds__(384, 1)
 chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
@@ -113,69 +88,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
     if (warp >= G::WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(G::REGS_LOADS));
         if (warp > G::WARPS) return;
-        // ====== loads: a box per page and 64 columns, by one lane; the page numbers are looked up a tile ahead ======
-        // (While each warp fetched its own 16 rows, asking for them took it as long as computing with them.)
-        const int ps = 1 << a.c.page_shift;
-        int st = 0, page = 0;
-        uint32_t use = 0;
-        bool alive = true;
-        auto look_up = [&]() {
-            const int key = me.tile * G::KEYS + lane * ps;
-            page = lane * ps < G::KEYS && key < me.keys ? __ldg(a.c.table + size_t(me.z) * a.c.width + (key >> a.c.page_shift)) : 0;
-        };
-        look_up();
-#pragma unroll 1
-        for (int i = 0; i < n_tiles; ++i) {
-            const int here = page, key0 = me.tile * G::KEYS, h = me.h, z = me.z;
-            const int pages = (min(G::KEYS, me.keys - key0) + ps - 1) >> a.c.page_shift;         // 0: an item that sees nothing
-            me.next(line);
-            if (i + 1 < n_tiles) look_up();
-            if (pages <= 0) continue;
-            const bool bad = lane < pages && unsigned(here) >= unsigned(a.c.n_pages);            // the boxes then read as zeros
-            const uint32_t wrong = __ballot_sync(0xffffffffu, bad);
-            if (bad) report(a.status, FST_DEV_INDEX_RANGE, z, key0 + lane * ps);
-#pragma unroll 1
-            for (int v = 0; v < 2; ++v) {
-                if (use > 0 && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_empty + st * 8, (use - 1) & 1, a.status, blockIdx.x));
-                if (!alive) break;
-                const CUtensorMap *map = v ? &tm_v : &tm_k;
-                const uint32_t bar = bar_full + st * 8, to = s_base + st * G::TILE;
-                unsigned char *scales = smem + G::OFF_SCALES + st * G::KEYS;
-                if constexpr (QUANT) {
-                    if (bad) {
-                        for (int k = 0; k < ps; k += 16) *reinterpret_cast<uint4 *>(scales + lane * ps + k) = make_uint4(0, 0, 0, 0);
-                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                    }
-                    __syncwarp();
-                }
-                if (lane == 0) mbar_arrive_expect_tx(bar, (pages << a.c.page_shift) * D * (QUANT ? 1 : 2) + (QUANT ? (pages - __popc(wrong)) * ps : 0));
-                __syncwarp();
-#pragma unroll 1
-                for (int p = 0; p < pages; ++p) {
-                    const int pg = __shfl_sync(0xffffffffu, here, p), row = p * ps;
-                    if (umma::elect_one()) {
-                        if constexpr (QUANT) {
-                            tma_load_4d(to + row * D, map, 0, 0, h, pg, bar);
-                            if (!(wrong >> p & 1u)) bulk_load(smem_u32(scales + row), (v ? a.c.v_scale : a.c.k_scale) + ((size_t(pg) * a.H_kv + h) << a.c.page_shift), ps, bar);
-                        } else {
-#pragma unroll
-                            for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(to + hf * HALF_BYTES + row * 128, map, hf * 64, 0, h, pg, bar);
-                        }
-                    }
-                }
-                if (++st == G::STAGES) {
-                    st = 0;
-                    ++use;
-                }
-            }
-            if (!alive) break;
-        }
-        // nothing may land after the CTA has left, also when a wait ran out: the last fill of every stage
-#pragma unroll 1
-        for (int s = 0; s < G::STAGES; ++s) {
-            const uint32_t fills = use + (s < st ? 1u : 0u);
-            if (fills > 0) mbar_wait(bar_full + s * 8, (fills - 1) & 1, a.status, blockIdx.x);
-        }
+        load_tiles<G, D, QUANT>(a, line, me, n_tiles, tm_k, tm_v, s_base, smem, bar_full, bar_empty);
         return;
     }
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(G::REGS));

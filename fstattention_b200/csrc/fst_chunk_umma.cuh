@@ -19,7 +19,7 @@
 
 #include "fst_chunk.cuh"
 #include "fst_chunk_map.cuh"
-#include "fst_chunk_mma.cuh"
+#include "fst_chunk_load.cuh"
 #include "fst_umma.cuh"
 
 namespace fst {
