@@ -9,10 +9,10 @@
 // agree, so lane (g, t) of a K fragment takes the contiguous bytes D/4 t .. of key g, and Q is loaded in the same order; of V it
 // takes bytes D/8 g .. of its four keys, which only permutes the columns of the result.  K is fp16, by the conversion instruction, and a
 // key's scale multiplies its score.  bf16 queries become fp16 times a power of two per row, with the row's largest value next to 2^15:
-// what fp16 loses then is 2^-39 of that.  V is bf16, as a row's scale goes into its probability and needs the range: a byte's seven
-// low bits moved under bf16's exponent are its value * 2^-120, half of which comes back with the scale and half at the end.
-// (Two sequences of 115000 rows: K by its bits as well 118 us; V as fp16 by the instruction, the scales in the exponents of weights
-// of their own, 108 us, but 47 instead of 41 with 28 rows a tile; as it is ...)
+// what fp16 loses then is 2^-39 of that.  Under bf16 queries V is bf16 too, as a row's scale goes into its probability and needs the range: a
+// byte's seven low bits moved under bf16's exponent are its value * 2^-120, half of which comes back with the scale and half at the
+// end.  Under fp16 queries, whose results have three more bits, V is fp16 and the scales go into the exponents of weights of their
+// own (WEIGHTS), as in chunk_token_kernel.
 #pragma once
 
 #include "fst_chunk_load.cuh"
@@ -50,10 +50,10 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
     using G = ChunkMmaGeo<D, QUANT, MT>;
     using MT_ = MmaTraits<T>;
     using MK = MmaTraits<typename std::conditional<QUANT, __half, T>::type>;     // of the first product, of the second
-    using MP = MmaTraits<typename std::conditional<QUANT, __nv_bfloat16, T>::type>;
+    using MP = MmaTraits<T>;
     using Line = ChunkLine<G::ROWS, G::KEYS, G::OVER>;
     using Cursor = ChunkCursor<G::ROWS, G::KEYS, G::OVER>;
-    constexpr bool BF16 = !std::is_same<T, __half>::value;
+    constexpr bool BF16 = !std::is_same<T, __half>::value, WEIGHTS = QUANT && !BF16;
     constexpr int KS = D / 16, ND = D / 8;               // steps of the first product, column tiles of the second
     constexpr int KW = G::KW, NK = KW / 8, SUBS = KW / 16;
     constexpr int HALF_BYTES = G::KEYS * 128, SUB_BYTES = 16 * (QUANT ? D : 128);         // a tile's half of 64 columns of 16 bits, 16 rows in it
@@ -111,6 +111,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
     };
     float acc[MT][ND][4], m[MT][2], l[MT][2];
     float row_c2[QUANT ? MT : 1][2];                      // an 8-bit cache: c2 over the row's factor
+    float m_w[WEIGHTS ? MT : 1][2];                       // running maximum of score and V's exponent
     int limit[MT][2], lim_first = 0, slot = 0;
     uint32_t parity = 0;
     bool poisoned = false, alive = true;                  // a V that is not finite was met where not every row attends to it
@@ -134,6 +135,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     const T *src = static_cast<const T *>(a.q) + me.z * a.qs_z + (me.h * a.group + (r - tok * a.group)) * a.qs_h + tok * a.qs_n;
                     // two of the four registers of a row tile's fragments: the row's part of two steps in an 8-bit cache's order, or of one
                     float by = 1.f;                       // the row's factor
+                    if constexpr (WEIGHTS) m_w[x][hh] = -INFINITY;
                     if constexpr (QUANT) {
                         if constexpr (BF16) {
                             uint32_t top = 0;
@@ -290,37 +292,57 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                 done_with(slot);
                 k_held = false;
             }
+            alive = __all_sync(0xffffffffu, mbar_wait(bar_full + (slot + 1) * 8, parity, a.status, blockIdx.x));     // V
+            float mw[WEIGHTS ? MT : 1][2], e_v[WEIGHTS ? NK : 1][2];
+            if constexpr (WEIGHTS) {
+#pragma unroll
+                for (int x = 0; x < MT; ++x) mw[x][0] = mw[x][1] = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < NK; ++n) {
+                    const int b = *reinterpret_cast<const uint16_t *>(scales + G::KEYS + 8 * n + 2 * t);
+                    e_v[n][0] = (b & 255) == 255 ? NAN : float((b & 255) - 127);
+                    e_v[n][1] = b >> 8 == 255 ? NAN : float((b >> 8) - 127);
+#pragma unroll
+                    for (int x = 0; x < MT; ++x)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mw[x][k >> 1] = fmaxf(mw[x][k >> 1], s[x][n][k] + e_v[n][k & 1]);        // (a maximum passes over a NaN)
+                }
+            }
 #pragma unroll
             for (int x = 0; x < MT; ++x) {
                 bool up = false;
-                float alpha[2];
+                float alpha[2], alpha_w[2];
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
-                    mx[x][hh] = fmaxf(mx[x][hh], __shfl_xor_sync(0xffffffffu, mx[x][hh], 1));
-                    mx[x][hh] = fmaxf(mx[x][hh], __shfl_xor_sync(0xffffffffu, mx[x][hh], 2));
-                    const float now = fmaxf(m[x][hh], mx[x][hh]);
-                    up = up || now > m[x][hh];
-                    alpha[hh] = now == -INFINITY ? 1.f : fast_exp2(m[x][hh] - now);
-                    m[x][hh] = now;
-                    mx[x][hh] = now == -INFINITY ? 0.f : now;
+                    auto move = [&](float &had, float &seen, float &by) {    // the running maximum, as a reference, and what it takes what was summed by
+                        seen = fmaxf(seen, __shfl_xor_sync(0xffffffffu, seen, 1));
+                        seen = fmaxf(seen, __shfl_xor_sync(0xffffffffu, seen, 2));
+                        const float now = fmaxf(had, seen);
+                        up = up || now > had;
+                        by = now == -INFINITY ? 1.f : fast_exp2(had - now);
+                        had = now;
+                        seen = now == -INFINITY ? 0.f : now;
+                    };
+                    move(m[x][hh], mx[x][hh], alpha[hh]);
+                    alpha_w[hh] = alpha[hh];
+                    if constexpr (WEIGHTS) move(m_w[x][hh], mw[x][hh], alpha_w[hh]);
                 }
                 if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
                     for (int n = 0; n < ND; ++n) {
-                        acc[x][n][0] *= alpha[0];
-                        acc[x][n][1] *= alpha[0];
-                        acc[x][n][2] *= alpha[1];
-                        acc[x][n][3] *= alpha[1];
+                        acc[x][n][0] *= alpha_w[0];
+                        acc[x][n][1] *= alpha_w[0];
+                        acc[x][n][2] *= alpha_w[1];
+                        acc[x][n][3] *= alpha_w[1];
                     }
                     l[x][0] *= alpha[0];
                     l[x][1] *= alpha[1];
                 }
             }
-            alive = __all_sync(0xffffffffu, mbar_wait(bar_full + (slot + 1) * 8, parity, a.status, blockIdx.x));     // V
 #pragma unroll
             for (int n = 0; n < NK; ++n) {
                 float vs[2] = {1.f, 1.f};
-                if constexpr (QUANT) {
+                if constexpr (QUANT && !WEIGHTS) {
                     const uint32_t b = *reinterpret_cast<const uint16_t *>(scales + G::KEYS + 8 * n + 2 * t);
                     vs[0] = e8m0_value(b & 255u) * kTiny;
                     vs[1] = e8m0_value(b >> 8) * kTiny;
@@ -330,10 +352,12 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     float p[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        p[k] = fast_exp2(s[x][n][k] - mx[x][k >> 1]);
+                        const float v = s[x][n][k];
+                        p[k] = fast_exp2(v - mx[x][k >> 1]);
                         l[x][k >> 1] += p[k];
                         // the row's scale; what a masked key holds, NaN too, stays out
-                        if constexpr (QUANT) p[k] = s[x][n][k] == -INFINITY ? 0.f : p[k] * vs[k & 1];
+                        if constexpr (WEIGHTS) p[k] = v == -INFINITY ? 0.f : fast_exp2(v + e_v[n][k & 1] - mw[x][k >> 1]);
+                        else if constexpr (QUANT) p[k] = v == -INFINITY ? 0.f : p[k] * vs[k & 1];
                     }
                     pf[x][n >> 1][(n & 1) * 2] = MP::pack(p[0], p[1]);
                     pf[x][n >> 1][(n & 1) * 2 + 1] = MP::pack(p[2], p[3]);
@@ -356,14 +380,26 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                             const uint2 b = lds64(v_at + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8);
                             w[k][0] = b.x; w[k][1] = b.y;
                         }
+                        if (WEIGHTS && edge && row >= here) {                    // zero times a NaN byte would be NaN
+#pragma unroll
+                            for (int c = 0; c < D / 32; ++c) w[k][c] = 0u;
+                        }
                     }
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c)
 #pragma unroll
                         for (int hl = 0; hl < 2; ++hl) {  // two column tiles from bytes 2 hl, 2 hl + 1 of either key
                             uint32_t b0[2], b1[2];
-                            e4m3_bits(__byte_perm(w[0][c], w[1][c], hl ? 0x7632 : 0x5410), b0[0], b0[1]);
-                            e4m3_bits(__byte_perm(w[2][c], w[3][c], hl ? 0x7632 : 0x5410), b1[0], b1[1]);
+                            if constexpr (WEIGHTS) {
+                                const uint32_t y0 = __byte_perm(w[0][c], w[1][c], hl ? 0x7362 : 0x5140), y1 = __byte_perm(w[2][c], w[3][c], hl ? 0x7362 : 0x5140);
+                                b0[0] = e4m3_halves(y0, false);
+                                b0[1] = e4m3_halves(y0, true);
+                                b1[0] = e4m3_halves(y1, false);
+                                b1[1] = e4m3_halves(y1, true);
+                            } else {
+                                e4m3_bits(__byte_perm(w[0][c], w[1][c], hl ? 0x7632 : 0x5410), b0[0], b0[1]);
+                                e4m3_bits(__byte_perm(w[2][c], w[3][c], hl ? 0x7632 : 0x5410), b1[0], b1[1]);
+                            }
 #pragma unroll
                             for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -416,6 +452,13 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                     if (t == 0) stats[warp * G::ROWS + x * 16 + hh * 8 + g] = make_float2(m[x][hh], sum);
                     float *to = rows + (warp * 16 + hh * 8 + g) * (D + 4);
+                    if constexpr (WEIGHTS) {              // weights back to the probabilities' reference
+                        const float by = m[x][hh] == -INFINITY ? 1.f : fast_exp2(m_w[x][hh] - m[x][hh]);
+#pragma unroll
+                        for (int j = 0; j < ND; ++j)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) acc[x][j][2 * hh + k] *= by;
+                    }
                     if constexpr (QUANT) {
 #pragma unroll
                         for (int j = 0; j < ND; j += 4)
@@ -452,7 +495,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         out[k + 3] += v.w * f;
                     }
                 }
-                if (QUANT) {
+                if (QUANT && !WEIGHTS) {
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) out[k] *= kTiny;
                 }
