@@ -63,7 +63,7 @@ static int cuda_status(cudaError_t e) {
 // a cache's fields, once they are found to be what the kernels can take
 static int open_cache(CacheArgs &c, const fst_paged_cache *cache, int head_dim, int dtype) {
     if (!cache || !cache->k_pool || !cache->v_pool || !cache->block_table || cache->table_stride <= 0 || cache->n_pages <= 0 ||
-        !cache->k_scale != !cache->v_scale)
+        !cache->k_scale != !cache->v_scale || cache->stride_page <= 0 || cache->stride_row <= 0 || cache->stride_head <= 0)
         return FST_ERR_INVALID_ARG;
     if ((head_dim != 64 && head_dim != 128) || (dtype != FST_F16 && dtype != FST_BF16)) return FST_ERR_UNSUPPORTED;
     const int ps = cache->page_size;

@@ -251,6 +251,11 @@ struct ChunkCut {
     int pad[3];
 };
 
+// Probabilities that are rounded to fp16 for the second product are taken 2^15 times too large (against a reference that is 15 below
+// the maximum), so that they fill its range: at most 2^15, and what lies 2^24 below that is lost.  At most 1 they would lose
+// what lies 2^24 below the largest one, which many keys together can make the larger part of the result.
+constexpr float kLift = 15.f;
+
 // ---- values that are not finite where not every row of a tile attends to them.  The second product multiplies a masked
 // key's V by a probability of zero, and zero times NaN or infinity is NaN.  In key groups that some row does not see, such elements
 // are taken out of V, and what they do to the rows that see them is added at the end: a kernel that met none never looks again.

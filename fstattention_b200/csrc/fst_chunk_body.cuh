@@ -15,7 +15,7 @@ cudaError_t launch_chunk_t(const ChunkArgs &a, int n_ctas, cudaStream_t stream) 
         if (!make_pool_maps(&tk, &tv, a.c, bf16, D, a.H_kv, 1 << a.c.page_shift)) return cudaErrorNotSupported;
         ChunkArgs b = a;
         alignas(64) CUtensorMap tq = tk;
-        b.q_boxes = 128 % a.group == 0;
+        b.q_boxes = 128 % a.group == 0 && a.qs_z > 0 && a.qs_h > 0 && a.qs_n > 0;       // (broadcast queries: by plain loads)
         if (b.q_boxes && !make_pool_map(&tq, PoolKey{a.q, a.qs_z, a.qs_h, a.qs_n, bf16 ? POOL_BF16 : POOL_F16, D, a.H, a.n_q, a.Z, a.group, 128 / a.group}))
             return cudaErrorNotSupported;
         return a.c.k_scale != nullptr ? launch_chunk_umma<T, D, true>(b, tq, tk, tv, n_ctas, stream) : launch_chunk_umma<T, D, false>(b, tq, tk, tv, n_ctas, stream);

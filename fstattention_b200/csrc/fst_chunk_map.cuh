@@ -1,4 +1,5 @@
-// Tensor maps over a page pool for the chunk kernels, kept per host thread like those of make_map.
+// Tensor maps over a page pool for the chunk kernels, encoded by every call: a table of them by address, as make_map has, gained nothing that
+// could be measured (5.3 us of host time for a small call either way).
 #pragma once
 
 #include "fst_attention_tma.cuh"
@@ -12,34 +13,12 @@ struct PoolKey {
     const void *base;
     int64_t stride_page, stride_row, stride_head;
     int32_t type, D, page, H, n_pages, box_rows, box_heads;
-    bool operator==(const PoolKey &o) const {
-        return base == o.base && stride_page == o.stride_page && stride_row == o.stride_row && stride_head == o.stride_head &&
-               type == o.type && D == o.D && page == o.page && H == o.H && n_pages == o.n_pages && box_rows == o.box_rows && box_heads == o.box_heads;
-    }
 };
 
 // Rank 4: columns, rows of a page, K/V heads, pages; boxes of 64 columns of 16 bits, or a whole row of e4m3, by box_rows rows by
 // box_heads heads.
 // 128 bytes of a row are swizzled over 128 bytes, the 64 bytes of an e4m3 row at D 64 over 64.
 inline bool make_pool_map(CUtensorMap *map, const PoolKey &key) {
-    struct Slot {
-        alignas(64) CUtensorMap map;
-        PoolKey key;
-        bool used = false;
-    };
-    constexpr int kSlots = 256;
-    static thread_local std::unique_ptr<Slot[]> table(new (std::nothrow) Slot[kSlots]);
-    Slot *slot = nullptr;
-    if (table) {
-        uint64_t h = reinterpret_cast<uintptr_t>(key.base) >> 4;
-        h = (h ^ (h >> 17) ^ uint64_t(key.n_pages) * 0x9E3779B97F4A7C15ull ^ uint64_t(key.stride_page) * 0xC2B2AE3D27D4EB4Full ^
-             uint64_t(key.box_rows) << 7) * 0xFF51AFD7ED558CCDull;
-        slot = &table[(h >> 40) % kSlots];
-        if (slot->used && slot->key == key) {
-            *map = slot->map;
-            return true;
-        }
-    }
     EncodeTiledFn fn = encode_tiled_fn();
     if (fn == nullptr) return false;
     const bool bytes = key.type == POOL_E4M3;
@@ -50,16 +29,9 @@ inline bool make_pool_map(CUtensorMap *map, const PoolKey &key) {
     const cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUtensorMapDataType type = bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                            : key.type == POOL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    if (fn(map, type, 4, const_cast<void *>(key.base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           bytes && key.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-        return false;
-    if (slot != nullptr) {
-        slot->map = *map;
-        slot->key = key;
-        slot->used = true;
-    }
-    return true;
+    return fn(map, type, 4, const_cast<void *>(key.base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              bytes && key.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // K's and V's maps of a cache (e4m3 where it has scales, else 16 bits as `bf16` says)

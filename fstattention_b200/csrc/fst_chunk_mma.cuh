@@ -54,6 +54,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
     using Line = ChunkLine<G::ROWS, G::KEYS, G::OVER>;
     using Cursor = ChunkCursor<G::ROWS, G::KEYS, G::OVER>;
     constexpr bool BF16 = !std::is_same<T, __half>::value, WEIGHTS = QUANT && !BF16;
+    constexpr float LIFT = !QUANT && !BF16 ? kLift : 0.f;
     constexpr int KS = D / 16, ND = D / 8;               // steps of the first product, column tiles of the second
     constexpr int KW = G::KW, NK = KW / 8, SUBS = KW / 16;
     constexpr int HALF_BYTES = G::KEYS * 128, SUB_BYTES = 16 * (QUANT ? D : 128);         // a tile's half of 64 columns of 16 bits, 16 rows in it
@@ -314,18 +315,18 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                 float alpha[2], alpha_w[2];
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
-                    auto move = [&](float &had, float &seen, float &by) {    // the running maximum, as a reference, and what it takes what was summed by
+                    auto move = [&](float &had, float &seen, float &by, float lift) {    // the running maximum, as a reference, and what it takes what was summed by
                         seen = fmaxf(seen, __shfl_xor_sync(0xffffffffu, seen, 1));
                         seen = fmaxf(seen, __shfl_xor_sync(0xffffffffu, seen, 2));
                         const float now = fmaxf(had, seen);
                         up = up || now > had;
                         by = now == -INFINITY ? 1.f : fast_exp2(had - now);
                         had = now;
-                        seen = now == -INFINITY ? 0.f : now;
+                        seen = now == -INFINITY ? 0.f : now - lift;
                     };
-                    move(m[x][hh], mx[x][hh], alpha[hh]);
+                    move(m[x][hh], mx[x][hh], alpha[hh], LIFT);
                     alpha_w[hh] = alpha[hh];
-                    if constexpr (WEIGHTS) move(m_w[x][hh], mw[x][hh], alpha_w[hh]);
+                    if constexpr (WEIGHTS) move(m_w[x][hh], mw[x][hh], alpha_w[hh], kLift);
                 }
                 if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -450,10 +451,10 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     float sum = l[x][hh];
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                    if (t == 0) stats[warp * G::ROWS + x * 16 + hh * 8 + g] = make_float2(m[x][hh], sum);
+                    if (t == 0) stats[warp * G::ROWS + x * 16 + hh * 8 + g] = make_float2(m[x][hh] - LIFT, sum);
                     float *to = rows + (warp * 16 + hh * 8 + g) * (D + 4);
                     if constexpr (WEIGHTS) {              // weights back to the probabilities' reference
-                        const float by = m[x][hh] == -INFINITY ? 1.f : fast_exp2(m_w[x][hh] - m[x][hh]);
+                        const float by = m[x][hh] == -INFINITY ? 1.f : fast_exp2(m_w[x][hh] - kLift - m[x][hh]);
 #pragma unroll
                         for (int j = 0; j < ND; ++j)
 #pragma unroll

@@ -7,7 +7,7 @@
 //
 // An 8-bit cache: K and V are fp16 fragments by the conversion instruction, without their scales.  A key's scale multiplies its score.  A value's
 // scale 2^e goes into the exponent of its weight: beside p = 2^(s - m), which the sum l is made of, there is w = 2^(s + e - m'), m' the
-// maximum of s + e, which multiplies V; both are at most 1, whatever the scales are, and the result is sum w v / l * 2^(m' - m).
+// maximum of s + e, which multiplies V; neither leaves its format, whatever the scales are, and the result is sum w v / l * 2^(m' - m).
 // bf16 queries become fp16 as in chunk_mma_kernel.
 //
 // Two sequences of 115000 e4m3 rows under 8 rows: chunk_mma_kernel 108 us, this ...
@@ -45,6 +45,7 @@ chunk_token_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, 
     using Line = ChunkLine<G::ROWS, G::KEYS, G::OVER>;
     using Cursor = ChunkCursor<G::ROWS, G::KEYS, G::OVER>;
     constexpr bool BF16 = !std::is_same<T, __half>::value;
+    constexpr float LIFT = !QUANT && !BF16 ? kLift : 0.f;
     constexpr int KS = D / 16, NP = D / 16;               // steps of the first product, 16-column tiles of the second
     constexpr int KW = G::KW, SUBS = KW / 16;
     constexpr int HALF_BYTES = G::KEYS * 128, SUB_BYTES = 16 * (QUANT ? D : 128);
@@ -233,18 +234,18 @@ chunk_token_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, 
             float alpha[2], alpha_w[2];
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                auto move = [&](float &had, float &seen, float &by) {        // the running maximum, as a reference, and what it takes what was summed by
+                auto move = [&](float &had, float &seen, float &by, float lift) {        // the running maximum, as a reference, and what it takes what was summed by
 #pragma unroll
                     for (int x = 4; x < 32; x *= 2) seen = fmaxf(seen, __shfl_xor_sync(0xffffffffu, seen, x));
                     const float now = fmaxf(had, seen);
                     up = up || now > had;
                     by = now == -INFINITY ? 1.f : fast_exp2(had - now);
                     had = now;
-                    seen = now == -INFINITY ? 0.f : now;
+                    seen = now == -INFINITY ? 0.f : now - lift;
                 };
-                move(m[q], mx[q], alpha[q]);
+                move(m[q], mx[q], alpha[q], LIFT);
                 alpha_w[q] = alpha[q];
-                if constexpr (QUANT) move(m_w[q], mw[q], alpha_w[q]);
+                if constexpr (QUANT) move(m_w[q], mw[q], alpha_w[q], kLift);
             }
             if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -340,10 +341,10 @@ chunk_token_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, 
                 float sum = l[q];
 #pragma unroll
                 for (int x = 4; x < 32; x *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-                if (g == 0) stats[warp * 8 + 2 * t + q] = make_float2(m[q], sum);
+                if (g == 0) stats[warp * 8 + 2 * t + q] = make_float2(m[q] - LIFT, sum);
                 float *to = rows + (warp * 8 + 2 * t + q) * (D + 4);
                 if constexpr (QUANT) {
-                    const float by = m[q] == -INFINITY ? 1.f : fast_exp2(m_w[q] - m[q]);          // weights back to the probabilities' reference
+                    const float by = m[q] == -INFINITY ? 1.f : fast_exp2(m_w[q] - kLift - m[q]);          // weights back to the probabilities' reference
 #pragma unroll
                     for (int n = 0; n < NP; n += 2)
                         *reinterpret_cast<float4 *>(to + g * (D / 8) + 2 * n) = make_float4(acc[n][q] * by, acc[n][2 + q] * by, acc[n + 1][q] * by, acc[n + 1][2 + q] * by);

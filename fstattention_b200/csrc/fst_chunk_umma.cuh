@@ -547,6 +547,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
         const uint32_t tmem_s = tmem + g * 128 + lanes, tmem_o = tmem + 256 + g * D + lanes, tmem_p = D == 128 ? tmem_s : tmem + 384 + g * 64 + lanes;
         const uint32_t my_s = bar_s + g * 8, my_p = bar_p + g * 16;
         const float c2 = a.scale_log2;
+        constexpr float LIFT = BF16 ? 0.f : kLift - 8.f;  // (a reference may be passed by 2^8, see below)
         uint32_t s_ph = 0, o_ph = 0;
         int item = 0, len;
         bool alive = true;
@@ -607,7 +608,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                 }
 #pragma unroll 1
                 for (int again = 0;; ++again) {
-                    const float mu = m_ref == -INFINITY ? 0.f : m_ref * c2;
+                    const float mu = m_ref == -INFINITY ? 0.f : m_ref * c2 - LIFT;
                     shift2 = pair(-mu, -mu);
                     float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
                     l2[0] = l2[1] = 0;
@@ -669,7 +670,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
             const bool bad = mine > 0 && *note <= item;   // (then also for the items behind: a look in vain)
             const bool whole = len == me.tiles, there = tok < me.ql;
             const int look_from = max(max(first_limit(), 0) & ~(G::KEYS - 1), me.tile * G::KEYS), look_to = min(limit, (me.tile + len) * G::KEYS);
-            const float f = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l, mu = m_ref == -INFINITY ? -INFINITY : m_ref * c2;
+            const float f = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l, mu = m_ref == -INFINITY ? -INFINITY : m_ref * c2 - LIFT;
             const int head = me.h * a.group + (row - tok * a.group);
             const size_t slot = (size_t(2) * blockIdx.x + (me.tile == 0 ? 1 : 0)) * G::ROWS + g * 128 + r;
             // The rows leave through shared memory, four whole lines of 128 bytes a store: by 16 or 32 bytes of 32 rows at a time a piece took

@@ -330,10 +330,12 @@ int fst_attention_fwd_paged(const void *q, const void *k_tree, const void *v_tre
  * r % page_size; element (page, row, head, d) of a pool at page * stride_page + row * stride_row + head * stride_head + d
  * (strides in elements, the same for both pools).  page_size is 16, 32, 64 or 128, head_dim 64 or 128.
  *
+ * The strides are positive, those of dimensions of one too.
  * With k_scale and v_scale NULL the pools hold 16-bit rows (fp16 or bf16, as the call's dtype says; strides multiples of
  * 8).  Otherwise they hold e4m3 bytes (strides multiples of 16) and the scales, contiguous
  * [n_pages][H_kv][page_size] bytes, a biased exponent b (e8m0) for every row and head: the row stands for e4m3 * 2^(b - 127),
- * for NaN where b is 255.
+ * for NaN where b is 255; the bytes are finite (0x7f and 0xff, e4m3's NaN, are what fst_cache_append never writes: read
+ * as NaN, their effect on the attention of rows that see them is not defined).
  * All addresses are device pointers on 16-byte boundaries (block_table: 4).  The struct itself is read during the call.
  */
 typedef struct fst_paged_cache {
@@ -377,11 +379,12 @@ int fst_cache_read(const fst_paged_cache *cache, void *k, void *v, const int32_t
  * q_lens[z] positions: query i attends to rows [0, kv_lens[z] - q_lens[z] + i], or with causal = 0 to all kv_lens[z] rows.
  * A query that sees no row gets zeros (lse -inf).  Rows i >= q_lens[z] of o and lse are left as they are.  What the
  * cache holds at rows that a query does not attend to, NaN and infinities included, does not reach it.
+ * Over an 8-bit cache fp16 queries take rows as fp16 where n_q H / H_kv > 32: values past 65504 saturate.
  * lse, when not NULL, is [Z][H][n_q], base-2 log-sum-exp of the scaled scores.  sm_scale must be positive and finite.
  * workspace: fst_attention_chunk_workspace_bytes() bytes (for the current device), 256-byte aligned, scratch of this call
  * alone; what is in it before does not matter.  May be NULL where that is 0.
- * A length that is negative or past the table (or n_q) is cut and sets FST_DEV_INDEX_RANGE, a page number outside
- * [0, n_pages) reads as zeros and does the same.
+ * A length that is negative or past the table (or n_q) is cut and sets FST_DEV_INDEX_RANGE (that of a sequence that has
+ * no queries after the cut may go unreported); a page number outside [0, n_pages) reads as zeros and sets it too.
  */
 size_t fst_attention_chunk_workspace_bytes(const fst_paged_cache *cache, int Z, int H, int H_kv, int n_q, int head_dim);
 int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cache *cache, const int32_t *kv_lens,
