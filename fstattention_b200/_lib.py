@@ -85,15 +85,14 @@ def _declare(lib):
     lib.fst_attention_fwd_ref.argtypes = ([_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i]
                                           + _TENSOR_STRIDES
                                           + [_i, _i, _f, _i, _i, _p, _sz, _p, _p])
-    cache = C.POINTER(PagedCache)
     lib.fst_cache_append.restype = _i
-    lib.fst_cache_append.argtypes = [cache, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i] + [_i64] * 6 + [_i, _p, _p]
+    lib.fst_cache_append.argtypes = [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i] + [_i64] * 6 + [_i, _p, _p]
     lib.fst_cache_read.restype = _i
-    lib.fst_cache_read.argtypes = [cache, _p, _p, _p, _i, _i, _i, _i] + [_i64] * 6 + [_i, _p, _p]
+    lib.fst_cache_read.argtypes = [_p, _p, _p, _p, _i, _i, _i, _i] + [_i64] * 6 + [_i, _p, _p]
     lib.fst_attention_chunk_workspace_bytes.restype = _sz
-    lib.fst_attention_chunk_workspace_bytes.argtypes = [cache, _i, _i, _i, _i, _i]
+    lib.fst_attention_chunk_workspace_bytes.argtypes = [_p, _i, _i, _i, _i, _i]
     lib.fst_attention_chunk.restype = _i
-    lib.fst_attention_chunk.argtypes = [_p, _p, _p, cache, _p, _p, _i, _i, _i, _i, _i] + [_i64] * 6 + [_f, _i, _i, _p, _sz, _p, _p]
+    lib.fst_attention_chunk.argtypes = [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i] + [_i64] * 6 + [_f, _i, _i, _p, _sz, _p, _p]
     lib.fst_attention_fwd_ref_static.restype = _i
     lib.fst_attention_fwd_ref_static.argtypes = ([_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i]
                                                  + _TENSOR_STRIDES + [_i, _i, _f, _i, _i, _p, _p])
