@@ -312,8 +312,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
             bool alive = true;
             uint32_t before = 0, now = 0;                 // the plan's words of the tile before and of this one
             // O += P V of the tile before, without a branch among the products where all of its 128 keys count
-            auto second_product = [&](auto gc) {
-                constexpr int g = decltype(gc)::value;
+            auto second_product = [&](int g) {
                 const uint32_t tmem_o = tmem + 256 + g * D, tmem_p = D == 128 ? tmem + g * 128 : tmem + 384 + g * 64;
                 const uint64_t dvs = dv + uint64_t(v_st * (TILE >> 4));
                 const int steps = before & 15u;
@@ -342,8 +341,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                     step2(v_st, v_ph);
                 }
             };
-            auto first_product = [&](auto gc) {
-                constexpr int g = decltype(gc)::value;
+            auto first_product = [&](int g) {
                 const uint32_t tmem_s = tmem + g * 128, at = (now >> 10 & 1u) * 2 + g;
                 if (now >> (6 + g) & 1u) {
                     alive = mbar_wait(bar_q + at * 8, q_ph >> at & 1, a.status, where);
@@ -374,10 +372,11 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                     alive = mbar_wait(bar_full + v_st * 8, v_ph, a.status, where);
                     fence_after_sync();
                 }
-                if (alive && (before & 16u)) second_product(std::integral_constant<int, 0>());
-                if (alive && (now & 16u)) first_product(std::integral_constant<int, 0>());
-                if (alive && (before & 32u)) second_product(std::integral_constant<int, 1>());
-                if (alive && (now & 32u)) first_product(std::integral_constant<int, 1>());
+#pragma unroll 1
+                for (int g = 0; g < 2; ++g) {             // (one copy of the code for both groups: see the note on instructions above)
+                    if (alive && (before >> (4 + g) & 1u)) second_product(g);
+                    if (alive && (now >> (4 + g) & 1u)) first_product(g);
+                }
                 before = now;
                 if (now == 0u) break;
             }
