@@ -46,6 +46,19 @@ struct ChunkUmmaGeo {
 };
 static_assert(256 * 192 + 256 * 64 <= 512 * 128, "the split draws on what the launch was given");
 
+// A wait with a limit: a million tries, each of which the hardware may hold back for a microsecond (20 ms to a second).  Short, and without the
+// report that mbar_wait makes, because it stands in two dozen places of a kernel that instruction fetches bound: the roles report at their ends.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+    for (int it = 0; it < (1 << 20); ++it) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+                     : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
+        if (ok != 0u) return true;
+    }
+    return false;
+}
+
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float r;
     asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(x), "f"(y), "f"(z));
@@ -188,8 +201,9 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
         if (g == 1 || !a.causal) return me.tiles;
         return line.tiles_of(max(0, min(me.kv, me.kv - me.ql + min(by_group(a, me.qt * G::ROWS + 127), me.ql - 1) + 1)));
     };
-    // keys that the item's first row sees: tiles past it are not seen whole by every row
-    auto first_limit = [&]() { return a.causal ? min(me.kv, me.kv - me.ql + by_group(a, me.qt * G::ROWS) + 1) : me.kv; };
+    // keys that the item's first row (that of its group g) sees: tiles past it are not seen whole by every row
+    auto first_limit = [&](int g = 0) { return a.causal ? min(me.kv, me.kv - me.ql + by_group(a, me.qt * G::ROWS + g * 128) + 1) : me.kv; };
+    auto gave_up = [&]() { report(a.status, FST_DEV_TIMEOUT, where, warp); };
 
     // (Each side asks for its share inside its own branch, since code that both reach gets the lower count; and no function is called
     // there, wait_slow for instance: ptxas then finds no allocation.)
@@ -239,7 +253,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
 #pragma unroll 1
                 for (int v = 0; v < (i < n_tiles ? 2 : 1); ++v) {
                     const uint32_t bar = bar_in + st * 8;
-                    if (use > 0) alive = __all_sync(0xffffffffu, mbar_wait(bar_out + st * 8, (use - 1) & 1, a.status, where));
+                    if (use > 0) alive = __all_sync(0xffffffffu, wait_for(bar_out + st * 8, (use - 1) & 1));
                     if (!alive) break;
                     const bool bad = lane < pages && unsigned(here) >= unsigned(a.c.n_pages);     // its rows read as zeros
                     unsigned char *scales = smem + G::OFF_SCALES + st * 128 + lane * ps;
@@ -267,7 +281,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
 #pragma unroll 1
             for (int v = 0; v < (i < n_tiles ? 2 : 1); ++v) {
                 const uint32_t dst = s_ring + st * TILE, bar = (v && edge ? bar_raw : bar_full) + st * 8;
-                if (use > 0) alive = __all_sync(0xffffffffu, mbar_wait(bar_empty + st * 8, (use - 1) & 1, a.status, where));
+                if (use > 0) alive = __all_sync(0xffffffffu, wait_for(bar_empty + st * 8, (use - 1) & 1));
                 if (!alive) break;
                 to_raw = (to_raw & ~(1u << st)) | uint32_t(v && edge) << st;
                 raw_fills ^= uint32_t(v && edge) << st;
@@ -292,9 +306,10 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
 #pragma unroll 1
         for (int s = 0; s < (QUANT ? RAW : RING); ++s) {
             const uint32_t fills = use + (s < st ? 1u : 0u);
-            if (QUANT && fills > 0) mbar_wait(bar_in + s * 8, (fills - 1) & 1, a.status, where);
-            else if (fills > 0) mbar_wait((to_raw >> s & 1 ? bar_raw : bar_full) + s * 8, to_raw >> s & 1 ? (raw_fills >> s & 1) ^ 1u : (fills - 1) & 1, a.status, where);
+            if (QUANT && fills > 0) alive = wait_for(bar_in + s * 8, (fills - 1) & 1) && alive;
+            else if (fills > 0) alive = wait_for((to_raw >> s & 1 ? bar_raw : bar_full) + s * 8, to_raw >> s & 1 ? (raw_fills >> s & 1) ^ 1u : (fills - 1) & 1) && alive;
         }
+        if (!alive && lane == 0) gave_up();
     } else if (warp == 9) {
         // ====== products: for either group O += P V of the tile before, then S of this one ======
         if (elect_one()) {
@@ -317,19 +332,19 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                 const uint64_t dvs = dv + uint64_t(v_st * (TILE >> 4));
                 const int steps = before & 15u;
                 const bool fresh = before >> (6 + g) & 1u;
-                alive = mbar_wait(bar_p + g * 16, p_ph >> g & 1, a.status, where);
+                alive = wait_for(bar_p + g * 16, p_ph >> g & 1);
                 if (!alive) return;
                 fence_after_sync();
                 if (steps == 8) {
                     mma_f16_ts(tmem_o, tmem_p, dvs, idesc_pv, !fresh);
 #pragma unroll
                     for (int ks = 1; ks < 4; ++ks) mma_f16_ts(tmem_o, tmem_p + ks * 8, dvs + uint64_t((ks * 16 * 128) >> 4), idesc_pv, true);
-                    alive = mbar_wait(bar_p + g * 16 + 8, p_ph >> g & 1, a.status, where);
+                    alive = wait_for(bar_p + g * 16 + 8, p_ph >> g & 1);
                     fence_after_sync();
 #pragma unroll
                     for (int ks = 4; ks < 8; ++ks) mma_f16_ts(tmem_o, tmem_p + ks * 8, dvs + uint64_t((ks * 16 * 128) >> 4), idesc_pv, true);
                 } else {
-                    alive = mbar_wait(bar_p + g * 16 + 8, p_ph >> g & 1, a.status, where);
+                    alive = wait_for(bar_p + g * 16 + 8, p_ph >> g & 1);
                     fence_after_sync();
 #pragma unroll 1
                     for (int ks = 0; ks < steps; ++ks) mma_f16_ts(tmem_o, tmem_p + ks * 8, dvs + uint64_t((ks * 16 * 128) >> 4), idesc_pv, ks > 0 || !fresh);
@@ -344,7 +359,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
             auto first_product = [&](int g) {
                 const uint32_t tmem_s = tmem + g * 128, at = (now >> 10 & 1u) * 2 + g;
                 if (now >> (6 + g) & 1u) {
-                    alive = mbar_wait(bar_q + at * 8, q_ph >> at & 1, a.status, where);
+                    alive = wait_for(bar_q + at * 8, q_ph >> at & 1);
                     q_ph ^= 1u << at;
                     if (!alive) return;
                     fence_after_sync();
@@ -364,12 +379,12 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
             };
 #pragma unroll 1
             while (alive) {
-                alive = mbar_wait(bar_full + k_st * 8, k_ph, a.status, where);
+                alive = wait_for(bar_full + k_st * 8, k_ph);
                 if (!alive) break;
                 fence_after_sync();
                 now = plan[k_st];
                 if (before != 0u) {
-                    alive = mbar_wait(bar_full + v_st * 8, v_ph, a.status, where);
+                    alive = wait_for(bar_full + v_st * 8, v_ph);
                     fence_after_sync();
                 }
 #pragma unroll 1
@@ -381,7 +396,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                 if (now == 0u) break;
             }
             mma_commit(bar_end);                          // all products are done before tensor memory is given back
-            mbar_wait(bar_end, 0, a.status, where);
+            if (!(wait_for(bar_end, 0) && alive)) gave_up();
         }
     } else if (warp == 10 || warp == 11) {
         // ====== rows of Q, an item (D 128) or two ahead of its products' end: one box where whole tokens fit a tile (3 us sooner) ======
@@ -399,7 +414,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                 if (group_tiles(g) <= me.tile) continue;      // (a piece may begin behind the first group's last tile)
                 const int at = (QBUF == 1 ? 0 : (item & 1) * 2) + g;
                 if (used >> at & 1) {                 // the products that read what is there
-                    if (alive) alive = mbar_wait(bar_qfree + at * 8, qfree_ph >> at & 1, a.status, where);
+                    if (alive) alive = wait_for(bar_qfree + at * 8, qfree_ph >> at & 1);
                     qfree_ph ^= 1u << at;
                 }
                 used |= 1u << at;
@@ -432,13 +447,14 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
             me.tile += len - 1;
             if (i + len < n_tiles) me.next(line);
         }
+        if (!alive && lane == 0) gave_up();
     } else {
         const int t128 = tid - 384;
+        bool alive = true;
         if constexpr (QUANT) {
             // ====== 8-bit tiles into 16-bit ones, a thread per row: a scale each, and rows of a swizzled tile are free of conflicts ======
             int st = 0, rs = 0, item = 0;
             uint32_t use = 0, turn = 0;
-            bool alive = true;
 #pragma unroll 1
             for (int i = 0; i <= n_tiles; ++i) {
                 if (i > 0 && i < n_tiles && me.tile == 0) ++item;
@@ -448,8 +464,8 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                     const int have = me.kv - key0;        // V rows behind the sequence's end become zeros
 #pragma unroll 1
                     for (int v = 0; v < (i < n_tiles ? 2 : 1); ++v) {
-                        if (alive) alive = mbar_wait(bar_in + rs * 8, turn & 1, a.status, where);
-                        if (alive && use > 0) alive = mbar_wait(bar_empty + st * 8, (use - 1) & 1, a.status, where);
+                        if (alive) alive = wait_for(bar_in + rs * 8, turn & 1);
+                        if (alive && use > 0) alive = wait_for(bar_empty + st * 8, (use - 1) & 1);
                         if (i < n_tiles) {
                             const uint32_t b = smem[G::OFF_SCALES + rs * 128 + t128];
                             bool none = false;            // a V row that is left out
@@ -485,14 +501,13 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
         // ====== V tiles that not every row attends to all of ======
         int st = 1, item = 0;                             // stage of the tile's V
         uint32_t raw_ph = 0;
-        bool alive = true;
 #pragma unroll 1
         for (int i = 0; i < n_tiles; ++i) {
             if (i > 0 && me.tile == 0) ++item;
             const int key0 = me.tile * G::KEYS;
             if (me.keys > 0) {
                 if (key0 + G::KEYS > first_limit()) {
-                    if (alive) alive = mbar_wait(bar_raw + st * 8, raw_ph >> st & 1, a.status, where);
+                    if (alive) alive = wait_for(bar_raw + st * 8, raw_ph >> st & 1);
                     raw_ph ^= 1u << st;
                     // Rows that take part, whole 16-key steps of them (what lies behind may be anything, and a look there would find it), and
                     // rows of the sequence: those behind become zeros.  Neighbouring threads have neighbouring chunks of 16 bytes.
@@ -536,6 +551,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
             if (i + 1 < n_tiles) me.next(line);
         }
         }
+        if (!alive && t128 == 0) gave_up();
         if (t128 == 0 && a.part != nullptr) leave_cut<D>(a, me, piece.total, n_tiles);
     }
     } else {
@@ -571,11 +587,11 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
             const int row = me.qt * G::ROWS + g * 128 + r, tok = by_group(a, row);
             const int limit = tok >= me.ql ? 0 : a.causal ? min(me.kv, me.kv - me.ql + tok + 1) : me.kv;
             float m_ref = -INFINITY, l = 0.f;
-            // keys of the tile that I see, and that every row sees
-            int n = limit - me.tile * G::KEYS, n_all = first_limit() - me.tile * G::KEYS;
+            // keys of the tile that I see, and that every row of my group sees
+            int n = limit - me.tile * G::KEYS, n_all = first_limit(g) - me.tile * G::KEYS;
 #pragma unroll 1
             for (int j = 0; j < mine; ++j, n -= G::KEYS, n_all -= G::KEYS) {
-                if (alive) alive = __all_sync(0xffffffffu, mbar_wait(my_s, s_ph, a.status, where));
+                if (alive) alive = __all_sync(0xffffffffu, wait_for(my_s, s_ph));
                 s_ph ^= 1u;
                 fence_after_sync();
                 uint32_t s[4][32];
@@ -662,7 +678,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
 
             // ---- the piece's rows: the output where it is the whole item, else sums for the merge
             if (mine > 0) {
-                if (alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_o + g * 8, o_ph, a.status, where));
+                if (alive) alive = __all_sync(0xffffffffu, wait_for(bar_o + g * 8, o_ph));
                 o_ph ^= 1u;
                 fence_after_sync();
             }
@@ -727,6 +743,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
             me.tile += len - 1;
             if (i + len < n_tiles) me.next(line);
         }
+        if (!alive && lane == 0) gave_up();
     }
     __syncwarp();
     fence_before_sync();
