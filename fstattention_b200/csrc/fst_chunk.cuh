@@ -226,20 +226,15 @@ struct ChunkPiece {
         if (warp > 1) return;
         ChunkCursor<ROWS, KEYS, OVER> c;
         const long long all = c.total(line), lo = chunk_first(all, blockIdx.x, gridDim.x), hi = chunk_first(all, blockIdx.x + 1, gridDim.x);
-        const bool lead = (threadIdx.x & 31) == 0;
-        if (hi == lo) {
-            if (lead && warp == 0) before = 0;
-            if (lead && warp == 1) upto = 0;
-        } else if (warp == 0) {
-            const long long n = c.seek(line, lo);
-            if (lead) {
-                from = c;
-                before = n;
-                total = all;
-            }
+        long long n = 0;
+        if (hi > lo) n = c.seek(line, warp == 0 ? lo : min(hi, all - 1)) + (warp == 1 && hi == all ? 1 : 0);         // (the line ends with a tile)
+        if ((threadIdx.x & 31) != 0) return;
+        if (warp == 0) {
+            from = c;
+            before = n;
+            total = all;
         } else {
-            const long long n = hi == all ? c.seek(line, hi - 1) + 1 : c.seek(line, hi);         // (the line ends with a tile)
-            if (lead) upto = n;
+            upto = n;
         }
     }
 };

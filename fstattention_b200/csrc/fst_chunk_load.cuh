@@ -7,6 +7,19 @@
 
 namespace fst {
 
+// A wait with a limit: a million tries, each of which the hardware may hold back for a microsecond (20 ms to a second).  Short, and without the
+// report that mbar_wait makes, because it stands in two dozen places of a kernel that instruction fetches bound: the roles report at their ends.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+    for (int it = 0; it < (1 << 20); ++it) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+                     : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
+        if (ok != 0u) return true;
+    }
+    return false;
+}
+
 // two e4m3 bytes (the low ones, the high ones) -> a pair of fp16
 __device__ __forceinline__ uint32_t e4m3_halves(uint32_t w, bool high) {
     uint32_t r;
@@ -59,7 +72,7 @@ __device__ __forceinline__ void load_tiles(const ChunkArgs &a, const Line &line,
         if (bad) report(a.status, FST_DEV_INDEX_RANGE, z, key0 + lane * ps);
 #pragma unroll 1
         for (int v = 0; v < 2; ++v) {
-            if (use > 0 && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_empty + st * 8, (use - 1) & 1, a.status, blockIdx.x));
+            if (use > 0 && alive) alive = __all_sync(0xffffffffu, wait_for(bar_empty + st * 8, (use - 1) & 1));
             if (!alive) break;
             const CUtensorMap *map = v ? &tm_v : &tm_k;
             const uint32_t bar = bar_full + st * 8, to = s_base + st * G::TILE;
@@ -97,8 +110,9 @@ __device__ __forceinline__ void load_tiles(const ChunkArgs &a, const Line &line,
 #pragma unroll 1
     for (int s = 0; s < G::STAGES; ++s) {
         const uint32_t fills = use + (s < st ? 1u : 0u);
-        if (fills > 0) mbar_wait(bar_full + s * 8, (fills - 1) & 1, a.status, blockIdx.x);
+        if (fills > 0) alive = wait_for(bar_full + s * 8, (fills - 1) & 1) && alive;
     }
+    if (!alive && lane == 0) report(a.status, FST_DEV_TIMEOUT, blockIdx.x, G::WARPS);
 }
 
 }  // namespace fst

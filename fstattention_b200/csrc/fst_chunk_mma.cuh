@@ -201,7 +201,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
         }
 
         const int key0 = group_of(me);
-        if (me.keys > 0 && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_full + slot * 8, parity, a.status, blockIdx.x));
+        if (me.keys > 0 && alive) alive = __all_sync(0xffffffffu, wait_for(bar_full + slot * 8, parity));
         bool k_held = me.keys > 0;
         auto done_with = [&](int stage) {
             __syncwarp();
@@ -293,7 +293,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                 done_with(slot);
                 k_held = false;
             }
-            alive = __all_sync(0xffffffffu, mbar_wait(bar_full + (slot + 1) * 8, parity, a.status, blockIdx.x));     // V
+            alive = __all_sync(0xffffffffu, wait_for(bar_full + (slot + 1) * 8, parity));     // V
             float mw[WEIGHTS ? MT : 1][2], e_v[WEIGHTS ? NK : 1][2];
             if constexpr (WEIGHTS) {
 #pragma unroll
@@ -530,6 +530,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
         }
         if (i + 1 < n_tiles) me.next(line);
     }
+    if (!alive && lane == 0) report(a.status, FST_DEV_TIMEOUT, blockIdx.x, warp);
     if (tid == 0 && a.part != nullptr) leave_cut<D>(a, me, total, n_tiles);
 }
 

@@ -152,7 +152,7 @@ chunk_token_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, 
         }
 
         const int key0 = me.tile * G::KEYS + warp * KW;
-        if (me.keys > 0 && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_full + slot * 8, parity, a.status, blockIdx.x));
+        if (me.keys > 0 && alive) alive = __all_sync(0xffffffffu, wait_for(bar_full + slot * 8, parity));
         bool k_held = me.keys > 0;
         if (key0 < me.keys && alive) {
             const uint32_t k_at = s_base + slot * G::TILE + warp * SUBS * SUB_BYTES, v_at = k_at + G::TILE;          // my rows
@@ -218,7 +218,7 @@ chunk_token_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, 
                 done_with(slot);
                 k_held = false;
             }
-            alive = __all_sync(0xffffffffu, mbar_wait(bar_full + (slot + 1) * 8, parity, a.status, blockIdx.x));     // V
+            alive = __all_sync(0xffffffffu, wait_for(bar_full + (slot + 1) * 8, parity));     // V
             if constexpr (QUANT) {
 #pragma unroll
                 for (int sub = 0; sub < SUBS; ++sub)
@@ -401,6 +401,7 @@ chunk_token_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, 
         }
         if (i + 1 < n_tiles) me.next(line);
     }
+    if (!alive && lane == 0) report(a.status, FST_DEV_TIMEOUT, blockIdx.x, warp);
     if (tid == 0 && a.part != nullptr) leave_cut<D>(a, me, total, n_tiles);
 }
 

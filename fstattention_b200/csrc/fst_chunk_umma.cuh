@@ -46,19 +46,6 @@ struct ChunkUmmaGeo {
 };
 static_assert(256 * 192 + 256 * 64 <= 512 * 128, "the split draws on what the launch was given");
 
-// A wait with a limit: a million tries, each of which the hardware may hold back for a microsecond (20 ms to a second).  Short, and without the
-// report that mbar_wait makes, because it stands in two dozen places of a kernel that instruction fetches bound: the roles report at their ends.
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
-#pragma unroll 1
-    for (int it = 0; it < (1 << 20); ++it) {
-        uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-                     : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
-        if (ok != 0u) return true;
-    }
-    return false;
-}
-
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float r;
     asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(x), "f"(y), "f"(z));
