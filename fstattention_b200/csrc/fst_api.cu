@@ -556,6 +556,7 @@ int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cach
     a.scale_log2 = sm_scale * 1.4426950408889634f;
     a.causal = causal != 0;
     const int n_ctas = chunk_ctas();
+    set_ctas(a, n_ctas);
     const bool splits = chunk_splits(a, 128);
     a.part = splits ? static_cast<float *>(workspace) : nullptr;
     a.status = status;

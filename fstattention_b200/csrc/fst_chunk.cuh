@@ -14,6 +14,7 @@
 // in the order of the CTAs, so the result does not depend on timing.
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "fst_attention_mma.cuh"
@@ -31,6 +32,7 @@ struct ChunkArgs {
     int64_t qs_z, qs_h, qs_n, os_z, os_h, os_n;
     uint32_t group_mul;                    // x / group = x * group_mul >> group_shift for x in [0, 2^31): see set_group
     int group_shift;
+    uint64_t cta_mul;                      // x / n = the high half of x * cta_mul for x < 2^64 / n, n the CTAs of a call: see set_ctas
     float scale_log2;                      // sm_scale * log2(e), positive
     int causal;
     int q_boxes;                           // Q comes as boxes of `group` heads by 128 / group tokens
@@ -48,6 +50,10 @@ inline void set_group(ChunkArgs &a, int group) {
     a.group_shift = 31 + s;
 }
 __device__ __forceinline__ int by_group(const ChunkArgs &a, int x) { return int(uint64_t(uint32_t(x)) * a.group_mul >> a.group_shift); }
+
+// With m = floor(2^64 / n) + 1, m n exceeds 2^64 by at most n, so x m / 2^64 exceeds x / n by at most x / 2^64: less than 1 / n for x < 2^64 / n.
+// (n is at least 2.)
+inline void set_ctas(ChunkArgs &a, int n) { a.cta_mul = ~uint64_t(0) / uint64_t(n) + 1; }
 
 // The line of work for row tiles of ROWS and key tiles of KEYS.  An item is OVER units longer than it has key tiles: its own start and end
 // cost a CTA as much as that many tiles (a CTA that got seven items of two tiles each ended at 51 us, the others at 30).  They lie
@@ -168,7 +174,9 @@ struct ChunkCursor {
             }
         }
         open(line);
-        h = int(pos / head);
+        h = int(__fdividef(float(pos), float(head)));     // (a division of 64 bits is a hundred instructions to fetch; the estimate is off by one at most, or little more)
+        while (h > 0 && h * head > pos) --h;
+        while ((h + 1) * head <= pos) ++h;
         pos -= h * head;
         qt = 0;
         if (n_qt > 1) {
@@ -212,7 +220,11 @@ struct ChunkCursor {
 
 
 // CTA i of n takes the tiles of units [first(i), first(i + 1)) of the line
-__device__ __forceinline__ long long chunk_first(long long total, int i, int n) { return total / n * i + min((long long)i, total % n); }
+__device__ __forceinline__ long long chunk_share(const ChunkArgs &a, long long total) { return (long long)__umul64hi(uint64_t(total), a.cta_mul); }
+__device__ __forceinline__ long long chunk_first(const ChunkArgs &a, long long total, int i, int n) {
+    const long long each = chunk_share(a, total);
+    return each * i + min((long long)i, total - each * n);
+}
 
 // A CTA's piece of the line, found by two of its warps for all (in shared memory).
 template <int ROWS, int KEYS, int OVER>
@@ -225,7 +237,7 @@ struct ChunkPiece {
         const int warp = threadIdx.x >> 5;
         if (warp > 1) return;
         ChunkCursor<ROWS, KEYS, OVER> c;
-        const long long all = c.total(line), lo = chunk_first(all, blockIdx.x, gridDim.x), hi = chunk_first(all, blockIdx.x + 1, gridDim.x);
+        const long long all = c.total(line), lo = chunk_first(line.a, all, blockIdx.x, gridDim.x), hi = chunk_first(line.a, all, blockIdx.x + 1, gridDim.x);
         long long n = 0;
         if (hi > lo) n = c.seek(line, warp == 0 ? lo : min(hi, all - 1)) + (warp == 1 && hi == all ? 1 : 0);         // (the line ends with a tile)
         if ((threadIdx.x & 31) != 0) return;
@@ -328,9 +340,9 @@ __device__ __forceinline__ void leave_cut(const ChunkArgs &a, const ChunkCursor<
         const int behind = last.tiles - last.tile - 1;
         if (behind > 0 && n_tiles > last.tile) {          // it goes on (then its next tile is the next CTA's first unit), and began here
             const int me = blockIdx.x, n = gridDim.x;
-            const long long end = chunk_first(total, me + 1, n) + behind;
-            int c = me + 1 + int((behind - 1) / (total / n + 1));
-            while (c + 1 < n && chunk_first(total, c + 1, n) < end) ++c;
+            const long long end = chunk_first(a, total, me + 1, n) + behind;
+            int c = me + 1 + (behind - 1) / int(min(chunk_share(a, total) + 1, 0x7fffffffLL));
+            while (c + 1 < n && chunk_first(a, total, c + 1, n) < end) ++c;
             cut.pieces = c - me + 1;
         }
     }
@@ -420,7 +432,7 @@ cudaError_t launch_chunk_combine(const ChunkArgs &a, int n_ctas, cudaStream_t st
 }
 
 // CTAs of a call's line: one per SM (a workspace holds two pieces for each).
-inline int chunk_ctas() { return sm_count(); }
+inline int chunk_ctas() { return std::max(sm_count(), 2); }
 // Which kernel: up to 32 rows those on mma.sync.
 inline bool chunk_many_rows(const ChunkArgs &a) { return (long long)a.n_q * a.group > 32; }
 inline int chunk_row_tile(const ChunkArgs &a) {
