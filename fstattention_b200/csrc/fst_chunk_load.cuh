@@ -68,7 +68,6 @@ __device__ __forceinline__ void load_tiles(const ChunkArgs &a, const Line &line,
         if (i + 1 < n_tiles) look_up();
         if (pages <= 0) continue;
         const bool bad = lane < pages && unsigned(here) >= unsigned(a.c.n_pages);            // the boxes then read as zeros
-        const uint32_t wrong = __ballot_sync(0xffffffffu, bad);
         if (bad) report(a.status, FST_DEV_INDEX_RANGE, z, key0 + lane * ps);
 #pragma unroll 1
         for (int v = 0; v < 2; ++v) {
@@ -77,14 +76,17 @@ __device__ __forceinline__ void load_tiles(const ChunkArgs &a, const Line &line,
             const CUtensorMap *map = v ? &tm_v : &tm_k;
             const uint32_t bar = bar_full + st * 8, to = s_base + st * G::TILE;
             unsigned char *scales = smem + G::OFF_SCALES + st * G::KEYS;
-            if constexpr (QUANT) {
-                if (bad) {
-                    for (int k = 0; k < ps; k += 16) *reinterpret_cast<uint4 *>(scales + lane * ps + k) = make_uint4(0, 0, 0, 0);
-                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            if constexpr (QUANT) {                        // sixteen rows' scales a lane, zeros for a bad page
+                static_assert(G::KEYS <= 512, "a lane each");
+                const int p = lane >> (a.c.page_shift - 4), pg = __shfl_sync(0xffffffffu, here, p);
+                if (p < pages && lane * 16 < G::KEYS) {
+                    const uint8_t *from = v ? a.c.v_scale : a.c.k_scale;
+                    const bool there = unsigned(pg) < unsigned(a.c.n_pages);
+                    cp_async16(smem_u32(scales + lane * 16), there ? from + ((size_t(pg) * a.H_kv + h) << a.c.page_shift) + (lane * 16 & (ps - 1)) : from, there);
                 }
-                __syncwarp();
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(bar) : "memory");
             }
-            if (lane == 0) mbar_arrive_expect_tx(bar, (pages << a.c.page_shift) * D * (QUANT ? 1 : 2) + (QUANT ? (pages - __popc(wrong)) * ps : 0));
+            if (lane == 0) mbar_arrive_expect_tx(bar, (pages << a.c.page_shift) * D * (QUANT ? 1 : 2));
             __syncwarp();
 #pragma unroll 1
             for (int p = 0; p < pages; ++p) {
@@ -92,7 +94,6 @@ __device__ __forceinline__ void load_tiles(const ChunkArgs &a, const Line &line,
                 if (umma::elect_one()) {
                     if constexpr (QUANT) {
                         tma_load_4d(to + row * D, map, 0, 0, h, pg, bar);
-                        if (!(wrong >> p & 1u)) bulk_load(smem_u32(scales + row), (v ? a.c.v_scale : a.c.k_scale) + ((size_t(pg) * a.H_kv + h) << a.c.page_shift), ps, bar);
                     } else {
 #pragma unroll
                         for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(to + hf * (G::KEYS * 128) + row * 128, map, hf * 64, 0, h, pg, bar);

@@ -29,8 +29,13 @@ inline bool make_pool_map(CUtensorMap *map, const PoolKey &key) {
     const cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUtensorMapDataType type = bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                            : key.type == POOL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    // What L2 is asked to bring along: a row (it is the neighbouring head's that lies next to it, and nobody needs that soon), or as much as
+    // goes where a head's rows lie together.  (Two sequences of 115000 e4m3 rows, heads inside rows: 100 us with 256 bytes, 87 with 128.)
+    const int64_t row_bytes = key.stride_row == key.D ? 256 : int64_t(key.D * size);
+    const CUtensorMapL2promotion along = row_bytes >= 256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                                         : row_bytes >= 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_64B;
     return fn(map, type, 4, const_cast<void *>(key.base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              bytes && key.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              bytes && key.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, along,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

@@ -58,7 +58,7 @@ chunk_token_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, 
     const uint32_t bar_full = s_base + G::OFF_BAR, bar_empty = bar_full + G::STAGES * 8;
     if (tid == 0) {
         for (int i = 0; i < G::STAGES; ++i) {
-            mbar_init(bar_full + i * 8, 1);
+            mbar_init(bar_full + i * 8, QUANT ? 33 : 1);      // (the lanes' scales, see load_tiles)
             mbar_init(bar_empty + i * 8, G::WARPS);
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
