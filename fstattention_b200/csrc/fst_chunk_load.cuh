@@ -88,15 +88,31 @@ __device__ __forceinline__ void load_tiles(const ChunkArgs &a, const Line &line,
             }
             if (lane == 0) mbar_arrive_expect_tx(bar, (pages << a.c.page_shift) * D * (QUANT ? 1 : 2));
             __syncwarp();
+            // Who asks for the pages, measured in us.  An 8-bit cache: a lane each, or one lane one after the other: 98 and 112 (two sequences of 115000
+            // rows) where pages have 16 rows, 90 and 87 where they have 64.  16 bits (64 sequences of 4500 rows): a lane each 187, one lane four
+            // at a time 183.
+            if constexpr (QUANT) {
+                if (ps <= 32) {
+                    if (lane < pages) tma_load_4d(to + lane * ps * D, map, 0, 0, h, here, bar);
+                } else {
 #pragma unroll 1
-            for (int p = 0; p < pages; ++p) {
-                const int pg = __shfl_sync(0xffffffffu, here, p), row = p * ps;
-                if (umma::elect_one()) {
-                    if constexpr (QUANT) {
-                        tma_load_4d(to + row * D, map, 0, 0, h, pg, bar);
-                    } else {
+                    for (int p = 0; p < pages; ++p) {
+                        const int pg = __shfl_sync(0xffffffffu, here, p);
+                        if (umma::elect_one()) tma_load_4d(to + p * ps * D, map, 0, 0, h, pg, bar);
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (int p = 0; p < pages; p += 4) {
+                    int pg[4];
 #pragma unroll
-                        for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(to + hf * (G::KEYS * 128) + row * 128, map, hf * 64, 0, h, pg, bar);
+                    for (int k = 0; k < 4; ++k) pg[k] = __shfl_sync(0xffffffffu, here, p + k);
+                    if (!umma::elect_one()) continue;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (p + k >= pages) break;
+#pragma unroll
+                        for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(to + hf * (G::KEYS * 128) + (p + k) * ps * 128, map, hf * 64, 0, h, pg[k], bar);
                     }
                 }
             }
