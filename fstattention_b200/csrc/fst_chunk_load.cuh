@@ -37,12 +37,6 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr));
     return v;
 }
-// `bytes` (a multiple of 16) contiguous bytes of global memory into shared memory
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, int bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-
 // By one warp: the tiles of a CTA's piece of the line, K and V in turn, into G::STAGES stages of G::TILE bytes at s_base (KEYS rows: 64-column
 // halves of 16 bits, or bytes), an 8-bit tile's scales at G::OFF_SCALES; full[stage] says that it has landed, empty[stage] that it may go.
 template <typename G, int D, bool QUANT, typename Line, typename Cursor>

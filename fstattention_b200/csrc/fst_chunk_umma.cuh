@@ -161,7 +161,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                 mbar_init(bar_o + i * 8, 1);
             }
             mbar_init(bar_end, 1);
-            for (int i = 0; i < 2 * RAW; ++i) mbar_init(bar_in + i * 8, 1);
+            for (int i = 0; i < 2 * RAW; ++i) mbar_init(bar_in + i * 8, i < RAW ? 33 : 1);
             *note = 0x7fffffff;
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         }
@@ -242,23 +242,21 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                     const uint32_t bar = bar_in + st * 8;
                     if (use > 0) alive = __all_sync(0xffffffffu, wait_for(bar_out + st * 8, (use - 1) & 1));
                     if (!alive) break;
-                    const bool bad = lane < pages && unsigned(here) >= unsigned(a.c.n_pages);     // its rows read as zeros
-                    unsigned char *scales = smem + G::OFF_SCALES + st * 128 + lane * ps;
-                    if (bad) {
-                        if (v == 0) report(a.status, FST_DEV_INDEX_RANGE, z, key0 + lane * ps);
-                        for (int k = 0; k < ps; k += 16) *reinterpret_cast<uint4 *>(scales + k) = make_uint4(0, 0, 0, 0);
-                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    if (v == 0 && lane < pages && unsigned(here) >= unsigned(a.c.n_pages)) report(a.status, FST_DEV_INDEX_RANGE, z, key0 + lane * ps);
+                    // sixteen rows' scales a lane, zeros for a bad page, as its rows are (see load_tiles)
+                    const int p = lane >> (a.c.page_shift - 4), pg = __shfl_sync(0xffffffffu, here, p);
+                    if (p < pages && lane < G::KEYS / 16) {
+                        const uint8_t *from = v ? a.c.v_scale : a.c.k_scale;
+                        const bool there = unsigned(pg) < unsigned(a.c.n_pages);
+                        cp_async16(smem_u32(smem + G::OFF_SCALES + st * 128 + lane * 16), there ? from + ((size_t(pg) * a.H_kv + h) << a.c.page_shift) + (lane * 16 & (ps - 1)) : from, there);
                     }
-                    const int good = pages - __popc(__ballot_sync(0xffffffffu, bad));
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(bar) : "memory");
                     if (lane == 0) {
                         if (v == 0) raw_plan[st] = word;
-                        mbar_arrive_expect_tx(bar, ((pages * D + good) << a.c.page_shift));
+                        mbar_arrive_expect_tx(bar, (pages * D) << a.c.page_shift);
                     }
                     __syncwarp();
-                    if (lane < pages) {
-                        tma_load_4d(s_base + G::OFF_RAW + st * 128 * D + lane * ps * D, v ? &tm_v : &tm_k, 0, 0, h, here, bar);
-                        if (!bad) bulk_load(smem_u32(scales), (v ? a.c.v_scale : a.c.k_scale) + ((size_t(here) * a.H_kv + h) << a.c.page_shift), ps, bar);
-                    }
+                    if (lane < pages) tma_load_4d(s_base + G::OFF_RAW + st * 128 * D + lane * ps * D, v ? &tm_v : &tm_k, 0, 0, h, here, bar);
                     if (++st == RAW) {
                         st = 0;
                         ++use;
