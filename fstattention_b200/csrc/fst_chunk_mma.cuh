@@ -13,6 +13,10 @@
 // byte's seven low bits moved under bf16's exponent are its value * 2^-120, half of which comes back with the scale and half at the
 // end.  Under fp16 queries, whose results have three more bits, V is fp16 and the scales go into the exponents of weights of their
 // own (WEIGHTS), as in chunk_token_kernel.
+//
+// 7 draft tokens of 4 heads behind 24 x 8 heads of 2300 e4m3 rows at D 64: 46 us (58 MB, 9 us of HBM): a fixed 20, of them 4 for the merge and as many for
+// the warps' meetings at every item's end, and 2.1 us a tile of 256 keys: some 1300 instructions a warp for it, most of them conversions and
+// the softmax, from two warps to a scheduler.
 #pragma once
 
 #include "fst_chunk_load.cuh"

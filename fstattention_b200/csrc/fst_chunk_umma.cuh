@@ -6,8 +6,13 @@
 //     O += P V     tcgen05.mma, A = P in tensor memory, B = V (its rows are the summed index)
 // A K/V tile comes in once for both groups, and while one group's products run the other group's warps take exponentials.
 //
-// What bounds a tile at D 128: the tensor cores need 4 x 512 cycles for it and the 16 exponentials a clock of an SM
-// just as many, so the hand-overs between the two have to stay short.
+// What bounds a tile: the tensor cores need 2048 cycles for it at D 128 (1024 at D 64) and the 16 exponentials a clock of an SM 2048, so the
+// hand-overs between the two have to stay short; it takes 3100 at either D.  Instructions come next: the roles' code is more than the
+// instruction cache holds, so what runs in turn is kept small (one copy of the issuing code for both groups and short waits: 4096 tokens over 32768
+// rows of 8 heads 929 -> 776 us, four prompts of 1024 tokens at D 64 69.5 -> 58.5).  The first is 1.05 - 1.25 PFLOP/s, as the power limit
+// lets clocks be; the second has 3.5 items of 2 to 8 tiles a CTA, and their starts and ends are half of it.
+// Tried and not kept: an issuing lane per group (263 -> 299 us at D 128: the groups fall into step; nothing at D 64, with S of the next tile
+// ahead), 4 or 8 of 32 exponentials by a polynomial (0 to 4 %, slower for short items), two threads a row, steps of 64 keys.
 //
 // Sixteen warps: 0-3 and 4-7 are the softmax groups; 8 loads K and V, lane j page j of a tile; one lane of 9 issues the products;
 // 10 and 11 bring the items' rows of Q; 12-15 look through the V tiles that not every row attends to all of (the diagonal, the
@@ -674,7 +679,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
             const int head = me.h * a.group + (row - tok * a.group);
             const size_t slot = (size_t(2) * blockIdx.x + (me.tile == 0 ? 1 : 0)) * G::ROWS + g * 128 + r;
             // The rows leave through shared memory, four whole lines of 128 bytes a store: by 16 or 32 bytes of 32 rows at a time a piece took
-            // 5 us to write, by lines ...
+            // 5 us to write, by lines 3.3.
             const uint32_t out_at = s_base + G::OFF_OUT + warp * 4096;
             const unsigned long long to = reinterpret_cast<unsigned long long>(
                 whole ? static_cast<void *>(static_cast<T *>(a.o) + me.z * a.os_z + head * a.os_h + tok * a.os_n) : static_cast<void *>(a.part + slot * D));

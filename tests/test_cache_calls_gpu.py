@@ -269,9 +269,9 @@ def test_a_query_that_is_not_finite_keeps_to_its_row(N):
 
 # ---- expanded 8-bit caches ---------------------------------------------------------------------------------
 def test_an_expanded_cache():
-    """512 rows of a head and more: bad pages, sequences without queries or rows, and a graph whose lengths grow."""
+    """2048 rows of a head and more: bad pages, sequences without queries or rows, and a graph whose lengths grow."""
     gen = torch.Generator().manual_seed(7)
-    H, H_kv, D, N = 4, 2, 64, 260
+    H, H_kv, D, N = 16, 2, 64, 260
     lens = [300, 0, 600, 17]
     cache = list(new_cache(gen, lens, H_kv, D, 16, "NHD", torch.bfloat16, True, extra=64))
     q = torch.randn((4, H, N, D), generator=gen).to(torch.bfloat16).cuda()

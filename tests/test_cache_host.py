@@ -116,14 +116,14 @@ def test_workspaces(built_lib):
     assert size(C.byref(large), 64, 4, 2, 3, 64) == need == size(C.byref(cache(table_stride=4000)), 1, 4, 2, 3, 64)
     assert lib.fst_attention_chunk(*chunk_args(large, workspace=None)) == WORKSPACE
     assert lib.fst_attention_chunk(*chunk_args(large, bytes=need - 1)) == WORKSPACE
-    # an 8-bit cache under 512 rows of a head or more: its rows in 16 bits as well, two tensors of Z * pages pages, and a table
+    # an 8-bit cache under 2048 rows of a head or more: its rows in 16 bits as well, two tensors of Z * pages pages, and a table
     quantised = cache(table_stride=9, k_scale=P(512), v_scale=P(1024))
-    few, many = size(C.byref(quantised), 3, 4, 2, 255, 64), size(C.byref(quantised), 3, 4, 2, 256, 64)
+    few, many = size(C.byref(quantised), 3, 4, 2, 1023, 64), size(C.byref(quantised), 3, 4, 2, 1024, 64)
     pages = 3 * 9
-    assert few == size(C.byref(large), 3, 4, 2, 255, 64)
+    assert few == size(C.byref(large), 3, 4, 2, 1023, 64)
     assert many - pages * (2 * 16 * 2 * 64 * 2 + 4) in range(few, few + 256)
     huge = cache(table_stride=1 << 17, k_scale=P(512), v_scale=P(1024))           # 2^21 rows of 2 heads of 64: 2 GB, and past that
-    assert size(C.byref(huge), 2, 4, 2, 256, 64) > 1 << 31 and size(C.byref(huge), 5, 4, 2, 256, 64) == few
+    assert size(C.byref(huge), 2, 4, 2, 1024, 64) > 1 << 31 and size(C.byref(huge), 5, 4, 2, 1024, 64) == few
 
 
 # ---- the oracle ---------------------------------------------------------------------------------
