@@ -8,7 +8,7 @@
 //
 // What bounds a tile: the tensor cores need 2048 cycles for it at D 128 (1024 at D 64) and the 16 exponentials a clock of an SM 2048, so the
 // hand-overs between the two have to stay short; it takes 3100 at either D.  Instructions come next: the roles' code is more than the
-// instruction cache holds, so what runs in turn is kept small (one copy of the issuing code for both groups and short waits: 4096 tokens over 32768
+// instruction cache holds, so what runs in turn is kept small (one copy of the issuing code for both groups and short waits: 4096 tokens over 16400
 // rows of 8 heads 929 -> 776 us, four prompts of 1024 tokens at D 64 69.5 -> 58.5).  The first is 1.05 - 1.25 PFLOP/s, as the power limit
 // lets clocks be; the second has 3.5 items of 2 to 8 tiles a CTA, and their starts and ends are half of it.
 // Tried and not kept: an issuing lane per group (263 -> 299 us at D 128: the groups fall into step; nothing at D 64, with S of the next tile
