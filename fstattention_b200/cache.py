@@ -14,7 +14,8 @@ float8_e8m0fnu ``[n_pages, H_kv, page_size]``, hold a power of two for every row
 
 All calls are asynchronous on torch's current stream and can be captured into a graph; lengths and tables are read
 on the GPU.  What only the GPU can see (a page number outside the pool, a length past the table) is
-recorded for ``last_status`` and never faults.
+recorded for ``last_status`` and never faults.  (A length is not looked at where a sequence has no queries.)  What an
+8-bit cache holds is what ``fst_cache_append`` wrote or zeros: e4m3's NaN bytes do not occur.
 """
 from __future__ import annotations
 
@@ -81,8 +82,9 @@ def fst_attention_chunk(q, k_pool, v_pool, block_table, kv_lens, sm_scale, *, q_
     mixed.  Both lengths are int32 ``[Z]``.
 
     A query that sees no row gets zeros.  Rows ``i >= q_lens[z]`` of ``out`` are left as they are (zeros where the call
-    allocates it).  What the cache holds at rows that a query does not attend to, NaN included, does not reach it.
+    allocates it).  ``out`` may be ``q``.  What the cache holds at rows that a query does not attend to, NaN included, does not reach it.
     An 8-bit cache under float16 queries is meant to hold values that float16 can hold (``fst_cache_read``).
+    Sums are float32: values of V that overflow it when added up (a number of rows times 1e38) are not averaged.
     With ``return_lse`` the result is ``(out, lse)``, ``lse`` the base-2 log-sum-exp of the scaled scores,
     ``[Z * H, N]``, -inf where nothing is seen.  ``sm_scale`` must be positive."""
     host = _lib._host or _lib.host()

@@ -377,7 +377,7 @@ int fst_cache_read(const fst_paged_cache *cache, void *k, void *v, const int32_t
  * Attention of new tokens over the cache, which holds their own rows too.  q: [Z][H][n_q][head_dim], H a multiple
  * of H_kv.  Sequence z has kv_lens[z] rows in the cache and q_lens[z] queries (NULL: n_q), its last
  * q_lens[z] positions: query i attends to rows [0, kv_lens[z] - q_lens[z] + i], or with causal = 0 to all kv_lens[z] rows.
- * A query that sees no row gets zeros (lse -inf).  Rows i >= q_lens[z] of o and lse are left as they are.  What the
+ * o may be q.  A query that sees no row gets zeros (lse -inf).  Rows i >= q_lens[z] of o and lse are left as they are.  What the
  * cache holds at rows that a query does not attend to, NaN and infinities included, does not reach it.
  * Over an 8-bit cache fp16 queries take rows as fp16 where n_q H / H_kv > 32: values past 65504 saturate.
  * lse, when not NULL, is [Z][H][n_q], base-2 log-sum-exp of the scaled scores.  sm_scale must be positive and finite.

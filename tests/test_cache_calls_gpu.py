@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import fstattention_b200 as fst
+import test_cache_gpu as basics
 from oracle import cache_oracle as orc
 from test_cache_gpu import E4M3, E8M0, append, check, chunk, clean, int32, new_cache, read
 
@@ -303,6 +304,25 @@ def test_an_expanded_cache():
     zeros[2] = table.clone()
     zeros[2][0, 3] = spare
     assert torch.equal(chunk(q, zeros, kv, 0.125, q_lens=ql), got)
+    clean()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_what_is_not_finite_in_an_expanded_cache(dtype):
+    basics.test_what_is_not_finite_stays_where_it_is_seen(520, 8, 2, 64, dtype, True)
+
+
+def test_queries_overwritten_by_their_results():
+    """``out`` may be ``q``: the rows of an item are read before they are written, whoever divides them."""
+    gen = torch.Generator().manual_seed(16)
+    for quantised in (False, True):
+        for N, lens in ((1, [5000, 30]), (7, [2000, 900]), (12, [3000, 12]), (300, [2500, 310])):
+            cache = new_cache(gen, lens, 2, 128, 64, "NHD", torch.bfloat16, quantised)
+            q = torch.randn((2, 8, N, 128), generator=gen).to(torch.bfloat16).cuda()
+            want = chunk(q, cache, int32(lens), 0.1)
+            for _ in range(3):
+                same = q.clone()
+                assert torch.equal(chunk(same, cache, int32(lens), 0.1, out=same), want)
     clean()
 
 
