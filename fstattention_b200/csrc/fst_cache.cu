@@ -10,7 +10,7 @@
 namespace fst {
 
 constexpr int CACHE_THREADS = 256;
-constexpr int CACHE_ROWS = 2;          // rows of a thread where there are many: 8192 rows of 8 heads quantised, 1: 12.9 us, 2: 11.0, 4: 12.0; 30011 read, 36.8, 33.2, 37.1
+constexpr int CACHE_ROWS = 2;          // rows of a thread that reads many: 30011 rows of 8 heads out of e4m3 with 1: 36.8 us, 2: 33.2, 4: 37.1
 
 template <typename T>
 __device__ __forceinline__ float2 two_floats(uint32_t w) {
@@ -18,98 +18,91 @@ __device__ __forceinline__ float2 two_floats(uint32_t w) {
     else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w));
 }
 
-// Eight values of a row that D / 8 neighbouring lanes hold: the row's largest magnitude is taken over them.  Magnitudes are compared as
+// Sixteen values of a row that D / 16 neighbouring lanes hold: the row's largest magnitude is taken over them.  Magnitudes are compared as
 // integers, two at a time, where NaN and infinity are the largest (instructions bound large appends: 12.9 us with floats, 11.2 so).
 template <typename T, int D>
-__device__ __forceinline__ uint2 quantise8(uint4 in, uint32_t &biased) {
+__device__ __forceinline__ uint4 quantise16(const uint4 (&in)[2], uint32_t &biased) {
     constexpr bool HALF = std::is_same<T, __half>::value;
-    const uint32_t w[4] = {in.x, in.y, in.z, in.w};
-    uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+    const uint32_t w[8] = {in[0].x, in[0].y, in[0].z, in[0].w, in[1].x, in[1].y, in[1].z, in[1].w};
+    uint32_t top = 0;
 #pragma unroll
-    for (int s = 1; s < D / 8; s *= 2) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, s));
+    for (int i = 0; i < 8; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+#pragma unroll
+    for (int s = 1; s < D / 16; s *= 2) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, s));
     top = max(top & 0xffffu, top >> 16);
     if (top >= (HALF ? 0x7c00u : 0x7f80u)) {
         biased = 255u;
-        return make_uint2(0u, 0u);
+        return make_uint4(0u, 0u, 0u, 0u);
     }
     const int e = e4m3_exponent(two_floats<T>(top).x);
     const float f = pow2f(-e);
     biased = uint32_t(e + 127);
-    uint32_t b[4];
+    uint32_t b[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
         const float2 x = two_floats<T>(w[i]);
         b[i] = e4m3_pair(x.x * f, x.y * f);
     }
-    return make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+    return make_uint4(b[0] | b[1] << 16, b[2] | b[3] << 16, b[4] | b[5] << 16, b[6] | b[7] << 16);
 }
 
-// Rows j of head h of sequence z, neighbours in the source and in a page by neighbouring threads.  R = 1: all (z, h, j) in one line.  R > 1: a block has
-// R * RPB rows of one head, so that nothing is divided and a thread has R rows on their way.
-template <typename T, int D, bool QUANT, int R>
+// New row j of head h of sequence z, all (z, h, j) in one line; neighbours in the source and in a page by neighbouring threads, 16 bytes a lane
+// into a page.  (Quantising, 8 bytes a lane and two rows a thread took 10.6 us for 8192 rows of 8 heads, this 8.6; two rows a thread then gain
+// nothing.)
+template <typename T, int D, bool QUANT>
 __global__ void __launch_bounds__(CACHE_THREADS)
 cache_append_kernel(const AppendArgs a) {
-    constexpr int LPR = D / 8, RPB = CACHE_THREADS / LPR;
+    constexpr int C = QUANT ? 2 : 1, LPR = D / (8 * C), RPB = CACHE_THREADS / LPR;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    const unsigned first = blockIdx.x * (RPB * R) + threadIdx.x / LPR, col = (threadIdx.x % LPR) * 8;
-    uint4 k[R], v[R];
-    int64_t pos[R];
-    int page[R];
-    unsigned head[R];
-    bool live[R];
+    const unsigned r = blockIdx.x * RPB + threadIdx.x / LPR, col = (threadIdx.x % LPR) * (8 * C);
+    const unsigned zh = r / unsigned(a.M), j = r - zh * unsigned(a.M), z = zh / unsigned(a.H_kv), h = zh - z * unsigned(a.H_kv);
+    uint4 k[C], v[C];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        unsigned j = first + i * RPB, z = blockIdx.z, h = blockIdx.y;
-        if constexpr (R == 1) {
-            const unsigned zh = j / unsigned(a.M);
-            j -= zh * unsigned(a.M);
-            z = zh / unsigned(a.H_kv);
-            h = zh - z * unsigned(a.H_kv);
-        }
-        live[i] = R == 1 ? z < unsigned(a.Z) : j < unsigned(a.M);
-        k[i] = v[i] = make_uint4(0, 0, 0, 0);
-        pos[i] = 0;
-        page[i] = 0;
-        head[i] = h;
-        if (!live[i]) continue;
+    for (int c = 0; c < C; ++c) k[c] = v[c] = make_uint4(0, 0, 0, 0);
+    int64_t pos = 0;
+    int page = 0;
+    bool live = z < unsigned(a.Z);
+    if (live) {
         const int row = a.rows != nullptr ? __ldg(a.rows + size_t(z) * a.M + j) : int(j);
         const int count = a.lens != nullptr ? __ldg(a.lens + z) : a.M;
-        pos[i] = int64_t(__ldg(a.start + z)) + j;
-        live[i] = int(j) < count;
-        if (live[i] && (row < 0 || row >= a.N || pos[i] < 0 || (pos[i] >> a.c.page_shift) >= a.c.width)) {
+        pos = int64_t(__ldg(a.start + z)) + j;
+        live = int(j) < count;
+        if (live && (row < 0 || row >= a.N || pos < 0 || (pos >> a.c.page_shift) >= a.c.width)) {
             if (col == 0) report(a.status, FST_DEV_INDEX_RANGE, int(z), int(j));
-            live[i] = false;
+            live = false;
         }
-        if (live[i]) {
-            k[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.k) + z * a.ks_z + h * a.ks_h + row * a.ks_n + col));
-            v[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.v) + z * a.vs_z + h * a.vs_h + row * a.vs_n + col));
-            page[i] = __ldg(a.c.table + size_t(z) * a.c.width + (pos[i] >> a.c.page_shift));
-            if (unsigned(page[i]) >= unsigned(a.c.n_pages)) {
+        if (live) {
+            const T *from_k = static_cast<const T *>(a.k) + z * a.ks_z + h * a.ks_h + row * a.ks_n + col;
+            const T *from_v = static_cast<const T *>(a.v) + z * a.vs_z + h * a.vs_h + row * a.vs_n + col;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                k[c] = __ldg(reinterpret_cast<const uint4 *>(from_k) + c);
+                v[c] = __ldg(reinterpret_cast<const uint4 *>(from_v) + c);
+            }
+            page = __ldg(a.c.table + size_t(z) * a.c.width + (pos >> a.c.page_shift));
+            if (unsigned(page) >= unsigned(a.c.n_pages)) {
                 if (col == 0) report(a.status, FST_DEV_INDEX_RANGE, int(z), int(j));
-                live[i] = false;
+                live = false;
             }
         }
     }
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int off = int(pos[i]) & ((1 << a.c.page_shift) - 1);
-        const int64_t to = page[i] * a.c.stride_page + off * a.c.stride_row + head[i] * a.c.stride_head + col;
-        if constexpr (QUANT) {
-            uint32_t ek, ev;                              // (all lanes take part in the maximum)
-            const uint2 qk = quantise8<T, D>(k[i], ek), qv = quantise8<T, D>(v[i], ev);
-            if (!live[i]) continue;
-            *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(a.c.k_pool) + to) = qk;
-            *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(a.c.v_pool) + to) = qv;
-            if (col == 0) {
-                const size_t at = ((size_t(page[i]) * a.H_kv + head[i]) << a.c.page_shift) + off;
-                a.c.k_scale[at] = uint8_t(ek);
-                a.c.v_scale[at] = uint8_t(ev);
-            }
-        } else if (live[i]) {
-            *reinterpret_cast<uint4 *>(static_cast<T *>(a.c.k_pool) + to) = k[i];
-            *reinterpret_cast<uint4 *>(static_cast<T *>(a.c.v_pool) + to) = v[i];
+    const int off = int(pos) & ((1 << a.c.page_shift) - 1);
+    const int64_t to = page * a.c.stride_page + off * a.c.stride_row + h * a.c.stride_head + col;
+    if constexpr (QUANT) {
+        uint32_t ek, ev;                                  // (all lanes take part in the maximum)
+        const uint4 qk = quantise16<T, D>(k, ek), qv = quantise16<T, D>(v, ev);
+        if (!live) return;
+        *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(a.c.k_pool) + to) = qk;
+        *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(a.c.v_pool) + to) = qv;
+        if (col == 0) {
+            const size_t at = ((size_t(page) * a.H_kv + h) << a.c.page_shift) + off;
+            a.c.k_scale[at] = uint8_t(ek);
+            a.c.v_scale[at] = uint8_t(ev);
         }
+    } else if (live) {
+        *reinterpret_cast<uint4 *>(static_cast<T *>(a.c.k_pool) + to) = k[0];
+        *reinterpret_cast<uint4 *>(static_cast<T *>(a.c.v_pool) + to) = v[0];
     }
 }
 
@@ -125,7 +118,8 @@ __device__ __forceinline__ uint4 expand8(uint2 b, float scale) {
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// Eight values a lane, so that the lanes of a row write it as a whole.  R as above; a block that lies behind its sequence's end only writes.
+// Eight values a lane, so that the lanes of a row write it as a whole.  R = 1: all (z, h, row) in one line.  R > 1: a block has R * RPB rows of one
+// head, so that nothing is divided and a thread has R rows on their way.  Rows behind a sequence's end are only written.
 template <typename T, int D, bool QUANT, int R>
 __global__ void __launch_bounds__(CACHE_THREADS)
 cache_read_kernel(const ReadArgs a) {
@@ -275,7 +269,10 @@ static cudaError_t launch_rows(K1 one, KR several, const A &a, cudaStream_t stre
 
 template <typename T, int D, bool QUANT>
 static cudaError_t launch_append_t(const AppendArgs &a, cudaStream_t stream) {
-    return launch_rows<CACHE_ROWS, CACHE_THREADS / (D / 8)>(cache_append_kernel<T, D, QUANT, 1>, cache_append_kernel<T, D, QUANT, CACHE_ROWS>, a, stream);
+    constexpr int RPB = CACHE_THREADS / (D / (QUANT ? 16 : 8));
+    const long long units = (long long)a.Z * a.H_kv * a.M;
+    if (units > 0x7fffffffLL - RPB) return cudaErrorInvalidConfiguration;
+    return launch_rows(cache_append_kernel<T, D, QUANT>, a, dim3(unsigned((units + RPB - 1) / RPB)), stream);
 }
 template <typename T, int D, bool QUANT>
 static cudaError_t launch_read_t(const ReadArgs &a, cudaStream_t stream) {
