@@ -12,7 +12,8 @@
 // rows of 8 heads 929 -> 776 us, four prompts of 1024 tokens at D 64 69.5 -> 58.5).  The first is 1.05 - 1.25 PFLOP/s, as the power limit
 // lets clocks be; the second has 3.5 items of 2 to 8 tiles a CTA, and their starts and ends are half of it.
 // Tried and not kept: an issuing lane per group (263 -> 299 us at D 128: the groups fall into step; nothing at D 64, with S of the next tile
-// ahead), 4 or 8 of 32 exponentials by a polynomial (0 to 4 %, slower for short items), two threads a row, steps of 64 keys.
+// ahead), 4 or 8 of 32 exponentials by a polynomial (0 to 4 %, slower for short items), two threads a row, steps of 64 keys, no exponentials for
+// the parts of a tile that a warp does not see (branches among them: 56.7 -> 59.4 us for the prompts).
 //
 // Sixteen warps: 0-3 and 4-7 are the softmax groups; 8 loads K and V, lane j page j of a tile; one lane of 9 issues the products;
 // 10 and 11 bring the items' rows of Q; 12-15 look through the V tiles that not every row attends to all of (the diagonal, the
