@@ -7,7 +7,7 @@ sm_scale * sum_d |q_d k_d|:
 * the output's own rounding, eps / 2 of its value, eps that of its type (an fp16 result below 2^-14: half of 2^-24);
 * the rounding of the probabilities to 16 bits for the second product, eps / 2 of A (bf16's eps over an 8-bit cache);
 * scores: fp32 sums of D products, D roundings of S (2^-23 each, the tensor cores may truncate), three more for the scale and
-  the distance to the maximum, and the exponential's own error, 2.6e-6 < 2^-18 for the polynomial; numerator and denominator are
+  the distance to the maximum, and the exponential's own error, below 2^-18; numerator and denominator are
   both off by that share: 2 A (2^-23 (D + 3) S + 2^-18);
 * the sums over T keys in fp32: T + 64 roundings of 2^-23 at the most, of numerator and denominator: 2 A 2^-23 (T + 64).
 """
