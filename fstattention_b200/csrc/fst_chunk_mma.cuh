@@ -429,6 +429,10 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     }
                 }
             }
+        } else if (me.keys > 0 && alive) {
+            // No key of this tile is mine.  V's stage is given back only once it has been filled: that is what says that every warp has
+            // given back its last filling, which an arrival ahead of that would have stood in for a warp that still reads it.
+            alive = __all_sync(0xffffffffu, wait_for(bar_full + (slot + 1) * 8, parity));
         }
         if (me.keys > 0) {
             if (k_held) done_with(slot);

@@ -320,6 +320,9 @@ chunk_token_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, 
                     }
                 }
             }
+        } else if (me.keys > 0 && alive) {
+            // No key of this tile is mine: V's stage goes back once it is full, see chunk_mma_kernel.
+            alive = __all_sync(0xffffffffu, wait_for(bar_full + (slot + 1) * 8, parity));
         }
         if (me.keys > 0) {
             if (k_held) done_with(slot);
