@@ -193,7 +193,10 @@ cache_expand_kernel(const ExpandArgs a) {
 #pragma unroll 1
     for (int z0 = 0; z0 < a.Z; z0 += 256) {
         __syncthreads();
-        if (z0 + int(threadIdx.x) < a.Z) pages[threadIdx.x] = min((max(__ldg(a.lens + z0 + threadIdx.x), 0) + ps - 1) >> a.c.page_shift, a.c.width);
+        if (z0 + int(threadIdx.x) < a.Z) {                 // (cut to the table first: the rounding up must not leave 31 bits)
+            const int rows = min(max(__ldg(a.lens + z0 + threadIdx.x), 0), a.c.width << a.c.page_shift);
+            pages[threadIdx.x] = (rows + ps - 1) >> a.c.page_shift;
+        }
         __syncthreads();
 #pragma unroll 1
         for (int z = z0; z < min(a.Z, z0 + 256); ++z) {

@@ -30,3 +30,25 @@ def test_long_items_whose_last_tile_is_nearly_empty(N, H, D, quantised):
         again, lse_again = chunk(q, cache, int32(lens), D ** -0.5, return_lse=True)
         assert torch.equal(again, first) and torch.equal(lse_again, lse)
     clean()
+
+
+# ---- lengths far past the table ----------------------------------------------------------------------------
+INT_MAX = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("length", [1 << 30, INT_MAX - 127, INT_MAX - 14, INT_MAX])
+def test_lengths_up_to_the_largest_are_cut(length, page):
+    """Cut to what the table holds and reported: by an 8-bit cache that is expanded first (2048 rows of a head), and by the other kernels."""
+    gen = torch.Generator().manual_seed(page)
+    for N, H in ((1, 4), (12, 4), (100, 4), (520, 8)):
+        cache = new_cache(gen, [600, 40], 2, 64, page, "NHD", torch.bfloat16, True)
+        q = torch.randn((2, H, N, 64), generator=gen).to(torch.bfloat16).cuda()
+        most = cache[2].shape[1] * page
+        want = chunk(q, cache, int32([most, 40]), 0.125)
+        clean()
+        got = chunk(q, cache, int32([length, 40]), 0.125)
+        assert fst.last_status(clear=True) == 18 and torch.equal(got, want)
+        x = torch.zeros((2, 2, 1, 64), dtype=torch.bfloat16, device="cuda")
+        append(x, x, cache, int32([length, 0]))
+        assert fst.last_status(clear=True) == 18
