@@ -7,12 +7,10 @@
 //
 // 8-bit rows become matrix fragments in registers, without their scales.  The order of the summed index is free as long as both operands
 // agree, so lane (g, t) of a K fragment takes the contiguous bytes D/4 t .. of key g, and Q is loaded in the same order; of V it
-// takes bytes D/8 g .. of its four keys, which only permutes the columns of the result.  K is fp16, by the conversion instruction, and a
-// key's scale multiplies its score.  bf16 queries become fp16 times a power of two per row, with the row's largest value next to 2^15:
-// what fp16 loses then is 2^-39 of that.  Under bf16 queries V is bf16 too, as a row's scale goes into its probability and needs the range: a
-// byte's seven low bits moved under bf16's exponent are its value * 2^-120, half of which comes back with the scale and half at the
-// end.  Under fp16 queries, whose results have three more bits, V is fp16 and the scales go into the exponents of weights of their
-// own (WEIGHTS), as in chunk_token_kernel.
+// takes bytes D/8 g .. of its four keys, which only permutes the columns of the result.  K and V are fp16, by the conversion instruction.  A
+// key's scale multiplies its score; bf16 queries become fp16 times a power of two per row, with the row's largest value next to 2^15:
+// what fp16 loses then is 2^-39 of that.  V's scales go into the exponents of weights of their own, as in chunk_token_kernel: no single
+// factor brings all of their range, 2^-117 to 2^119, through a 16-bit probability and an fp32 sum.
 //
 // 7 draft tokens of 4 heads behind 24 x 8 heads of 2300 e4m3 rows at D 64: 46 us (58 MB, 9 us of HBM): a fixed 20, of them 4 for the merge and as many for
 // the warps' meetings at every item's end, and 2.1 us a tile of 256 keys: some 1300 instructions a warp for it, most of them conversions and
@@ -40,24 +38,15 @@ struct ChunkMmaGeo {
     static constexpr int BYTES = OFF_BAR + 2 * STAGES * 8 + 1024;   // + alignment
 };
 
-constexpr float kTiny = 1.152921504606846976e18f;        // 2^60, half of what a bf16 made of an e4m3's bits lacks
-
-// four e4m3 bytes -> two pairs of bf16 (bytes 0 and 2, bytes 1 and 3), smaller by 2^120
-__device__ __forceinline__ void e4m3_bits(uint32_t w, uint32_t &even, uint32_t &odd) {
-    odd = (w & 0x80008000u) | ((w >> 4) & 0x07f007f0u);
-    const uint32_t u = w << 8;
-    even = (u & 0x80008000u) | ((u >> 4) & 0x07f007f0u);
-}
 template <typename T, int D, bool QUANT, int MT>
 __global__ void __launch_bounds__(384, 1)
 chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
     using G = ChunkMmaGeo<D, QUANT, MT>;
     using MT_ = MmaTraits<T>;
-    using MK = MmaTraits<typename std::conditional<QUANT, __half, T>::type>;     // of the first product, of the second
-    using MP = MmaTraits<T>;
+    using MP = MmaTraits<typename std::conditional<QUANT, __half, T>::type>;     // of the products
     using Line = ChunkLine<G::ROWS, G::KEYS, G::OVER>;
     using Cursor = ChunkCursor<G::ROWS, G::KEYS, G::OVER>;
-    constexpr bool BF16 = !std::is_same<T, __half>::value, WEIGHTS = QUANT && !BF16;
+    constexpr bool BF16 = !std::is_same<T, __half>::value;
     constexpr float LIFT = !QUANT && !BF16 ? kLift : 0.f;
     constexpr int KS = D / 16, ND = D / 8;               // steps of the first product, column tiles of the second
     constexpr int KW = G::KW, NK = KW / 8, SUBS = KW / 16;
@@ -116,7 +105,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
     };
     float acc[MT][ND][4], m[MT][2], l[MT][2];
     float row_c2[QUANT ? MT : 1][2];                      // an 8-bit cache: c2 over the row's factor
-    float m_w[WEIGHTS ? MT : 1][2];                       // running maximum of score and V's exponent
+    float m_w[QUANT ? MT : 1][2];                       // running maximum of score and V's exponent
     int limit[MT][2], lim_first = 0, slot = 0;
     uint32_t parity = 0;
     bool poisoned = false, alive = true;                  // a V that is not finite was met where not every row attends to it
@@ -140,7 +129,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     const T *src = static_cast<const T *>(a.q) + me.z * a.qs_z + (me.h * a.group + (r - tok * a.group)) * a.qs_h + tok * a.qs_n;
                     // two of the four registers of a row tile's fragments: the row's part of two steps in an 8-bit cache's order, or of one
                     float by = 1.f;                       // the row's factor
-                    if constexpr (WEIGHTS) m_w[x][hh] = -INFINITY;
+                    if constexpr (QUANT) m_w[x][hh] = -INFINITY;
                     if constexpr (QUANT) {
                         if constexpr (BF16) {
                             uint32_t top = 0;
@@ -162,7 +151,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         f[0] = w.x; f[1] = w.y; f[2] = w.z; f[3] = w.w;
                         if constexpr (BF16) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) f[k] = MK::pack(__uint_as_float(f[k] << 16) * by, __uint_as_float(f[k] & 0xffff0000u) * by);
+                            for (int k = 0; k < 4; ++k) f[k] = MP::pack(__uint_as_float(f[k] << 16) * by, __uint_as_float(f[k] & 0xffff0000u) * by);
                         }
                     };
                     auto one_step = [&](int st, uint32_t &lo, uint32_t &hi) {
@@ -242,7 +231,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                             const uint32_t w = k == 0 ? b[n].x : k == 1 ? b[n].y : k == 2 ? b[n].z : b[n].w;
                             const uint32_t b0 = e4m3_halves(w, false), b1 = e4m3_halves(w, true);
 #pragma unroll
-                            for (int x = 0; x < MT; ++x) MK::mma(s[x][n], q[x], b0, b1);
+                            for (int x = 0; x < MT; ++x) MP::mma(s[x][n], q[x], b0, b1);
                         }
                     }
                 }
@@ -298,8 +287,8 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                 k_held = false;
             }
             alive = __all_sync(0xffffffffu, wait_for(bar_full + (slot + 1) * 8, parity));     // V
-            float mw[WEIGHTS ? MT : 1][2], e_v[WEIGHTS ? NK : 1][2];
-            if constexpr (WEIGHTS) {
+            float mw[QUANT ? MT : 1][2], e_v[QUANT ? NK : 1][2];
+            if constexpr (QUANT) {
 #pragma unroll
                 for (int x = 0; x < MT; ++x) mw[x][0] = mw[x][1] = -INFINITY;
 #pragma unroll
@@ -330,7 +319,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     };
                     move(m[x][hh], mx[x][hh], alpha[hh], LIFT);
                     alpha_w[hh] = alpha[hh];
-                    if constexpr (WEIGHTS) move(m_w[x][hh], mw[x][hh], alpha_w[hh], kLift);
+                    if constexpr (QUANT) move(m_w[x][hh], mw[x][hh], alpha_w[hh], kLift);
                 }
                 if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -346,12 +335,6 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
             }
 #pragma unroll
             for (int n = 0; n < NK; ++n) {
-                float vs[2] = {1.f, 1.f};
-                if constexpr (QUANT && !WEIGHTS) {
-                    const uint32_t b = *reinterpret_cast<const uint16_t *>(scales + G::KEYS + 8 * n + 2 * t);
-                    vs[0] = e8m0_value(b & 255u) * kTiny;
-                    vs[1] = e8m0_value(b >> 8) * kTiny;
-                }
 #pragma unroll
                 for (int x = 0; x < MT; ++x) {
                     float p[4];
@@ -360,9 +343,8 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         const float v = s[x][n][k];
                         p[k] = fast_exp2(v - mx[x][k >> 1]);
                         l[x][k >> 1] += p[k];
-                        // the row's scale; what a masked key holds, NaN too, stays out
-                        if constexpr (WEIGHTS) p[k] = v == -INFINITY ? 0.f : fast_exp2(v + e_v[n][k & 1] - mw[x][k >> 1]);
-                        else if constexpr (QUANT) p[k] = v == -INFINITY ? 0.f : p[k] * vs[k & 1];
+                        // (what a masked key holds, NaN too, stays out)
+                        if constexpr (QUANT) p[k] = v == -INFINITY ? 0.f : fast_exp2(v + e_v[n][k & 1] - mw[x][k >> 1]);
                     }
                     pf[x][n >> 1][(n & 1) * 2] = MP::pack(p[0], p[1]);
                     pf[x][n >> 1][(n & 1) * 2 + 1] = MP::pack(p[2], p[3]);
@@ -385,7 +367,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                             const uint2 b = lds64(v_at + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8);
                             w[k][0] = b.x; w[k][1] = b.y;
                         }
-                        if (WEIGHTS && edge && row >= here) {                    // zero times a NaN byte would be NaN
+                        if (edge && row >= here) {                    // zero times a NaN byte would be NaN
 #pragma unroll
                             for (int c = 0; c < D / 32; ++c) w[k][c] = 0u;
                         }
@@ -394,17 +376,8 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     for (int c = 0; c < D / 32; ++c)
 #pragma unroll
                         for (int hl = 0; hl < 2; ++hl) {  // two column tiles from bytes 2 hl, 2 hl + 1 of either key
-                            uint32_t b0[2], b1[2];
-                            if constexpr (WEIGHTS) {
-                                const uint32_t y0 = __byte_perm(w[0][c], w[1][c], hl ? 0x7362 : 0x5140), y1 = __byte_perm(w[2][c], w[3][c], hl ? 0x7362 : 0x5140);
-                                b0[0] = e4m3_halves(y0, false);
-                                b0[1] = e4m3_halves(y0, true);
-                                b1[0] = e4m3_halves(y1, false);
-                                b1[1] = e4m3_halves(y1, true);
-                            } else {
-                                e4m3_bits(__byte_perm(w[0][c], w[1][c], hl ? 0x7632 : 0x5410), b0[0], b0[1]);
-                                e4m3_bits(__byte_perm(w[2][c], w[3][c], hl ? 0x7632 : 0x5410), b1[0], b1[1]);
-                            }
+                            const uint32_t y0 = __byte_perm(w[0][c], w[1][c], hl ? 0x7362 : 0x5140), y1 = __byte_perm(w[2][c], w[3][c], hl ? 0x7362 : 0x5140);
+                            const uint32_t b0[2] = {e4m3_halves(y0, false), e4m3_halves(y0, true)}, b1[2] = {e4m3_halves(y1, false), e4m3_halves(y1, true)};
 #pragma unroll
                             for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -461,7 +434,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                     if (t == 0) stats[warp * G::ROWS + x * 16 + hh * 8 + g] = make_float2(m[x][hh] - LIFT, sum);
                     float *to = rows + (warp * 16 + hh * 8 + g) * (D + 4);
-                    if constexpr (WEIGHTS) {              // weights back to the probabilities' reference
+                    if constexpr (QUANT) {                // weights back to the probabilities' reference
                         const float by = m[x][hh] == -INFINITY ? 1.f : fast_exp2(m_w[x][hh] - kLift - m[x][hh]);
 #pragma unroll
                         for (int j = 0; j < ND; ++j)
@@ -503,10 +476,6 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         out[k + 2] += v.z * f;
                         out[k + 3] += v.w * f;
                     }
-                }
-                if (QUANT && !WEIGHTS) {
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) out[k] *= kTiny;
                 }
                 const int r = me.qt * G::ROWS + x * 16 + row, tok = by_group(a, r), head = me.h * a.group + (r - tok * a.group);
                 if (bad != 0u && tok < me.ql) {

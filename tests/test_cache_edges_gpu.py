@@ -52,3 +52,46 @@ def test_lengths_up_to_the_largest_are_cut(length, page):
         x = torch.zeros((2, 2, 1, 64), dtype=torch.bfloat16, device="cuda")
         append(x, x, cache, int32([length, 0]))
         assert fst.last_status(clear=True) == 18
+
+
+# ---- scales of V over all of their range ---------------------------------------------------------------------
+def with_v_exponents(cache, low, high, gen):
+    """The same cache with every V row's exponent drawn from [low, high]."""
+    c = list(cache)
+    c[4] = torch.randint(low + 127, high + 128, c[4].shape, generator=gen).to(torch.uint8).cuda().view(torch.float8_e8m0fnu)
+    return c
+
+
+def check_scaled(got, lse, want, T, p_eps, floor):
+    """As ``check``, for outputs of any size: ``floor`` is half the smallest step of what the output and its sums are held in."""
+    out, _, mag, size = want
+    share = 2.0 ** -23 * (got.shape[-1] + 3) * size[..., None] + 2.0 ** -18
+    tol = out.abs() * torch.finfo(got.dtype).eps / 2 + mag * (p_eps / 2 + 2 * share + 2 * 2.0 ** -23 * (T + 64)) + floor
+    assert torch.isfinite(got).all()
+    worst = float(((got.double() - out).abs() - tol).max())
+    assert worst <= 0, (worst, float(out.abs().max()))
+    check(torch.zeros_like(got), lse, (torch.zeros_like(out), *want[1:]), True, T)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("N", [1, 3, 7, 60])
+def test_v_exponents_over_their_whole_range(N, dtype, D):
+    """4, 12, 28 and 240 rows of a head.  bf16: rows of V up to 448 * 2^105, and one at 2^119 where no sum of many can leave fp32; fp16:
+    up to 448 * 2^6, which its outputs hold.  Probabilities are off by bf16's rounding at the most."""
+    gen = torch.Generator().manual_seed(N + D)
+    lens, bf16 = [700, 333], dtype == torch.bfloat16
+    base = new_cache(gen, lens, 2, D, 32, "NHD", dtype, True)
+    q = torch.randn((2, 8, N, D), generator=gen).to(dtype).cuda()
+    p_eps = torch.finfo(torch.bfloat16).eps
+    floor = 2.0 ** -134 if bf16 else 2.0 ** -25
+    for low, high, one in ((-117, 105 if bf16 else 6, None), (66, 70, None), (-90, -86, None), (-117, 60, 119)):
+        if not bf16 and high > 6 or one is not None and N == 60:
+            continue
+        cache = with_v_exponents(base, low, high, gen)
+        if one is not None:
+            page, off = orc.row_of(cache, 0, torch.tensor([555], device="cuda"))
+            cache[4].view(torch.uint8)[page, :, off] = one + 127
+        out, lse = chunk(q, cache, int32(lens), D ** -0.5, return_lse=True)
+        clean()
+        check_scaled(out, lse, orc.attention(q, cache, lens, D ** -0.5), 700, p_eps, floor)
