@@ -435,11 +435,12 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     if (t == 0) stats[warp * G::ROWS + x * 16 + hh * 8 + g] = make_float2(m[x][hh] - LIFT, sum);
                     float *to = rows + (warp * 16 + hh * 8 + g) * (D + 4);
                     if constexpr (QUANT) {                // weights back to the probabilities' reference
-                        const float by = m[x][hh] == -INFINITY ? 1.f : fast_exp2(m_w[x][hh] - kLift - m[x][hh]);
+                        float by, then;
+                        weights_back(m[x][hh], m_w[x][hh], by, then);
 #pragma unroll
                         for (int j = 0; j < ND; ++j)
 #pragma unroll
-                            for (int k = 0; k < 2; ++k) acc[x][j][2 * hh + k] *= by;
+                            for (int k = 0; k < 2; ++k) acc[x][j][2 * hh + k] = acc[x][j][2 * hh + k] * by * then;
                     }
                     if constexpr (QUANT) {
 #pragma unroll

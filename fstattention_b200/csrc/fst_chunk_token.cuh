@@ -350,10 +350,12 @@ chunk_token_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, 
                 if (g == 0) stats[warp * 8 + 2 * t + q] = make_float2(m[q] - LIFT, sum);
                 float *to = rows + (warp * 8 + 2 * t + q) * (D + 4);
                 if constexpr (QUANT) {
-                    const float by = m[q] == -INFINITY ? 1.f : fast_exp2(m_w[q] - kLift - m[q]);          // weights back to the probabilities' reference
+                    float by, then;                       // weights back to the probabilities' reference
+                    weights_back(m[q], m_w[q], by, then);
 #pragma unroll
                     for (int n = 0; n < NP; n += 2)
-                        *reinterpret_cast<float4 *>(to + g * (D / 8) + 2 * n) = make_float4(acc[n][q] * by, acc[n][2 + q] * by, acc[n + 1][q] * by, acc[n + 1][2 + q] * by);
+                        *reinterpret_cast<float4 *>(to + g * (D / 8) + 2 * n) =
+                            make_float4(acc[n][q] * by * then, acc[n][2 + q] * by * then, acc[n + 1][q] * by * then, acc[n + 1][2 + q] * by * then);
                 } else {
 #pragma unroll
                     for (int n = 0; n < NP; ++n) {

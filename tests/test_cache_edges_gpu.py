@@ -95,3 +95,21 @@ def test_v_exponents_over_their_whole_range(N, dtype, D):
         out, lse = chunk(q, cache, int32(lens), D ** -0.5, return_lse=True)
         clean()
         check_scaled(out, lse, orc.attention(q, cache, lens, D ** -0.5), 700, p_eps, floor)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("N", [1, 3, 7, 60])
+def test_rows_of_v_of_the_smallest_scales(N, dtype):
+    """Values down to 2^-126 are bf16 numbers: they reach the output.  (fp16 outputs hold none of them.)"""
+    gen = torch.Generator().manual_seed(N)
+    lens = [700, 333]
+    q = torch.randn((2, 8, N, 64), generator=gen).to(dtype).cuda()
+    cache = with_v_exponents(new_cache(gen, lens, 2, 64, 32, "NHD", dtype, True), -117, -114, gen)
+    out, lse = chunk(q, cache, int32(lens), 0.125, return_lse=True)
+    clean()
+    want = orc.attention(q, cache, lens, 0.125)
+    if dtype == torch.float16:
+        assert not out.any()
+        return
+    assert (want[0].abs() > 2.0 ** -126).any()
+    check_scaled(out, lse, want, 700, torch.finfo(torch.bfloat16).eps, 2.0 ** -134)
