@@ -47,7 +47,8 @@ def fst_cache_append(k, v, k_pool, v_pool, block_table, start, *, lens: Optional
     at most 448.  A row with an element that is not finite reads as NaN.
 
     A row whose position lies outside its table, whose page is not one of the pool's or whose entry of ``rows`` is not
-    one of ``k``'s is not written (``last_status``).  No two rows of a call may go to the same place: pages that
+    one of ``k``'s is not written, and of a count ``lens[z]`` above the call's rows only those are (``last_status`` in
+    either case); a count below zero is none.  No two rows of a call may go to the same place: pages that
     sequences share are to be copied before one of them writes there."""
     host = _lib._host or _lib.host()
     host.cache_append(k, v, k_pool, v_pool, _nhd(pool_layout), block_table, start, lens, rows, k_scale, v_scale)

@@ -68,6 +68,7 @@ cache_append_kernel(const AppendArgs a) {
         const int count = a.lens != nullptr ? __ldg(a.lens + z) : a.M;
         pos = int64_t(__ldg(a.start + z)) + j;
         live = int(j) < count;
+        if (count > a.M && j == 0 && h == 0 && col == 0) report(a.status, FST_DEV_INDEX_RANGE, int(z), count);
         if (live && (row < 0 || row >= a.N || pos < 0 || (pos >> a.c.page_shift) >= a.c.width)) {
             if (col == 0) report(a.status, FST_DEV_INDEX_RANGE, int(z), int(j));
             live = false;

@@ -354,7 +354,7 @@ typedef struct fst_paged_cache {
  * [-117, 119] with a <= 448 * 2^e, the values rounded to e4m3(x * 2^-e) (nearest, ties to even, saturating) and
  * b = e + 127; a row with an element that is not finite gets zeros and b = 255.
  * A position outside the table, a page number outside [0, n_pages) or an entry of rows outside [0, N) is not written and sets
- * FST_DEV_INDEX_RANGE.  Two rows of a call must not go to the same place: which of them (and of its halves) stays is not defined.
+ * FST_DEV_INDEX_RANGE, and so does a count lens[z] > M, of which M rows are written (one below zero is none).  Two rows of a call must not go to the same place: which of them (and of its halves) stays is not defined.
  */
 int fst_cache_append(const fst_paged_cache *cache, const void *k, const void *v, const int32_t *start,
                      const int32_t *lens, const int32_t *rows, int Z, int H_kv, int N, int M, int head_dim,

@@ -113,3 +113,26 @@ def test_rows_of_v_of_the_smallest_scales(N, dtype):
         return
     assert (want[0].abs() > 2.0 ** -126).any()
     check_scaled(out, lse, want, 700, torch.finfo(torch.bfloat16).eps, 2.0 ** -134)
+
+
+# ---- counts that a call does not have ------------------------------------------------------------------------
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("path", [False, True])
+def test_a_count_above_the_rows_of_an_append_is_reported(path, quantised):
+    """The rows that there are go into the pages, as they do without a count; one below zero is none."""
+    gen = torch.Generator().manual_seed(6)
+    k = torch.randn((3, 2, 4, 64), generator=gen).to(torch.bfloat16).cuda()
+    rows = int32([[2, 0, 3]] * 3) if path else None
+    M = 3 if path else 4
+    cache = list(new_cache(gen, [20, 20, 20], 2, 64, 16, "NHD", torch.bfloat16, quantised))
+    other = [t.clone() if torch.is_tensor(t) else t for t in cache]
+    append(k, k, cache, int32([14, 3, 0]), rows=rows)
+    append(k, k, other, int32([14, 3, 0]), rows=rows, lens=int32([M, M, M]))
+    clean()
+    for count in (M + 1, INT_MAX):
+        append(k, k, other, int32([14, 3, 0]), rows=rows, lens=int32([M, count, M]))
+        assert fst.last_status(clear=True) == 18
+    append(k, k, other, int32([0, 0, 0]), rows=rows, lens=int32([-1, -INT_MAX - 1, 0]))
+    clean()
+    for a, b in zip(cache[:5], other[:5]):
+        assert a is b or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
