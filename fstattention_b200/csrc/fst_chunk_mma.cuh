@@ -268,9 +268,9 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
             for (int n = 0; n < NK; ++n) {
                 float ks[2] = {1.f, 1.f};                 // of my keys 8 n + 2 t + k
                 if constexpr (QUANT) {
-                    const uint32_t b = *reinterpret_cast<const uint16_t *>(scales + 8 * n + 2 * t);
-                    ks[0] = e8m0_value(b & 255u);
-                    ks[1] = e8m0_value(b >> 8);
+                    const float2 both = e8m0_values(*reinterpret_cast<const uint16_t *>(scales + 8 * n + 2 * t));
+                    ks[0] = both.x;
+                    ks[1] = both.y;
                 }
 #pragma unroll
                 for (int x = 0; x < MT; ++x)

@@ -136,3 +136,41 @@ def test_a_count_above_the_rows_of_an_append_is_reported(path, quantised):
     clean()
     for a, b in zip(cache[:5], other[:5]):
         assert a is b or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+# ---- every byte that a scale can be -------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_every_byte_under_every_scale(dtype):
+    """Two heads of 128 bytes have all 256 values, 256 rows all scales: 2^(b - 127) for b from 0 to 254, NaN for 255.  One rounding."""
+    value = torch.arange(256, dtype=torch.uint8).view(1, 1, 2, 128).expand(2, 128, 2, 128).contiguous().cuda().view(torch.float8_e4m3fn)
+    scale = torch.arange(256, dtype=torch.uint8).view(2, 1, 128).expand(2, 2, 128).contiguous().cuda().view(torch.float8_e8m0fnu)
+    table, n = int32([[0, 1]]), int32([256])
+    got = fst.fst_cache_read(value, value, table, n, 256, k_scale=scale, v_scale=scale, dtype=dtype)
+    clean()
+    power = torch.cat([orc.pow2(torch.arange(255) - 127), torch.tensor([float("nan")], dtype=torch.float64)]).cuda()
+    want = value.view(256, 2, 128).double().transpose(0, 1) * power[None, :, None]
+    most = torch.finfo(torch.float16).max
+    want = (want.clamp(-most, most) if dtype == torch.float16 else want).to(dtype)
+    for x in got:
+        assert torch.equal(torch.isnan(x[0]), torch.isnan(want)) and torch.equal(torch.nan_to_num(x[0]), torch.nan_to_num(want))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("N", [1, 3, 7, 60])
+def test_the_smallest_scale_byte_means_the_same_to_every_kernel(N, D):
+    """Rows of V under b = 0, 2^-127: up to 2^-118, of which sums may lose what lies below 2^-126, the smallest normal number."""
+    gen = torch.Generator().manual_seed(N)
+    lens = [700, 333]
+    q = torch.randn((2, 8, N, D), generator=gen).to(torch.bfloat16).cuda()
+    cache = with_v_exponents(new_cache(gen, lens, 2, D, 32, "NHD", torch.bfloat16, True), -127, -127, gen)
+    cache[1].view(torch.uint8).fill_(0x7e)                # 448 everywhere
+    out, lse = chunk(q, cache, int32(lens), D ** -0.5, return_lse=True)
+    clean()
+    want = orc.attention(q, cache, lens, D ** -0.5)
+    assert (want[0] > 2.0 ** -119).all()
+    check_scaled(out, lse, want, 700, torch.finfo(torch.bfloat16).eps, 2.0 ** -126)
+    # K under it: scores of next to nothing, so that all weights are alike
+    cache = list(new_cache(gen, lens, 2, D, 32, "NHD", torch.bfloat16, True))
+    cache[3].view(torch.uint8).zero_()
+    check(*chunk(q, cache, int32(lens), D ** -0.5, return_lse=True), orc.attention(q, cache, lens, D ** -0.5), True, 700)
+    clean()
