@@ -64,9 +64,9 @@ cache_append_kernel(const AppendArgs a) {
     int page = 0;
     bool live = z < unsigned(a.Z);
     if (live) {
-        const int row = a.rows != nullptr ? __ldg(a.rows + size_t(z) * a.M + j) : int(j);
-        const int count = a.lens != nullptr ? __ldg(a.lens + z) : a.M;
-        pos = int64_t(__ldg(a.start + z)) + j;
+        const int row = a.rows != nullptr ? load(a.rows + size_t(z) * a.M + j) : int(j);
+        const int count = a.lens != nullptr ? load(a.lens + z) : a.M;
+        pos = int64_t(load(a.start + z)) + j;
         live = int(j) < count;
         if (count > a.M && j == 0 && h == 0 && col == 0) report(a.status, FST_DEV_INDEX_RANGE, int(z), count);
         if (live && (row < 0 || row >= a.N || pos < 0 || (pos >> a.c.page_shift) >= a.c.width)) {
@@ -78,10 +78,10 @@ cache_append_kernel(const AppendArgs a) {
             const T *from_v = static_cast<const T *>(a.v) + z * a.vs_z + h * a.vs_h + row * a.vs_n + col;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                k[c] = __ldg(reinterpret_cast<const uint4 *>(from_k) + c);
-                v[c] = __ldg(reinterpret_cast<const uint4 *>(from_v) + c);
+                k[c] = load(reinterpret_cast<const uint4 *>(from_k) + c);
+                v[c] = load(reinterpret_cast<const uint4 *>(from_v) + c);
             }
-            page = __ldg(a.c.table + size_t(z) * a.c.width + (pos >> a.c.page_shift));
+            page = load(a.c.table + size_t(z) * a.c.width + (pos >> a.c.page_shift));
             if (unsigned(page) >= unsigned(a.c.n_pages)) {
                 if (col == 0) report(a.status, FST_DEV_INDEX_RANGE, int(z), int(j));
                 live = false;
@@ -141,8 +141,8 @@ cache_read_kernel(const ReadArgs a) {
         }
         k[i] = v[i] = make_uint4(0, 0, 0, 0);             // (rows behind a sequence's end are zeros)
         ek[i] = ev[i] = 0.f;
-        if ((R == 1 ? z >= unsigned(a.Z) : r >= unsigned(a.M)) || int(r) >= __ldg(a.lens + z)) continue;
-        const int idx = int(r >> a.c.page_shift), page = idx < a.c.width ? __ldg(a.c.table + size_t(z) * a.c.width + idx) : -1;
+        if ((R == 1 ? z >= unsigned(a.Z) : r >= unsigned(a.M)) || int(r) >= load(a.lens + z)) continue;
+        const int idx = int(r >> a.c.page_shift), page = idx < a.c.width ? load(a.c.table + size_t(z) * a.c.width + idx) : -1;
         if (unsigned(page) >= unsigned(a.c.n_pages)) {
             if (col == 0) report(a.status, FST_DEV_INDEX_RANGE, int(z), int(r));
             continue;
@@ -151,15 +151,15 @@ cache_read_kernel(const ReadArgs a) {
         const int64_t from = page * a.c.stride_page + off * a.c.stride_row + h * a.c.stride_head + col;
         if constexpr (QUANT) {
             const size_t at = ((size_t(page) * a.H_kv + h) << a.c.page_shift) + off;
-            const uint2 bk = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.k_pool) + from));
-            const uint2 bv = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.v_pool) + from));
+            const uint2 bk = load(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.k_pool) + from));
+            const uint2 bv = load(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.v_pool) + from));
             k[i] = make_uint4(bk.x, bk.y, 0, 0);
             v[i] = make_uint4(bv.x, bv.y, 0, 0);
-            ek[i] = e8m0_value(__ldg(a.c.k_scale + at));
-            ev[i] = e8m0_value(__ldg(a.c.v_scale + at));
+            ek[i] = e8m0_value(load(a.c.k_scale + at));
+            ev[i] = e8m0_value(load(a.c.v_scale + at));
         } else {
-            k[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.c.k_pool) + from));
-            v[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.c.v_pool) + from));
+            k[i] = load(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.c.k_pool) + from));
+            v[i] = load(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.c.v_pool) + from));
         }
     }
 #pragma unroll
@@ -195,7 +195,7 @@ cache_expand_kernel(const ExpandArgs a) {
     for (int z0 = 0; z0 < a.Z; z0 += 256) {
         __syncthreads();
         if (z0 + int(threadIdx.x) < a.Z) {                 // (cut to the table first: the rounding up must not leave 31 bits)
-            const int rows = min(max(__ldg(a.lens + z0 + threadIdx.x), 0), a.c.width << a.c.page_shift);
+            const int rows = min(max(load(a.lens + z0 + threadIdx.x), 0), a.c.width << a.c.page_shift);
             pages[threadIdx.x] = (rows + ps - 1) >> a.c.page_shift;
         }
         __syncthreads();
@@ -206,22 +206,36 @@ cache_expand_kernel(const ExpandArgs a) {
             for (; skip < n; skip += gridDim.x) {
                 const int idx = int(skip / unsigned(a.H_kv)), h = int(skip - unsigned(idx) * unsigned(a.H_kv));
                 const size_t to_page = size_t(z) * a.c.width + idx;
-                const int page = __ldg(a.c.table + to_page);
+                const int page = load(a.c.table + to_page);
                 const bool bad = unsigned(page) >= unsigned(a.c.n_pages);        // its rows read as zeros: no page of the new pool either
                 if (h == 0 && threadIdx.x == 0) {
                     if (bad) report(a.status, FST_DEV_INDEX_RANGE, z, idx << a.c.page_shift);
                     a.table[to_page] = bad ? -1 : int(to_page);
                 }
                 if (bad) continue;
-#pragma unroll 2
-                for (int r = threadIdx.x / LPR; r < ps; r += RPB) {
-                    const int64_t from = page * a.c.stride_page + r * a.c.stride_row + h * a.c.stride_head + col;
-                    const size_t at = ((size_t(page) * a.H_kv + h) << a.c.page_shift) + r, to = (((to_page * a.H_kv + h) << a.c.page_shift) + r) * D + col;
-                    const uint2 bk = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.k_pool) + from));
-                    const uint2 bv = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.v_pool) + from));
-                    const float ek = e8m0_value(__ldg(a.c.k_scale + at)), ev = e8m0_value(__ldg(a.c.v_scale + at));
-                    *reinterpret_cast<uint4 *>(static_cast<T *>(a.k) + to) = expand8<T>(bk, ek);
-                    *reinterpret_cast<uint4 *>(static_cast<T *>(a.v) + to) = expand8<T>(bv, ev);
+#pragma unroll 1
+                for (int r0 = threadIdx.x / LPR; r0 < ps; r0 += 2 * RPB) {       // two rows on their way
+                    uint2 bk[2], bv[2];
+                    float ek[2], ev[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int r = r0 + i * RPB;
+                        if (r >= ps) continue;
+                        const int64_t from = page * a.c.stride_page + r * a.c.stride_row + h * a.c.stride_head + col;
+                        const size_t at = ((size_t(page) * a.H_kv + h) << a.c.page_shift) + r;
+                        bk[i] = load(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.k_pool) + from));
+                        bv[i] = load(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.c.v_pool) + from));
+                        ek[i] = e8m0_value(load(a.c.k_scale + at));
+                        ev[i] = e8m0_value(load(a.c.v_scale + at));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int r = r0 + i * RPB;
+                        if (r >= ps) continue;
+                        const size_t to = (((to_page * a.H_kv + h) << a.c.page_shift) + r) * D + col;
+                        *reinterpret_cast<uint4 *>(static_cast<T *>(a.k) + to) = expand8<T>(bk[i], ek[i]);
+                        *reinterpret_cast<uint4 *>(static_cast<T *>(a.v) + to) = expand8<T>(bv[i], ev[i]);
+                    }
                 }
             }
             skip -= n;

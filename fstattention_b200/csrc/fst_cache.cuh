@@ -23,6 +23,14 @@ struct CacheArgs {
     int64_t stride_page, stride_row, stride_head;
 };
 
+// These kernels become resident while the launch ahead of them still writes their tables, lengths and rows, and wait for it before their first
+// access: loads for data that is read-only for a kernel's whole life (__ldg) would not have to see that.
+template <typename T>
+__device__ __forceinline__ T load(const T *p) {
+    __builtin_assume(__isGlobal(p));
+    return *p;
+}
+
 // e of a row whose largest magnitude is a (finite)
 __device__ __forceinline__ int e4m3_exponent(float a) {
     const uint32_t bits = __float_as_uint(a);

@@ -64,10 +64,10 @@ struct ChunkLine {
     __device__ __forceinline__ explicit ChunkLine(const ChunkArgs &args) : a(args) {}
 
     __device__ __forceinline__ int kv_len(int z) const {
-        const int n = __ldg(a.kv_lens + z), most = a.c.width << a.c.page_shift;
+        const int n = load(a.kv_lens + z), most = a.c.width << a.c.page_shift;
         return min(max(n, 0), most);
     }
-    __device__ __forceinline__ int q_len(int z) const { return a.q_lens == nullptr ? a.n_q : min(max(__ldg(a.q_lens + z), 0), a.n_q); }
+    __device__ __forceinline__ int q_len(int z) const { return a.q_lens == nullptr ? a.n_q : min(max(load(a.q_lens + z), 0), a.n_q); }
     __device__ __forceinline__ int row_tiles(int ql) const { return (ql * a.group + ROWS - 1) / ROWS; }
     // keys that the last row of a row tile sees
     __device__ __forceinline__ int keys(int kv, int ql, int qt) const {
@@ -289,10 +289,10 @@ __device__ __forceinline__ void add_not_finite(const ChunkArgs &a, int z, int h,
 #pragma unroll 1
     for (int key = from; key < to; ++key) {
         const int idx = key >> a.c.page_shift, off = key & ((1 << a.c.page_shift) - 1);
-        const int page = __ldg(a.c.table + size_t(z) * a.c.width + idx);
+        const int page = load(a.c.table + size_t(z) * a.c.width + idx);
         if (unsigned(page) >= unsigned(a.c.n_pages)) continue;
         if constexpr (QUANT) {
-            const bool odd = __ldg(a.c.v_scale + ((size_t(page) * a.H_kv + h) << a.c.page_shift) + off) == 255;
+            const bool odd = load(a.c.v_scale + ((size_t(page) * a.H_kv + h) << a.c.page_shift) + off) == 255;
 #pragma unroll
             for (int k = 0; k < N; ++k) out[k] = odd ? NAN : out[k];
         } else {

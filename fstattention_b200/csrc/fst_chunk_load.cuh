@@ -59,7 +59,7 @@ __device__ __forceinline__ void load_tiles(const ChunkArgs &a, const Line &line,
     bool alive = true;
     auto look_up = [&]() {
         const int key = me.tile * G::KEYS + lane * ps;
-        page = lane * ps < G::KEYS && key < me.keys ? __ldg(a.c.table + size_t(me.z) * a.c.width + (key >> a.c.page_shift)) : 0;
+        page = lane * ps < G::KEYS && key < me.keys ? load(a.c.table + size_t(me.z) * a.c.width + (key >> a.c.page_shift)) : 0;
     };
     look_up();
 #pragma unroll 1

@@ -113,8 +113,8 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
 #pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
         if (i == 0 || me.tile == 0) {                     // a new item: its rows of Q
-            if (tid == 0 && me.h == 0 && me.qt == 0 && (me.kv != __ldg(a.kv_lens + me.z) || (a.q_lens != nullptr && me.ql != __ldg(a.q_lens + me.z))))
-                report(a.status, FST_DEV_INDEX_RANGE, me.z, __ldg(a.kv_lens + me.z));
+            if (tid == 0 && me.h == 0 && me.qt == 0 && (me.kv != load(a.kv_lens + me.z) || (a.q_lens != nullptr && me.ql != load(a.q_lens + me.z))))
+                report(a.status, FST_DEV_INDEX_RANGE, me.z, load(a.kv_lens + me.z));
             poisoned = false;
             lim_first = a.causal ? min(me.kv, me.kv - me.ql + by_group(a, me.qt * G::ROWS) + 1) : me.kv;
 #pragma unroll
@@ -135,7 +135,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                             uint32_t top = 0;
 #pragma unroll
                             for (int s2 = 0; s2 < KS / 2; ++s2) {
-                                const uint4 w = real ? __ldg(reinterpret_cast<const uint4 *>(src + t * (D / 4) + s2 * 8)) : make_uint4(0, 0, 0, 0);
+                                const uint4 w = real ? load(reinterpret_cast<const uint4 *>(src + t * (D / 4) + s2 * 8)) : make_uint4(0, 0, 0, 0);
                                 top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
                             }
                             top = max(top & 0xffffu, top >> 16);
@@ -147,7 +147,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         row_c2[x][hh] = c2 / by;
                     }
                     auto two_steps = [&](int s2, uint32_t (&f)[4]) {         // steps 2 s2 and 2 s2 + 1: D / 4 contiguous values
-                        const uint4 w = real ? __ldg(reinterpret_cast<const uint4 *>(src + t * (D / 4) + s2 * 8)) : make_uint4(0, 0, 0, 0);
+                        const uint4 w = real ? load(reinterpret_cast<const uint4 *>(src + t * (D / 4) + s2 * 8)) : make_uint4(0, 0, 0, 0);
                         f[0] = w.x; f[1] = w.y; f[2] = w.z; f[3] = w.w;
                         if constexpr (BF16) {
 #pragma unroll
@@ -155,8 +155,8 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         }
                     };
                     auto one_step = [&](int st, uint32_t &lo, uint32_t &hi) {
-                        lo = real ? __ldg(reinterpret_cast<const uint32_t *>(src + st * 16 + 2 * t)) : 0u;
-                        hi = real ? __ldg(reinterpret_cast<const uint32_t *>(src + st * 16 + 8 + 2 * t)) : 0u;
+                        lo = real ? load(reinterpret_cast<const uint32_t *>(src + st * 16 + 2 * t)) : 0u;
+                        hi = real ? load(reinterpret_cast<const uint32_t *>(src + st * 16 + 8 + 2 * t)) : 0u;
                     };
                     if constexpr (G::Q_SHARED) {          // every warp brings a step (KS = 8 warps)
                         uint32_t lo, hi;

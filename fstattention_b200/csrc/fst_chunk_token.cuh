@@ -98,8 +98,8 @@ chunk_token_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, 
 #pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
         if (i == 0 || me.tile == 0) {                     // a new item
-            if (tid == 0 && me.h == 0 && me.qt == 0 && (me.kv != __ldg(a.kv_lens + me.z) || (a.q_lens != nullptr && me.ql != __ldg(a.q_lens + me.z))))
-                report(a.status, FST_DEV_INDEX_RANGE, me.z, __ldg(a.kv_lens + me.z));
+            if (tid == 0 && me.h == 0 && me.qt == 0 && (me.kv != load(a.kv_lens + me.z) || (a.q_lens != nullptr && me.ql != load(a.q_lens + me.z))))
+                report(a.status, FST_DEV_INDEX_RANGE, me.z, load(a.kv_lens + me.z));
             poisoned = false;
             lim_first = a.causal ? min(me.kv, me.kv - me.ql + by_group(a, me.qt * G::ROWS) + 1) : me.kv;
 #pragma unroll
@@ -122,7 +122,7 @@ chunk_token_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, 
                 uint32_t top = 0;
 #pragma unroll
                 for (int s2 = 0; s2 < KS / 2; ++s2) {
-                    w[s2] = real ? __ldg(reinterpret_cast<const uint4 *>(src + t * (D / 4) + s2 * 8)) : make_uint4(0, 0, 0, 0);
+                    w[s2] = real ? load(reinterpret_cast<const uint4 *>(src + t * (D / 4) + s2 * 8)) : make_uint4(0, 0, 0, 0);
                     top = __vmaxu2(top, __vmaxu2(__vmaxu2(w[s2].x & 0x7fff7fffu, w[s2].y & 0x7fff7fffu), __vmaxu2(w[s2].z & 0x7fff7fffu, w[s2].w & 0x7fff7fffu)));
                 }
                 float by = 1.f;                           // the row's factor: its largest magnitude's exponent to 14
@@ -150,7 +150,7 @@ chunk_token_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, 
 #pragma unroll
                 for (int st = 0; st < KS; ++st)
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) qf[st][k] = real ? __ldg(reinterpret_cast<const uint32_t *>(src + st * 16 + k * 8 + 2 * t)) : 0u;
+                    for (int k = 0; k < 2; ++k) qf[st][k] = real ? load(reinterpret_cast<const uint32_t *>(src + st * 16 + k * 8 + 2 * t)) : 0u;
             }
         }
 

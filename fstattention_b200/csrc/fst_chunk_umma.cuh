@@ -212,7 +212,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
             const int idx = me.tile * npt + lane;
             page = 0;
             if (lane < npt && idx * ps < me.keys)
-                page = __ldg(a.c.table + size_t(me.z) * a.c.width + idx);
+                page = load(a.c.table + size_t(me.z) * a.c.width + idx);
         };
         // The plan of a tile goes into the word of its K's stage: 16-key steps with keys in them (bits 0-3), and of either group whether it
         // takes part (4, 5), whether the tile is its piece's first (6, 7) or last (8, 9), which buffer holds Q (10); 0: no more tiles.
@@ -398,8 +398,8 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
 #pragma unroll 1
         for (int i = 0; i < n_tiles; i += len, ++item) {
             len = min(me.tiles - me.tile, n_tiles - i);
-            if (t64 == 0 && me.h == 0 && me.qt == 0 && (me.kv != __ldg(a.kv_lens + me.z) || (a.q_lens != nullptr && me.ql != __ldg(a.q_lens + me.z))))
-                report(a.status, FST_DEV_INDEX_RANGE, me.z, __ldg(a.kv_lens + me.z));
+            if (t64 == 0 && me.h == 0 && me.qt == 0 && (me.kv != load(a.kv_lens + me.z) || (a.q_lens != nullptr && me.ql != load(a.q_lens + me.z))))
+                report(a.status, FST_DEV_INDEX_RANGE, me.z, load(a.kv_lens + me.z));
 #pragma unroll 1
             for (int g = 0; g < 2; ++g) {
                 if (group_tiles(g) <= me.tile) continue;      // (a piece may begin behind the first group's last tile)

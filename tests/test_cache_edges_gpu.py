@@ -7,7 +7,7 @@ import torch
 
 import fstattention_b200 as fst
 from oracle import cache_oracle as orc
-from test_cache_gpu import append, check, chunk, clean, int32, new_cache
+from test_cache_gpu import append, check, chunk, clean, int32, new_cache, read
 
 pytestmark = pytest.mark.gpu
 
@@ -173,4 +173,41 @@ def test_the_smallest_scale_byte_means_the_same_to_every_kernel(N, D):
     cache = list(new_cache(gen, lens, 2, D, 32, "NHD", torch.bfloat16, True))
     cache[3].view(torch.uint8).zero_()
     check(*chunk(q, cache, int32(lens), D ** -0.5, return_lse=True), orc.attention(q, cache, lens, D ** -0.5), True, 700)
+    clean()
+
+
+# ---- calls that read what the launch ahead of them writes ---------------------------------------------------
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("N", [1, 12, 40])
+def test_a_chain_of_calls_without_a_pause(N, quantised):
+    """Rows, lengths, tables and results that the kernel just ahead writes: each call starts early and still sees them."""
+    gen = torch.Generator().manual_seed(N)
+    Z, H, D, steps = 4, 2, 64, 12
+    base = new_cache(gen, [steps * N + N] * Z, H, D, 16, "NHD", torch.bfloat16, quantised)
+    q0 = torch.randn((Z, H, N, D), generator=gen).to(torch.bfloat16).cuda()
+
+    def run(pause):
+        cache = [t.clone() if torch.is_tensor(t) else t for t in base]
+        start, kv, x = int32([0] * Z), int32([0] * Z), q0.clone()
+        outs, first = [], cache[2].clone()
+        for i in range(steps):
+            cache[2].copy_(first.roll(1, 0))              # another table, and this one again
+            cache[2].copy_(first)
+            kv.add_(N)
+            pause()
+            append(x, x, cache, start)                    # x: what the attention ahead has written
+            pause()
+            x = chunk(x, cache, kv, D ** -0.5)
+            pause()
+            k, v = read(cache, kv, steps * N)
+            pause()
+            x = x + k[:, :, i * N:i * N + N] * 0.5        # (of a length that is known here)
+            start.add_(N)
+            outs += [x, k, v]
+        return outs
+
+    want = run(torch.cuda.synchronize)
+    for _ in range(5):
+        for a, b in zip(run(lambda: None), want):
+            assert torch.equal(a, b)
     clean()
