@@ -259,8 +259,10 @@ struct ChunkCut {
 };
 
 // Probabilities that are rounded to fp16 for the second product are taken 2^15 times too large (against a reference that is 15 below
-// the maximum), so that they fill its range: at most 2^15, and what lies 2^24 below that is lost.  At most 1 they would lose
-// what lies 2^24 below the largest one, which many keys together can make the larger part of the result.
+// the maximum), so that they fill its range: at most 2^15, and those below 2^-14 are rounded to steps of 2^-24, by 2^-40 of the largest one.  At
+// most 1 they would lose what lies 2^24 below the largest one, which many keys together can make the larger part of the result.  Where the
+// reference may lag by 2^8 (chunk_umma_kernel) the factor is 2^7 and that step's half 2^-32 of the largest: equal probabilities of
+// 2^-25.5 of it all become 45 steps where they are 45.25, and what 60000 of them make of a result comes out half a percent low.
 constexpr float kLift = 15.f;
 
 // ---- values that are not finite where not every row of a tile attends to them.  The second product multiplies a masked

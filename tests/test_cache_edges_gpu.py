@@ -2,6 +2,8 @@
 
 Tolerances are those of ``test_cache_gpu.py`` where a test does not derive its own.
 """
+import math
+
 import pytest
 import torch
 
@@ -211,3 +213,41 @@ def test_a_chain_of_calls_without_a_pause(N, quantised):
         for a, b in zip(run(lambda: None), want):
             assert torch.equal(a, b)
     clean()
+
+
+# ---- what small probabilities lose ----------------------------------------------------------------------------
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("N", [1, 5, 12, 60])
+def test_small_probabilities_lose_no_more_than_their_step(N, dtype, quantised):
+    """One key whose value is zero has nearly all of the weight, the 60000 others 2^-25.5 of it each (2^-26 over 8 bits) and the value one.
+
+    The second product's probabilities are fp16 (bf16 for bf16 queries over 16 bits or of more than 32 rows of a head).  Rounding costs each
+    eps / 2 of itself, or half of fp16's smallest step, 2^-24: of the largest weight that is 2^-40, and 2^-32 on tcgen05 (more than 32
+    rows), where weights are 2^15 and 2^7 times too large.  Sums of 16 keys go into fp32 accumulators, two roundings each at the most."""
+    T, H, D = 60000, 2, 64
+    gen = torch.Generator().manual_seed(N)
+    cache = list(new_cache(gen, [T + N], 1, D, 64, "NHD", dtype, False))
+    cache[0].zero_()
+    cache[1].fill_(1.0)
+    page, off = orc.row_of(cache, 0, torch.tensor([777], device="cuda"))
+    cache[0][page, off, :, 5] = 51.0
+    cache[1][page, off] = 0.0
+    if quantised:
+        for which in range(2):
+            values, e, _ = orc.quantise(cache[which])
+            cache[which], cache[3 + which] = values.to(torch.float8_e4m3fn), (e + 127).to(torch.uint8).transpose(1, 2).contiguous().view(torch.float8_e8m0fnu)
+    q = torch.zeros((1, H, N, D), dtype=dtype, device="cuda")
+    q[..., 5] = 1.0
+    out = chunk(q, cache, int32([T + N]), math.log(2) / 2, causal=False)
+    clean()
+    want, _, mag, size = orc.attention(q, cache, [T + N], math.log(2) / 2, causal=False)
+    tcgen05 = N * H > 32
+    in_bf16 = dtype == torch.bfloat16 and (tcgen05 or not quantised)
+    p_eps = torch.finfo(torch.bfloat16 if in_bf16 else torch.float16).eps
+    share = 2.0 ** -23 * (D + 3) * size[..., None] + 2.0 ** -18
+    tol = want * torch.finfo(dtype).eps / 2 + mag * (p_eps / 2 + 2 * share + 2 * 2.0 ** -23 * (T / 8 + 64)) + 2.0 ** -25
+    if not in_bf16:
+        tol = tol + (T + N) * 2.0 ** -(32 if tcgen05 else 40)
+    worst = float(((out.double() - want).abs() - tol).max())
+    assert worst <= 0, (worst, float(want.max()), float(out.double().max()))
