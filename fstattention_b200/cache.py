@@ -14,7 +14,7 @@ float8_e8m0fnu ``[n_pages, H_kv, page_size]``, hold a power of two for every row
 
 All calls are asynchronous on torch's current stream and can be captured into a graph; lengths and tables are read
 on the GPU.  What only the GPU can see (a page number outside the pool, a length past the table) is
-recorded for ``last_status`` and never faults.  (A length is not looked at where a sequence has no queries.)  What an
+recorded for ``last_status`` and never faults.  (Length and pages are not looked at where a sequence has no queries.)  What an
 8-bit cache holds is what ``fst_cache_append`` wrote or zeros: e4m3's NaN bytes do not occur.
 """
 from __future__ import annotations

@@ -564,7 +564,7 @@ int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cach
     if (chunk_expands(a, head_dim)) {
         unsigned char *at = static_cast<unsigned char *>(workspace) + (splits ? align256(chunk_part_bytes(n_ctas, chunk_row_tile(a), head_dim)) : 0);
         const size_t pool = size_t(chunk_expanded_bytes(a, head_dim)) / 2;
-        const ExpandArgs x{a.c, at, at + pool, reinterpret_cast<int32_t *>(at + 2 * pool), kv_lens, Z, H_kv, status};
+        const ExpandArgs x{a.c, at, at + pool, reinterpret_cast<int32_t *>(at + 2 * pool), kv_lens, q_lens, Z, H_kv, status};
         const cudaError_t e = launch_cache_expand(x, dtype, head_dim, st);
         if (e != cudaSuccess) return cuda_status(e);
         a.c.k_pool = x.k; a.c.v_pool = x.v; a.c.k_scale = a.c.v_scale = nullptr;

@@ -196,7 +196,8 @@ cache_expand_kernel(const ExpandArgs a) {
         __syncthreads();
         if (z0 + int(threadIdx.x) < a.Z) {                 // (cut to the table first: the rounding up must not leave 31 bits)
             const int rows = min(max(load(a.lens + z0 + threadIdx.x), 0), a.c.width << a.c.page_shift);
-            pages[threadIdx.x] = (rows + ps - 1) >> a.c.page_shift;
+            const bool idle = a.q_lens != nullptr && load(a.q_lens + z0 + threadIdx.x) <= 0;
+            pages[threadIdx.x] = idle ? 0 : (rows + ps - 1) >> a.c.page_shift;
         }
         __syncthreads();
 #pragma unroll 1

@@ -97,7 +97,7 @@ struct ExpandArgs {
     CacheArgs c;
     void *k, *v;
     int32_t *table;
-    const int32_t *lens;
+    const int32_t *lens, *q_lens;          // [Z], [Z] or null: a sequence without queries has no rows
     int Z, H_kv;
     int32_t *status;
 };

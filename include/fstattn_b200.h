@@ -384,7 +384,7 @@ int fst_cache_read(const fst_paged_cache *cache, void *k, void *v, const int32_t
  * workspace: fst_attention_chunk_workspace_bytes() bytes (for the current device), 256-byte aligned, scratch of this call
  * alone; what is in it before does not matter.  May be NULL where that is 0.
  * A length that is negative or past the table (or n_q) is cut and sets FST_DEV_INDEX_RANGE (that of a sequence that has
- * no queries after the cut may go unreported); a page number outside [0, n_pages) reads as zeros and sets it too.
+ * no queries after the cut may go unreported, and its pages are not looked at); a page number outside [0, n_pages) reads as zeros and sets it too.
  * (Waits inside the kernels end after some four seconds, with FST_DEV_TIMEOUT: enough for sequences of 3e8 rows.)
  */
 size_t fst_attention_chunk_workspace_bytes(const fst_paged_cache *cache, int Z, int H, int H_kv, int n_q, int head_dim);

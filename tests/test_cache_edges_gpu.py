@@ -56,6 +56,36 @@ def test_lengths_up_to_the_largest_are_cut(length, page):
         assert fst.last_status(clear=True) == 18
 
 
+# ---- sequences without queries --------------------------------------------------------------------------------
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("N,H", [(1, 4), (12, 4), (100, 4), (520, 8)])
+def test_a_sequence_without_queries_is_not_looked_at(N, H, quantised):
+    """One whose pages have been taken away and whose length nobody has reset: nothing is reported, the others are as they are without it."""
+    gen = torch.Generator().manual_seed(N)
+    lens = [600, 700, 530]
+    cache = new_cache(gen, lens, 2, 64, 16, "NHD", torch.bfloat16, quantised)
+    q = torch.randn((3, H, N, 64), generator=gen).to(torch.bfloat16).cuda()
+    want = chunk(q, cache, int32([600, 0, 530]), 0.125, q_lens=int32([N, 0, N]))
+    cache[2][1] = -1
+    for idle in (0, -3):
+        got = chunk(q, cache, int32(lens), 0.125, q_lens=int32([N, idle, N]))
+        clean()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompts_and_tokens_in_one_call(dtype):
+    """A chunk of 520 tokens by 4 heads beside single tokens and an idle sequence: over 8 bits all of them go through the expanded copy."""
+    gen = torch.Generator().manual_seed(31)
+    lens, q_lens, H, H_kv, D = [900, 3000, 1, 2049, 77, 640], [520, 1, 1, 1, 0, 1], 8, 2, 128
+    for quantised in (False, True):
+        cache = new_cache(gen, lens, H_kv, D, 64, "NHD", dtype, quantised)
+        q = torch.randn((6, H, 520, D), generator=gen).to(dtype).cuda()
+        out, lse = chunk(q, cache, int32(lens), D ** -0.5, q_lens=int32(q_lens), return_lse=True)
+        clean()
+        check(out, lse, orc.attention(q, cache, lens, D ** -0.5, q_lens), quantised, 3000)
+
+
 # ---- scales of V over all of their range ---------------------------------------------------------------------
 def with_v_exponents(cache, low, high, gen):
     """The same cache with every V row's exponent drawn from [low, high]."""
