@@ -452,7 +452,8 @@ constexpr long long kExpandRows = 2048;
 constexpr long long kMostExpanded = 2LL << 30;
 inline long long chunk_expanded_bytes(const ChunkArgs &a, int D) { return 4LL * a.Z * a.c.width * a.H_kv * D << a.c.page_shift; }
 inline bool chunk_expands(const ChunkArgs &a, int D) {
-    return a.c.k_scale != nullptr && (long long)a.n_q * a.group >= kExpandRows && (long long)a.Z * a.c.width < 0x7fffffffLL && chunk_expanded_bytes(a, D) <= kMostExpanded;
+    const long long pages = (long long)a.Z * a.c.width;   // (times the heads it is below 2^62, times the bytes of a page it need not be)
+    return a.c.k_scale != nullptr && (long long)a.n_q * a.group >= kExpandRows && pages < 0x7fffffffLL && pages * a.H_kv <= kMostExpanded / (4LL * D << a.c.page_shift);
 }
 // Whether any piece can be less than an item: not if all that the table can hold is one key tile.
 inline bool chunk_splits(const ChunkArgs &a, int keys) { return ((long long)a.c.width << a.c.page_shift) > keys; }
