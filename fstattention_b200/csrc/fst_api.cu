@@ -538,7 +538,8 @@ int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cach
                         float sm_scale, int causal, int dtype, void *workspace, size_t workspace_bytes, int32_t *status, void *stream) {
     ChunkArgs a = {};
     if (!q || !o || !kv_lens || Z <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || n_q <= 0) return FST_ERR_INVALID_ARG;
-    if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return FST_ERR_INVALID_ARG;
+    const float scale_log2 = sm_scale * 1.4426950408889634f;
+    if (!(sm_scale > 0.f) || !std::isfinite(scale_log2)) return FST_ERR_INVALID_ARG;
     const int rc = open_cache(a.c, cache, head_dim, dtype);
     if (rc != FST_OK) return rc;
     if ((long long)n_q * (H / H_kv) > 0x7fffffffLL - 1024) return FST_ERR_TOO_LARGE;
@@ -553,7 +554,7 @@ int fst_attention_chunk(const void *q, void *o, float *lse, const fst_paged_cach
     set_group(a, H / H_kv);
     a.qs_z = q_stride_z; a.qs_h = q_stride_h; a.qs_n = q_stride_n;
     a.os_z = o_stride_z; a.os_h = o_stride_h; a.os_n = o_stride_n;
-    a.scale_log2 = sm_scale * 1.4426950408889634f;
+    a.scale_log2 = scale_log2;
     a.causal = causal != 0;
     const int n_ctas = chunk_ctas();
     set_ctas(a, n_ctas);

@@ -583,7 +583,7 @@ PyObject *attention_chunk(PyObject *const *a, Py_ssize_t n) {
     if (c.D != cache.D || c.H_kv < 1 || c.H < 1 || c.H % c.H_kv) raise(PyExc_ValueError, "q must have the cache's head dimension and a multiple of its heads");
     if (c.Z > INT_MAX || c.H > INT_MAX || c.n_q > INT_MAX) raise(PyExc_ValueError, "q is too large");
     const double s = real(a[10]);
-    if (!std::isfinite(s) || !(float(s) > 0.f)) raise(PyExc_ValueError, "sm_scale must be positive and finite");
+    if (!std::isfinite(float(s) * 1.4426950408889634f) || !(float(s) > 0.f)) raise(PyExc_ValueError, "sm_scale must be positive and finite, in base 2 too");
     c.scale = float(s);
     head_contiguous(c.q);
     const c10::cuda::CUDAGuard guard(dev);

@@ -12,3 +12,11 @@ def test_an_expansion_whose_size_does_not_fit_is_not_made(built_lib):
     for stride, Z, heads in ((1 << 20, 1 << 10, 1 << 24), (1 << 20, 2000, (1 << 31) - 1), (1 << 20, 1 << 10, 1 << 23)):
         c = cache(table_stride=stride, k_scale=P(512), v_scale=P(1024))
         assert size(C.byref(c), Z, heads, heads, 2048, 64) == few
+
+
+def test_a_factor_that_overflows_in_base_two_is_refused(built_lib):
+    """sm_scale * log2(e) has to be finite too."""
+    from fstattention_b200 import _lib
+    lib = _lib.lib()
+    for scale in (2.4e38, 3.4e38):
+        assert lib.fst_attention_chunk(*chunk_args(cache(), scale=scale)) == INVALID
