@@ -391,7 +391,10 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
         }
     } else if (warp == 10 || warp == 11) {
         // ====== rows of Q, an item (D 128) or two ahead of its products' end: one box where whole tokens fit a tile (3 us sooner) ======
+        // With boxes this is warp 10's role, which waits for a buffer as a whole before it fills that.  (Threads that wait and hold up no fill by it may
+        // miss a phase and the one behind it; then they wait for a third, which need not come.)
         const int t64 = tid - 320;
+        if (!a.q_boxes || warp == 10) {
         uint32_t qfree_ph = 0, used = 0;                  // bit: buffer and group
         bool alive = true;
         int item = 0, len;
@@ -405,7 +408,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
                 if (group_tiles(g) <= me.tile) continue;      // (a piece may begin behind the first group's last tile)
                 const int at = (QBUF == 1 ? 0 : (item & 1) * 2) + g;
                 if (used >> at & 1) {                 // the products that read what is there
-                    if (alive) alive = wait_for(bar_qfree + at * 8, qfree_ph >> at & 1);
+                    if (alive) alive = __all_sync(0xffffffffu, wait_for(bar_qfree + at * 8, qfree_ph >> at & 1));
                     qfree_ph ^= 1u << at;
                 }
                 used |= 1u << at;
@@ -439,6 +442,7 @@ chunk_umma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_q, c
             if (i + len < n_tiles) me.next(line);
         }
         if (!alive && lane == 0) gave_up();
+        }
     } else {
         const int t128 = tid - 384;
         bool alive = true;

@@ -281,3 +281,22 @@ def test_small_probabilities_lose_no_more_than_their_step(N, dtype, quantised):
         tol = tol + (T + N) * 2.0 ** -(32 if tcgen05 else 40)
     worst = float(((out.double() - want).abs() - tol).max())
     assert worst <= 0, (worst, float(want.max()), float(out.double().max()))
+
+
+# ---- many short items ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Z,H,H_kv,N,T", [(40, 8, 8, 300, 6), (64, 16, 8, 64, 100), (40, 10, 5, 1258, 17)])
+def test_many_short_items_of_many_rows(Z, H, H_kv, N, T, D):
+    """Items of one tile, some of rows that see nothing, one after the other: every wait ends, and every call gives the same."""
+    gen = torch.Generator().manual_seed(D)
+    lens = [int(x) for x in torch.randint(0, T + 1, (Z,), generator=gen)]
+    cache = new_cache(gen, [T] * Z, H_kv, D, 32, "HND", torch.bfloat16, False, extra=200)
+    q = torch.randn((Z, H, N, D), generator=gen).to(torch.bfloat16).cuda()
+    kv = int32(lens)
+    out, lse = chunk(q, cache, kv, D ** -0.5, return_lse=True)
+    check(out, lse, orc.attention(q, cache, lens, D ** -0.5), False, T)
+    clean()
+    for _ in range(200):
+        again = chunk(q, cache, kv, D ** -0.5)
+    clean()
+    assert torch.equal(again, out)
