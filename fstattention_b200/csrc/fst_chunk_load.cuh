@@ -21,13 +21,13 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
     return false;
 }
 
-// Sums of weights against m_w - kLift become sums against m when multiplied by `by` and `then`: halves of the factor, since 2^(m_w - kLift - m) itself
-// may be below what an exponential returns as a normal number (rows of V around 2^-110).
-__device__ __forceinline__ void weights_back(float m, float m_w, float &by, float &then) {
+// Sums of weights against m_w become sums against m when multiplied by `by` and `then`: halves of the factor, since 2^(m_w - m) itself may be below
+// what an exponential returns as a normal number (rows of V around 2^-110).  `unlift` takes back what the sums are too large by.
+__device__ __forceinline__ void weights_back(float m, float m_w, float unlift, float &by, float &then) {
     by = m == -INFINITY ? 1.f : fast_exp2(0.5f * (m_w - m));
-    then = by * (1.f / 32768.f);
-    static_assert(kLift == 15.f, "2^-kLift");
+    then = by * unlift;
 }
+static_assert(kLift == 15.f, "fp16 weights are 2^15 times too large");
 
 // two e4m3 bytes (the low ones, the high ones) -> a pair of fp16
 __device__ __forceinline__ uint32_t e4m3_halves(uint32_t w, bool high) {

@@ -7,10 +7,12 @@
 //
 // 8-bit rows become matrix fragments in registers, without their scales.  The order of the summed index is free as long as both operands
 // agree, so lane (g, t) of a K fragment takes the contiguous bytes D/4 t .. of key g, and Q is loaded in the same order; of V it
-// takes bytes D/8 g .. of its four keys, which only permutes the columns of the result.  K and V are fp16, by the conversion instruction.  A
+// takes bytes D/8 g .. of its four keys, which only permutes the columns of the result.  K is fp16, by the conversion instruction.  A
 // key's scale multiplies its score; bf16 queries become fp16 times a power of two per row, with the row's largest value next to 2^15:
 // what fp16 loses then is 2^-39 of that.  V's scales go into the exponents of weights of their own, as in chunk_token_kernel: no single
-// factor brings all of their range, 2^-117 to 2^119, through a 16-bit probability and an fp32 sum.
+// factor brings all of their range, 2^-117 to 2^119, through a 16-bit probability and an fp32 sum.  Under fp16 queries weights and V are fp16.  Under
+// bf16 queries they are bf16, whose range keeps rows of V apart that are more than 2^39 smaller than others: a byte's seven low bits
+// moved under bf16's exponent are its value * 2^-120, and weights are taken 2^120 times too large.
 //
 // 7 draft tokens of 4 heads behind 24 x 8 heads of 2300 e4m3 rows at D 64: 46 us (58 MB, 9 us of HBM): a fixed 20, of them 4 for the merge and as many for
 // the warps' meetings at every item's end, and 2.1 us a tile of 256 keys: some 1300 instructions a warp for it, most of them conversions and
@@ -38,16 +40,22 @@ struct ChunkMmaGeo {
     static constexpr int BYTES = OFF_BAR + 2 * STAGES * 8 + 1024;   // + alignment
 };
 
+// four e4m3 bytes -> two pairs of bf16 (bytes 0 and 2, bytes 1 and 3), smaller by 2^120
+__device__ __forceinline__ void e4m3_bits(uint32_t w, uint32_t &even, uint32_t &odd) {
+    odd = (w & 0x80008000u) | ((w >> 4) & 0x07f007f0u);
+    const uint32_t u = w << 8;
+    even = (u & 0x80008000u) | ((u >> 4) & 0x07f007f0u);
+}
 template <typename T, int D, bool QUANT, int MT>
 __global__ void __launch_bounds__(384, 1)
 chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
     using G = ChunkMmaGeo<D, QUANT, MT>;
     using MT_ = MmaTraits<T>;
-    using MP = MmaTraits<typename std::conditional<QUANT, __half, T>::type>;     // of the products
+    using MK = MmaTraits<typename std::conditional<QUANT, __half, T>::type>;     // of the first product
     using Line = ChunkLine<G::ROWS, G::KEYS, G::OVER>;
     using Cursor = ChunkCursor<G::ROWS, G::KEYS, G::OVER>;
     constexpr bool BF16 = !std::is_same<T, __half>::value;
-    constexpr float LIFT = !QUANT && !BF16 ? kLift : 0.f;
+    constexpr float LIFT = !QUANT && !BF16 ? kLift : 0.f, LIFT_W = BF16 ? 120.f : kLift;      // of probabilities, of weights
     constexpr int KS = D / 16, ND = D / 8;               // steps of the first product, column tiles of the second
     constexpr int KW = G::KW, NK = KW / 8, SUBS = KW / 16;
     constexpr int HALF_BYTES = G::KEYS * 128, SUB_BYTES = 16 * (QUANT ? D : 128);         // a tile's half of 64 columns of 16 bits, 16 rows in it
@@ -151,7 +159,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         f[0] = w.x; f[1] = w.y; f[2] = w.z; f[3] = w.w;
                         if constexpr (BF16) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) f[k] = MP::pack(__uint_as_float(f[k] << 16) * by, __uint_as_float(f[k] & 0xffff0000u) * by);
+                            for (int k = 0; k < 4; ++k) f[k] = MK::pack(__uint_as_float(f[k] << 16) * by, __uint_as_float(f[k] & 0xffff0000u) * by);
                         }
                     };
                     auto one_step = [&](int st, uint32_t &lo, uint32_t &hi) {
@@ -231,7 +239,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                             const uint32_t w = k == 0 ? b[n].x : k == 1 ? b[n].y : k == 2 ? b[n].z : b[n].w;
                             const uint32_t b0 = e4m3_halves(w, false), b1 = e4m3_halves(w, true);
 #pragma unroll
-                            for (int x = 0; x < MT; ++x) MP::mma(s[x][n], q[x], b0, b1);
+                            for (int x = 0; x < MT; ++x) MK::mma(s[x][n], q[x], b0, b1);
                         }
                     }
                 }
@@ -319,7 +327,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     };
                     move(m[x][hh], mx[x][hh], alpha[hh], LIFT);
                     alpha_w[hh] = alpha[hh];
-                    if constexpr (QUANT) move(m_w[x][hh], mw[x][hh], alpha_w[hh], kLift);
+                    if constexpr (QUANT) move(m_w[x][hh], mw[x][hh], alpha_w[hh], LIFT_W);
                 }
                 if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -346,8 +354,8 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         // (what a masked key holds, NaN too, stays out)
                         if constexpr (QUANT) p[k] = v == -INFINITY ? 0.f : fast_exp2(v + e_v[n][k & 1] - mw[x][k >> 1]);
                     }
-                    pf[x][n >> 1][(n & 1) * 2] = MP::pack(p[0], p[1]);
-                    pf[x][n >> 1][(n & 1) * 2 + 1] = MP::pack(p[2], p[3]);
+                    pf[x][n >> 1][(n & 1) * 2] = MT_::pack(p[0], p[1]);
+                    pf[x][n >> 1][(n & 1) * 2 + 1] = MT_::pack(p[2], p[3]);
                 }
             }
             // ---- second product
@@ -367,7 +375,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                             const uint2 b = lds64(v_at + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8);
                             w[k][0] = b.x; w[k][1] = b.y;
                         }
-                        if (edge && row >= here) {                    // zero times a NaN byte would be NaN
+                        if (!BF16 && edge && row >= here) {           // zero times a NaN byte would be NaN
 #pragma unroll
                             for (int c = 0; c < D / 32; ++c) w[k][c] = 0u;
                         }
@@ -376,12 +384,21 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     for (int c = 0; c < D / 32; ++c)
 #pragma unroll
                         for (int hl = 0; hl < 2; ++hl) {  // two column tiles from bytes 2 hl, 2 hl + 1 of either key
-                            const uint32_t y0 = __byte_perm(w[0][c], w[1][c], hl ? 0x7362 : 0x5140), y1 = __byte_perm(w[2][c], w[3][c], hl ? 0x7362 : 0x5140);
-                            const uint32_t b0[2] = {e4m3_halves(y0, false), e4m3_halves(y0, true)}, b1[2] = {e4m3_halves(y1, false), e4m3_halves(y1, true)};
+                            uint32_t b0[2], b1[2];
+                            if constexpr (BF16) {
+                                e4m3_bits(__byte_perm(w[0][c], w[1][c], hl ? 0x7632 : 0x5410), b0[0], b0[1]);
+                                e4m3_bits(__byte_perm(w[2][c], w[3][c], hl ? 0x7632 : 0x5410), b1[0], b1[1]);
+                            } else {
+                                const uint32_t y0 = __byte_perm(w[0][c], w[1][c], hl ? 0x7362 : 0x5140), y1 = __byte_perm(w[2][c], w[3][c], hl ? 0x7362 : 0x5140);
+                                b0[0] = e4m3_halves(y0, false);
+                                b0[1] = e4m3_halves(y0, true);
+                                b1[0] = e4m3_halves(y1, false);
+                                b1[1] = e4m3_halves(y1, true);
+                            }
 #pragma unroll
                             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                                for (int x = 0; x < MT; ++x) MP::mma(acc[x][c * 4 + hl * 2 + k], pf[x][sub], b0[k], b1[k]);
+                                for (int x = 0; x < MT; ++x) MT_::mma(acc[x][c * 4 + hl * 2 + k], pf[x][sub], b0[k], b1[k]);
                         }
                 } else {
                     const int row = (lane & 7) + ((lane >> 3) & 1) * 8;
@@ -396,8 +413,8 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                         }
 #pragma unroll
                         for (int x = 0; x < MT; ++x) {
-                            MP::mma(acc[x][2 * j], pf[x][sub], b[0], b[1]);
-                            MP::mma(acc[x][2 * j + 1], pf[x][sub], b[2], b[3]);
+                            MT_::mma(acc[x][2 * j], pf[x][sub], b[0], b[1]);
+                            MT_::mma(acc[x][2 * j + 1], pf[x][sub], b[2], b[3]);
                         }
                     }
                 }
@@ -436,7 +453,7 @@ chunk_mma_kernel(const ChunkArgs a, const __grid_constant__ CUtensorMap tm_k, co
                     float *to = rows + (warp * 16 + hh * 8 + g) * (D + 4);
                     if constexpr (QUANT) {                // weights back to the probabilities' reference
                         float by, then;
-                        weights_back(m[x][hh], m_w[x][hh], by, then);
+                        weights_back(m[x][hh], m_w[x][hh], BF16 ? 1.f : 1.f / 32768.f, by, then);
 #pragma unroll
                         for (int j = 0; j < ND; ++j)
 #pragma unroll

@@ -379,7 +379,8 @@ int fst_cache_read(const fst_paged_cache *cache, void *k, void *v, const int32_t
  * q_lens[z] positions: query i attends to rows [0, kv_lens[z] - q_lens[z] + i], or with causal = 0 to all kv_lens[z] rows.
  * o may be q.  A query that sees no row gets zeros (lse -inf).  Rows i >= q_lens[z] of o and lse are left as they are.  What the
  * cache holds at rows that a query does not attend to, NaN and infinities included, does not reach it.
- * Over an 8-bit cache fp16 queries take rows as fp16 where n_q H / H_kv > 32: values past 65504 saturate.
+ * Over an 8-bit cache fp16 queries take rows as fp16 where n_q H / H_kv > 32: values past 65504 saturate.  Where n_q H / H_kv <= 8, or <= 32 with
+ * fp16 queries, what a row of V adds is rounded by 2^-40 of the largest probability times scale.
  * lse, when not NULL, is [Z][H][n_q], base-2 log-sum-exp of the scaled scores.  sm_scale must be positive, sm_scale * log2(e) finite.
  * workspace: fst_attention_chunk_workspace_bytes() bytes (for the current device), 256-byte aligned, scratch of this call
  * alone; what is in it before does not matter.  May be NULL where that is 0.

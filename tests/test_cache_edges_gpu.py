@@ -147,6 +147,26 @@ def test_rows_of_v_of_the_smallest_scales(N, dtype):
     check_scaled(out, lse, want, 700, torch.finfo(torch.bfloat16).eps, 2.0 ** -134)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("N", [3, 4, 7, 8, 60])
+def test_small_rows_of_v_beside_a_row_of_another_size(N, D):
+    """A row 2^80 times as large as the others has one column: the others' columns are what they are without it (more than 8 rows of a head, bf16)."""
+    gen = torch.Generator().manual_seed(N + D)
+    lens = [700, 333]
+    cache = with_v_exponents(new_cache(gen, lens, 2, D, 32, "NHD", torch.bfloat16, True), -22, -18, gen)
+    for z in range(2):
+        page, off = orc.row_of(cache, z, torch.tensor([17], device="cuda"))
+        cache[1].view(torch.uint8)[page, off] = 0
+        cache[1].view(torch.uint8)[page, off, :, 0] = 0x7e
+        cache[4].view(torch.uint8)[page, :, off] = 127 + 60
+    q = torch.randn((2, 8, N, D), generator=gen).to(torch.bfloat16).cuda()
+    out, lse = chunk(q, cache, int32(lens), D ** -0.5, return_lse=True)
+    clean()
+    want = orc.attention(q, cache, lens, D ** -0.5)
+    assert (want[0][..., 0] > 2.0 ** 50).all() and (want[0][..., 1:].abs() < 1).all()
+    check_scaled(out, lse, want, 700, torch.finfo(torch.bfloat16).eps, 2.0 ** -134)
+
+
 # ---- counts that a call does not have ------------------------------------------------------------------------
 @pytest.mark.parametrize("quantised", [False, True])
 @pytest.mark.parametrize("path", [False, True])
