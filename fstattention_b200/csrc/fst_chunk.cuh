@@ -436,9 +436,9 @@ cudaError_t launch_chunk_combine(const ChunkArgs &a, int n_ctas, cudaStream_t st
 // CTAs of a call's line: one per SM (a workspace holds two pieces for each).
 inline int chunk_ctas() { return std::max(sm_count(), 2); }
 // Which kernel: up to 32 rows those on mma.sync, which read a key for little more than its bytes; up to 8 the one that has them as columns.  Measured
-// with 8 sequences of 16000 rows, us at bf16 D 128 / e4m3 D 128 / fp16 D 64 / e4m3 D 64: 24 rows on mma.sync 100 / 93 / 59 / 75, on
-// tcgen05 105 / 128 / 92 / 101; 36 rows on tcgen05 106 / 130 / 92 / 102, in two tiles on mma.sync 177 / 164 / 100 / 134; 8 rows
-// as columns 86 / 55 / 53 / 42, as a tile of 16 rows 88 / 62 / 53 / 48.
+// with 8 sequences of 16000 rows, us at bf16 D 128 / e4m3 D 128 / fp16 D 64 / e4m3 D 64: 24 rows on mma.sync 102 / 109 / 58 / 73, on
+// tcgen05 105 / 128 / 92 / 101; 36 rows on tcgen05 106 / 130 / 93 / 99, in two tiles on mma.sync 177 / 164 (before bf16 weights had exponents
+// of their own) / 100 / 134; 8 rows as columns 86 / 54 / 53 / 43, as a tile of 16 rows 88 / 62 / 53 / 48.
 inline bool chunk_many_rows(const ChunkArgs &a) { return (long long)a.n_q * a.group > 32; }
 inline int chunk_row_tile(const ChunkArgs &a) {
     const long long rows = (long long)a.n_q * a.group;
@@ -446,8 +446,8 @@ inline int chunk_row_tile(const ChunkArgs &a) {
 }
 // An 8-bit cache under many queries is expanded once, ahead of the call, rather than by every row tile on its way, but only as long as the copy
 // of all that the tables can hold stays below 2 GB.  What it costs goes with the keys, what it saves with keys and rows, so rows decide:
-// 8 heads, D 128 / 64, expanded and on the way, us: 512 rows over 16384 71 and 55 / 51 and 44; 2048 rows over 16384 145 and 148 / 120
-// and 120; 8192 rows over 8192 218 and 251 / 190 and 201.
+// 8 heads, D 128 / 64, expanded and on the way, us: 512 rows over 16384 71 and 55 / 51 and 44; 2048 rows over 16384 146 and 148 / 123
+// and 120; 8192 rows over 8192 220 and 251 / 196 and 201.  (The rows are those of n_q: a call of a prompt and 63 single tokens expands all 64.)
 constexpr long long kExpandRows = 2048;
 constexpr long long kMostExpanded = 2LL << 30;
 inline long long chunk_expanded_bytes(const ChunkArgs &a, int D) { return 4LL * a.Z * a.c.width * a.H_kv * D << a.c.page_shift; }

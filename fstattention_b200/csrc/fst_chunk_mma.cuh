@@ -14,7 +14,7 @@
 // bf16 queries they are bf16, whose range keeps rows of V apart that are more than 2^39 smaller than others: a byte's seven low bits
 // moved under bf16's exponent are its value * 2^-120, and weights are taken 2^120 times too large.
 //
-// 7 draft tokens of 4 heads behind 24 x 8 heads of 2300 e4m3 rows at D 64: 46 us (58 MB, 9 us of HBM): a fixed 20, of them 4 for the merge and as many for
+// 7 draft tokens of 4 heads behind 24 x 8 heads of 2300 e4m3 rows at D 64: 45 us (58 MB, 9 us of HBM): a fixed 20, of them 4 for the merge and as many for
 // the warps' meetings at every item's end, and 2.1 us a tile of 256 keys: some 1300 instructions a warp for it, most of them conversions and
 // the softmax, from two warps to a scheduler.
 #pragma once

@@ -12,8 +12,8 @@
 // adds is rounded by 2^-40 of what the largest scale times its probability stands for, which shows where that row has zeros.
 // bf16 queries become fp16 as in chunk_mma_kernel.
 //
-// Two sequences of 115000 e4m3 rows under 8 rows: 87 us where heads lie inside rows (5.4 TB/s; a copy has 6.55), 80 where a head's rows lie
-// together; chunk_mma_kernel took 108 when this took 101.  64 sequences of 4500 bf16 rows: 183 us, 6.6 TB/s.  What bounds it: HBM in 16 bits; in 8 bits
+// Two sequences of 115000 e4m3 rows under 8 rows: 89 us where heads lie inside rows (5.3 TB/s; a copy has 6.55), 81 where a head's rows lie
+// together; chunk_mma_kernel took 108 when this took 101.  64 sequences of 4500 bf16 rows: 185 us, 6.5 TB/s.  What bounds it: HBM in 16 bits; in 8 bits
 // requests of 128 bytes, and the chain of a warp's dependent instructions (two warps to a scheduler issue in 37 % of the cycles; 12 or 16 warps were
 // slower, so were half tiles in more stages: 117 us, and a reference for the maximum that moves less often made no difference).
 #pragma once

@@ -11,12 +11,13 @@
 // instruction cache holds, so what runs in turn is kept small (one copy of the issuing code for both groups and short waits: 4096 tokens over 16400
 // rows of 8 heads 929 -> 776 us, four prompts of 1024 tokens at D 64 69.5 -> 58.5).  The first is 1.05 - 1.25 PFLOP/s, as the power limit
 // lets clocks be; the second has 3.5 items of 2 to 8 tiles a CTA, and their starts and ends are half of it.
+// ptxas spills 432 bytes a thread in every instance, the softmax's most likely: its 128 scores, packed halves and sums.
 // Tried and not kept: an issuing lane per group (263 -> 299 us at D 128: the groups fall into step; nothing at D 64, with S of the next tile
 // ahead), 4 or 8 of 32 exponentials by a polynomial (0 to 4 %, slower for short items), two threads a row, steps of 64 keys, no exponentials for
 // the parts of a tile that a warp does not see (branches among them: 56.7 -> 59.4 us for the prompts).
 //
 // Sixteen warps: 0-3 and 4-7 are the softmax groups; 8 loads K and V, lane j page j of a tile; one lane of 9 issues the products;
-// 10 and 11 bring the items' rows of Q; 12-15 look through the V tiles that not every row attends to all of (the diagonal, the
+// 10 (and 11, where rows come one by one) bring the items' rows of Q; 12-15 look through the V tiles that not every row attends to all of (the diagonal, the
 // sequence's end): rows past the end become zeros, elements that are not finite are taken out and noted, see fst_chunk.cuh.
 // All hand-offs are mbarriers, the CTA's items follow one another without a break: Q of the next item arrives while the last
 // tile of the one before is in the softmax.  Every wait is bounded; on expiry FST_DEV_TIMEOUT is recorded and
